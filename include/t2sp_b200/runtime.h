@@ -71,7 +71,8 @@ enum halide_error_code_t {
 
 /* ---- element types accepted --------------------------------------------------------
  * fp32 in / fp32 out (the reference's only type: type word 73730, syrk-interface.cpp:149);
- * additionally bf16 or f16 in / fp32 out and int8 in / int32 out for GEMM.            */
+ * additionally bf16 or f16 in / fp32 out and int8 in / int32 out for GEMM; the grouped and the 4-bit
+ * products take bf16 or f16 and give that type or fp32.                               */
 
 /* How fp32 inputs are multiplied on the tensor cores. */
 enum t2sp_precision {
@@ -191,6 +192,49 @@ typedef struct t2sp_mttkrp_desc {
 } t2sp_mttkrp_desc;
 int t2sp_b200_mttkrp(halide_buffer_t *a, halide_buffer_t *b, halide_buffer_t *c, halide_buffer_t *d,
                      const t2sp_mttkrp_desc *desc);
+
+/* ---- Products grouped by expert (no counterpart in the reference) ---------------------------
+ * Rows sorted by group, one matrix for each group:
+ *   C(n,t) = sum_k A(k,t) * B(n,k,e)   for offsets(e) <= t < offsets(e+1)
+ * A: 2-D (K, M), B: 3-D (N, K, E) or, with trans_b, (K, N, E) with k innermost, offsets: 1-D (E+1) int32,
+ * C: 2-D (N, M). bf16 or f16 operands; C has their type (rounded once) or fp32. Sums are fp32.
+ * With B stored as the forward product reads it, the gradient of A is the same call with trans_b flipped.
+ * Rows outside every group (before offsets(0), from offsets(E) on) are neither read into a result nor written; groups may be
+ * empty. E <= 1024. The offsets are read on the device only: values that decrease or leave 0..M make the kernel
+ * compute nothing and report halide_error_code_access_out_of_bounds (for asynchronous calls at t2sp_b200_sync).
+ *   grouped_gemm_grad: the gradient of B, G(n,k,e) = sum over the rows t of group e of A(k,t) * D(n,t);
+ * D: 2-D (N, M), G: 3-D (N, K, E), zeros for an empty group. For a B with trans_b, exchange A and D.
+ * Strides: innermost 1, outer ones positive, outputs without overlap. Operands whose base and outer strides are multiples
+ * of 16 bytes are read in place; others are first copied into scratch memory, which a captured stream refuses
+ * (halide_error_code_constraint_violated). */
+typedef struct t2sp_grouped_desc {
+    int32_t trans_b;
+} t2sp_grouped_desc;
+int t2sp_b200_grouped_gemm(halide_buffer_t *A, halide_buffer_t *B, halide_buffer_t *offsets, halide_buffer_t *C,
+                           const t2sp_grouped_desc *desc);
+int t2sp_b200_grouped_gemm_grad(halide_buffer_t *A, halide_buffer_t *D, halide_buffer_t *offsets, halide_buffer_t *G);
+
+/* ---- Products of a few rows with 4-bit matrices (no counterpart in the reference) ------------
+ *   q4_pack    W -> (Q, S): for `group` consecutive k of one n, s = max|w| / 7 rounded to W's type and
+ *              q = w / s rounded to the nearest of -7..7 (ties to even). A group of zeros has s = 0; a group that holds a NaN
+ *              or an infinity has a scale that is not finite, and products with it are not finite.
+ *   q4_unpack  (Q, S) -> W = q * s, rounded to W's type.
+ *   q4_gemv    Y(n,r) = sum_k X(k, r / (R/T)) * q(n,k,e) * s(n,k,e), e = index(r); products with the integers are
+ *              summed in fp32 within a group and scaled in fp32.
+ * W: 3-D (N, K, E) or, with trans_b, (K, N, E); bf16 or f16. Q: 4-D uint8 (512, ceil(K/64), ceil(N/16), E), S: 4-D of W's
+ * type (16, groups, ceil(N/16), E), both dense and in an order of the library's own (a bounds query on Q and S
+ * gives their shapes; Q 16-byte aligned). X: 2-D (K, T), Y: 2-D (N, R) with R a multiple of T, of X's type or fp32;
+ * X and S have one type. index: 1-D (R) int32, or NULL with E = 1. A row with a negative index is left as it was; an index
+ * of E or more leaves the row as it was and reports halide_error_code_access_out_of_bounds (for asynchronous calls
+ * at t2sp_b200_sync). For many rows, q4_unpack and grouped_gemm are faster. */
+typedef struct t2sp_q4_desc {
+    int32_t group;   /* 32, 64 or 128; 0 = 64 */
+    int32_t trans_b; /* W has k innermost (q4_gemv ignores it) */
+} t2sp_q4_desc;
+int t2sp_b200_q4_pack(halide_buffer_t *W, halide_buffer_t *Q, halide_buffer_t *S, const t2sp_q4_desc *desc);
+int t2sp_b200_q4_unpack(halide_buffer_t *Q, halide_buffer_t *S, halide_buffer_t *W, const t2sp_q4_desc *desc);
+int t2sp_b200_q4_gemv(halide_buffer_t *X, halide_buffer_t *Q, halide_buffer_t *S, halide_buffer_t *index, halide_buffer_t *Y,
+                      const t2sp_q4_desc *desc);
 
 /* ---- MTTKRP without any allocation ---------------------------------------------------
  * No counterpart in the reference (its runtime allocates per call,

@@ -1,5 +1,6 @@
 """B200-native replacement for the host interface and device kernels that T2SP generates for
-its dense-tensor workloads (GEMM, 2-D convolution, capsule convolution, TTM, MTTKRP).
+its dense-tensor workloads (GEMM, 2-D convolution, capsule convolution, TTM, MTTKRP), with products grouped by
+expert and products with 4-bit matrices beside them.
 
 The product is the C ABI in include/t2sp_b200/runtime.h, served by libt2sp_b200.so (CUDA,
 sm_100a). This package only loads that library and mirrors its entry points for Python
@@ -40,6 +41,14 @@ class MttkrpDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("precision", "splits")]
 
 
+class GroupedDesc(ctypes.Structure):
+    _fields_ = [("trans_b", ctypes.c_int32)]
+
+
+class Q4Desc(ctypes.Structure):
+    _fields_ = [("group", ctypes.c_int32), ("trans_b", ctypes.c_int32)]
+
+
 ERROR_NAMES = {
     0: "success", -1: "generic_error", -3: "bad_type", -4: "access_out_of_bounds",
     -5: "buffer_allocation_too_large", -6: "buffer_extents_too_large", -8: "constraint_violated",
@@ -62,6 +71,11 @@ def lib():
         P = ctypes.c_void_p
         for name, nargs in (("t2sp_b200_gemm", 4), ("t2sp_b200_conv", 4), ("t2sp_b200_capsule", 4),
                             ("t2sp_b200_ttm", 4), ("t2sp_b200_mttkrp", 5)):
+            fn = getattr(L, name)
+            fn.argtypes = [P] * nargs
+            fn.restype = ctypes.c_int
+        for name, nargs in (("t2sp_b200_grouped_gemm", 5), ("t2sp_b200_grouped_gemm_grad", 4), ("t2sp_b200_q4_pack", 4),
+                            ("t2sp_b200_q4_unpack", 4), ("t2sp_b200_q4_gemv", 6)):
             fn = getattr(L, name)
             fn.argtypes = [P] * nargs
             fn.restype = ctypes.c_int
@@ -149,6 +163,32 @@ def ttm(a, b, c, desc=None):
 def mttkrp(a, b, c, d, desc=None):
     """d(i,r) = sum_k (sum_l a(l,i,k) c(l,r)) b(k,r) (t2s/tests/correctness/util/util.h:464-481)."""
     return lib().t2sp_b200_mttkrp(a.ptr, b.ptr, c.ptr, d.ptr, _opt(desc))
+
+
+def grouped_gemm(A, B, offsets, C, desc=None):
+    """C(n,t) = sum_k A(k,t) B(n,k,e) for the rows offsets(e) <= t < offsets(e+1) of group e; with `desc.trans_b` B is
+    (K, N, E). Returns the halide error code."""
+    return lib().t2sp_b200_grouped_gemm(A.ptr, B.ptr, offsets.ptr, C.ptr, _opt(desc))
+
+
+def grouped_gemm_grad(A, D, offsets, G):
+    """G(n,k,e) = sum over the rows t of group e of A(k,t) D(n,t): the gradient of grouped_gemm's B."""
+    return lib().t2sp_b200_grouped_gemm_grad(A.ptr, D.ptr, offsets.ptr, G.ptr)
+
+
+def q4_pack(W, Q, S, desc=None):
+    """Quantises the matrices W(n,k,e) to 4 bits with a scale for every `desc.group` values along k."""
+    return lib().t2sp_b200_q4_pack(W.ptr, Q.ptr, S.ptr, _opt(desc))
+
+
+def q4_unpack(Q, S, W, desc=None):
+    """W(n,k,e) = the values that the packed matrices stand for, rounded to W's type."""
+    return lib().t2sp_b200_q4_unpack(Q.ptr, S.ptr, W.ptr, _opt(desc))
+
+
+def q4_gemv(X, Q, S, index, Y, desc=None):
+    """Y(n,r) = sum_k X(k, r / (R/T)) W(n,k,index(r)) with the packed W; `index` is None for a single matrix."""
+    return lib().t2sp_b200_q4_gemv(X.ptr, Q.ptr, S.ptr, index.ptr if index is not None else None, Y.ptr, _opt(desc))
 
 
 def wrap_device(buf, device_ptr):

@@ -224,14 +224,20 @@ int rt_check_status(const char* who) {
         return halide_error_code_device_run_failed;
     }
     if (*d.status_host != 0) {
-        fprintf(stderr, "t2sp_b200: %s: a kernel gave up waiting (status 0x%x: %s%s%s%s)\n", who, *d.status_host,
-                (*d.status_host & ST_TIMEOUT_PRODUCER) ? "producer " : "", (*d.status_host & ST_TIMEOUT_MMA) ? "mma " : "",
-                (*d.status_host & ST_TIMEOUT_EPILOGUE) ? "epilogue " : "",
-                (*d.status_host & ST_TIMEOUT_SPLITTER) ? "splitter " : "");
+        const unsigned st = *d.status_host;
+        if (st & (ST_TIMEOUT_PRODUCER | ST_TIMEOUT_MMA | ST_TIMEOUT_EPILOGUE | ST_TIMEOUT_SPLITTER))
+            fprintf(stderr, "t2sp_b200: %s: a kernel gave up waiting (status 0x%x: %s%s%s%s)\n", who, st,
+                    (st & ST_TIMEOUT_PRODUCER) ? "producer " : "", (st & ST_TIMEOUT_MMA) ? "mma " : "",
+                    (st & ST_TIMEOUT_EPILOGUE) ? "epilogue " : "", (st & ST_TIMEOUT_SPLITTER) ? "splitter " : "");
+        if (st & ST_BAD_OFFSETS)
+            fprintf(stderr, "t2sp_b200: %s: the group offsets decrease or lie outside the rows; nothing was computed\n", who);
+        if (st & ST_BAD_INDEX)
+            fprintf(stderr, "t2sp_b200: %s: a row names a matrix beyond the last one; the row was left as it was\n", who);
+        const bool only_values = (st & ~(ST_BAD_OFFSETS | ST_BAD_INDEX)) == 0;
         cudaMemsetAsync(d.status_dev, 0, sizeof(unsigned), s);
         cudaStreamSynchronize(s);
         *d.status_host = 0;
-        return halide_error_code_device_run_failed;
+        return only_values ? halide_error_code_access_out_of_bounds : halide_error_code_device_run_failed;
     }
     return 0;
 }

@@ -1,0 +1,185 @@
+// Entry points of the grouped products: argument validation in the order of the other entries (ops.cpp), then one
+// launch over the rows of all groups. The group boundaries stay on the device: nothing here reads them.
+#include "grouped.h"
+#include "op_common.h"
+
+using namespace t2sp;
+
+namespace t2sp {
+namespace {
+
+int check_offsets(const Arg& a) {
+    if (a.b->dim[0].extent < 1) return constraint("offsets.extent.0", a.b->dim[0].extent, "groups + 1", 1);
+    if (a.b->dim[0].extent > kMaxGroups + 1)
+        return constraint("offsets.extent.0", a.b->dim[0].extent, "at most groups + 1", kMaxGroups + 1);
+    return 0;
+}
+
+// Launch with the timing and the error report of the other operators.
+int run_grouped(const char* who, GroupedParams& p, bool sync_after) {
+    cudaStream_t s = rt_stream();
+    p.status = rt_status_word();
+    if (sync_after) cudaEventRecord(rt_event(0), s);
+    const cudaError_t e = grouped_launch(p, s);
+    if (e != cudaSuccess) {
+        fprintf(stderr, "t2sp_b200: %s: kernel launch failed: %s\n", who, cudaGetErrorString(e));
+        return halide_error_code_device_run_failed;
+    }
+    rt_count_launch(1);
+    if (sync_after) cudaEventRecord(rt_event(1), s);
+    return 0;
+}
+
+}  // namespace
+}  // namespace t2sp
+
+extern "C" int t2sp_b200_grouped_gemm(halide_buffer_t* A, halide_buffer_t* B, halide_buffer_t* offsets, halide_buffer_t* C,
+                                      const t2sp_grouped_desc* desc) {
+    Arg args[4] = {{A, "A", false, 2}, {B, "B", false, 3}, {offsets, "offsets", false, 1}, {C, "C", true, 2}};
+    if (int e = check_null(args, 4)) return e;
+    const int tb = desc && desc->trans_b ? 1 : 0;
+    if (buf_is_bounds_query(A) || buf_is_bounds_query(B) || buf_is_bounds_query(offsets) || buf_is_bounds_query(C)) {
+        int K = 0, M = 0, N = 0, E = 0;
+        if (!buf_is_bounds_query(A) && A->dimensions == 2) { K = A->dim[0].extent; M = A->dim[1].extent; }
+        if (!buf_is_bounds_query(B) && B->dimensions == 3) {
+            N = B->dim[tb ? 1 : 0].extent;
+            E = B->dim[2].extent;
+            if (!K) K = B->dim[tb ? 0 : 1].extent;
+        }
+        if (!buf_is_bounds_query(offsets) && offsets->dimensions == 1 && !E) E = offsets->dim[0].extent - 1;
+        if (!buf_is_bounds_query(C) && C->dimensions == 2) {
+            if (!N) N = C->dim[0].extent;
+            if (!M) M = C->dim[1].extent;
+        }
+        const uint32_t t = !buf_is_bounds_query(A) ? buf_type_word(A) : (!buf_is_bounds_query(B) ? buf_type_word(B) : kBF16);
+        if (buf_is_bounds_query(A)) { int x[2] = {K, M}; fill_query(A, t, 2, x); }
+        if (buf_is_bounds_query(B)) { int x[3] = {tb ? K : N, tb ? N : K, E}; fill_query(B, t, 3, x); }
+        if (buf_is_bounds_query(offsets)) { int x[1] = {E + 1}; fill_query(offsets, kI32, 1, x); }
+        if (buf_is_bounds_query(C)) { int x[2] = {N, M}; fill_query(C, t, 2, x); }
+        return 0;
+    }
+    const uint32_t in_t = buf_type_word(A);
+    if (in_t != kBF16 && in_t != kF16) return halide_error_bad_type(nullptr, args[0].role().c_str(), in_t, kBF16);
+    const bool out_f32 = buf_type_word(C) == kF32;
+    if (int e = check_type_dims(args[0], in_t)) return e;
+    if (int e = check_type_dims(args[1], in_t)) return e;
+    if (int e = check_type_dims(args[2], kI32)) return e;
+    if (int e = check_type_dims(args[3], out_f32 ? kF32 : in_t)) return e;
+    for (auto& a : args)
+        if (int e = check_extents_nonneg(a)) return e;
+    const int K = A->dim[0].extent, M = A->dim[1].extent, N = B->dim[tb ? 1 : 0].extent, E = B->dim[2].extent;
+    if (B->dim[tb ? 0 : 1].extent != K)
+        return constraint(tb ? "B.extent.0" : "B.extent.1", B->dim[tb ? 0 : 1].extent, "A.extent.0", K);
+    if (int e = check_offsets(args[2])) return e;
+    if (offsets->dim[0].extent != E + 1) return constraint("offsets.extent.0", offsets->dim[0].extent, "B.extent.2 + 1", E + 1);
+    for (int i = 0; i < 3; ++i)
+        if (int e = check_min0(args[i])) return e;
+    if (int e = check_covers(args[3], 0, N)) return e;
+    if (int e = check_covers(args[3], 1, M)) return e;
+    for (auto& a : args)
+        if (int e = check_stride0(a)) return e;
+    for (auto& a : args)
+        if (int e = check_strides(a)) return e;
+    for (auto& a : args)
+        if (int e = check_sizes(a)) return e;
+    for (auto& a : args)
+        if (int e = check_host(a)) return e;
+    if (M == 0 || N == 0 || E == 0) return 0;
+
+    if (int e = rt_ensure_device()) return e;
+    const bool sync_after = !(all_resident({A, B, offsets, C}) && tls().async);
+    if (int e = check_capture("grouped_gemm", sync_after, false)) return e;
+    Views vw;
+    for (int i = 0; i < 3; ++i, ++vw.n)
+        if (int e = rt_input_view(args[i].b, args[i].name, &vw.v[vw.n])) return e;
+    if (int e = rt_output_view(C, "C", &vw.v[vw.n])) return e;
+    vw.n++;
+    if (int e = preload_output(C, &vw.v[3])) return e;   // rows outside the groups keep their values
+    GroupedParams p = {};
+    p.a = vw.v[0].ptr;
+    p.b = vw.v[1].ptr;
+    p.offsets = static_cast<const int*>(vw.v[2].ptr);
+    p.c = static_cast<char*>(vw.v[3].ptr) + origin_offset(C) * (out_f32 ? 4 : 2);
+    p.lda = A->dim[1].stride;
+    p.ldb = B->dim[1].stride;
+    p.bs_b = B->dim[2].stride;
+    p.ldc = C->dim[1].stride;
+    p.rows = M; p.E = E; p.K = K; p.N = N;
+    p.trans_b = tb; p.bf16 = in_t == kBF16; p.out_f32 = out_f32;
+    if (int e = run_grouped("grouped_gemm", p, sync_after)) return e;
+    if (int e = rt_finish_output(C, "C", &vw.v[3])) return e;
+    return finish_call("grouped_gemm", "kernel_Out", sync_after);
+}
+
+extern "C" int t2sp_b200_grouped_gemm_grad(halide_buffer_t* A, halide_buffer_t* D, halide_buffer_t* offsets, halide_buffer_t* G) {
+    Arg args[4] = {{A, "A", false, 2}, {D, "D", false, 2}, {offsets, "offsets", false, 1}, {G, "G", true, 3}};
+    if (int e = check_null(args, 4)) return e;
+    if (buf_is_bounds_query(A) || buf_is_bounds_query(D) || buf_is_bounds_query(offsets) || buf_is_bounds_query(G)) {
+        int K = 0, M = 0, N = 0, E = 0;
+        if (!buf_is_bounds_query(A) && A->dimensions == 2) { K = A->dim[0].extent; M = A->dim[1].extent; }
+        if (!buf_is_bounds_query(D) && D->dimensions == 2) { N = D->dim[0].extent; if (!M) M = D->dim[1].extent; }
+        if (!buf_is_bounds_query(G) && G->dimensions == 3) {
+            if (!N) N = G->dim[0].extent;
+            if (!K) K = G->dim[1].extent;
+            E = G->dim[2].extent;
+        }
+        if (!buf_is_bounds_query(offsets) && offsets->dimensions == 1 && !E) E = offsets->dim[0].extent - 1;
+        const uint32_t t = !buf_is_bounds_query(A) ? buf_type_word(A) : (!buf_is_bounds_query(D) ? buf_type_word(D) : kBF16);
+        if (buf_is_bounds_query(A)) { int x[2] = {K, M}; fill_query(A, t, 2, x); }
+        if (buf_is_bounds_query(D)) { int x[2] = {N, M}; fill_query(D, t, 2, x); }
+        if (buf_is_bounds_query(offsets)) { int x[1] = {E + 1}; fill_query(offsets, kI32, 1, x); }
+        if (buf_is_bounds_query(G)) { int x[3] = {N, K, E}; fill_query(G, t, 3, x); }
+        return 0;
+    }
+    const uint32_t in_t = buf_type_word(A);
+    if (in_t != kBF16 && in_t != kF16) return halide_error_bad_type(nullptr, args[0].role().c_str(), in_t, kBF16);
+    const bool out_f32 = buf_type_word(G) == kF32;
+    if (int e = check_type_dims(args[0], in_t)) return e;
+    if (int e = check_type_dims(args[1], in_t)) return e;
+    if (int e = check_type_dims(args[2], kI32)) return e;
+    if (int e = check_type_dims(args[3], out_f32 ? kF32 : in_t)) return e;
+    for (auto& a : args)
+        if (int e = check_extents_nonneg(a)) return e;
+    const int K = A->dim[0].extent, M = A->dim[1].extent, N = D->dim[0].extent;
+    if (D->dim[1].extent != M) return constraint("D.extent.1", D->dim[1].extent, "A.extent.1", M);
+    if (int e = check_offsets(args[2])) return e;
+    const int E = offsets->dim[0].extent - 1;
+    for (int i = 0; i < 3; ++i)
+        if (int e = check_min0(args[i])) return e;
+    if (int e = check_covers(args[3], 0, N)) return e;
+    if (int e = check_covers(args[3], 1, K)) return e;
+    if (int e = check_covers(args[3], 2, E)) return e;
+    for (auto& a : args)
+        if (int e = check_stride0(a)) return e;
+    for (auto& a : args)
+        if (int e = check_strides(a)) return e;
+    for (auto& a : args)
+        if (int e = check_sizes(a)) return e;
+    for (auto& a : args)
+        if (int e = check_host(a)) return e;
+    if (K == 0 || N == 0 || E == 0) return 0;
+
+    if (int e = rt_ensure_device()) return e;
+    const bool sync_after = !(all_resident({A, D, offsets, G}) && tls().async);
+    if (int e = check_capture("grouped_gemm_grad", sync_after, false)) return e;
+    Views vw;
+    for (int i = 0; i < 3; ++i, ++vw.n)
+        if (int e = rt_input_view(args[i].b, args[i].name, &vw.v[vw.n])) return e;
+    if (int e = rt_output_view(G, "G", &vw.v[vw.n])) return e;
+    vw.n++;
+    if (int e = preload_output(G, &vw.v[3])) return e;   // what G holds beyond (N, K, E) keeps its values
+    GroupedParams p = {};
+    p.a = vw.v[0].ptr;
+    p.b = vw.v[1].ptr;
+    p.offsets = static_cast<const int*>(vw.v[2].ptr);
+    p.c = static_cast<char*>(vw.v[3].ptr) + origin_offset(G) * (out_f32 ? 4 : 2);
+    p.lda = A->dim[1].stride;
+    p.ldb = D->dim[1].stride;
+    p.ldc = G->dim[1].stride;
+    p.bs_c = G->dim[2].stride;
+    p.rows = M; p.E = E; p.K = K; p.N = N;
+    p.grad = 1; p.bf16 = in_t == kBF16; p.out_f32 = out_f32;
+    if (int e = run_grouped("grouped_gemm_grad", p, sync_after)) return e;
+    if (int e = rt_finish_output(G, "G", &vw.v[3])) return e;
+    return finish_call("grouped_gemm_grad", "kernel_Out", sync_after);
+}

@@ -16,6 +16,9 @@ enum : unsigned {
     ST_TIMEOUT_MMA = 2u,
     ST_TIMEOUT_EPILOGUE = 4u,
     ST_TIMEOUT_SPLITTER = 8u,
+    // bits that name bad values in an index operand; the kernel has skipped what they address
+    ST_BAD_OFFSETS = 16u,  // group offsets that decrease or leave the rows
+    ST_BAD_INDEX = 32u,    // a row's matrix number beyond the last matrix
 };
 
 constexpr long long kWaitTimeoutCycles = 4000000000ll;  // SM cycles: 2 s at 1965 MHz, 4 s at 1 GHz

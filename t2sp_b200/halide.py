@@ -28,9 +28,9 @@ assert ctypes.sizeof(HalideBuffer) == 56 and ctypes.sizeof(HalideDimension) == 1
 
 DTYPES = {
     "f32": (TYPE_FLOAT, 32), "bf16": (TYPE_BFLOAT, 16), "f16": (TYPE_FLOAT, 16),
-    "i8": (TYPE_INT, 8), "i32": (TYPE_INT, 32), "f64": (TYPE_FLOAT, 64),
+    "i8": (TYPE_INT, 8), "u8": (TYPE_UINT, 8), "i32": (TYPE_INT, 32), "f64": (TYPE_FLOAT, 64),
 }
-_NP = {np.dtype(np.float32): "f32", np.dtype(np.float16): "f16", np.dtype(np.int8): "i8",
+_NP = {np.dtype(np.float32): "f32", np.dtype(np.float16): "f16", np.dtype(np.int8): "i8", np.dtype(np.uint8): "u8",
        np.dtype(np.int32): "i32", np.dtype(np.float64): "f64"}
 
 

@@ -1,0 +1,279 @@
+"""4-bit matrices on the GPU: quantising and reading back exactly as the definition in 64 bits says, products with a few rows
+against 64-bit products of the values that the integers stand for.
+
+Tolerance of a product: its final rounding (half a step of its type) and the fp32 sums: within a group
+(group / 16 + 16) * 2^-23 and over the groups (groups + 16) * 2^-23, of sum |x||w|."""
+import numpy as np
+import pytest
+
+import t2sp_b200
+from t2sp_b200 import Buffer, GroupedDesc, Q4Desc
+from tests.device_util import buf, eps_half, on_stream, packed, quantised64
+
+pytestmark = pytest.mark.gpu
+
+
+def matrices(E, K, N, dtype, seed=0, scale=1.0):
+    import torch
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return (torch.randn(E, K, N, generator=g, device="cuda") * scale).to(dtype)
+
+
+def unpacked(Q, S, like, group, trans=False):
+    import torch
+    w = torch.full_like(like, float("nan"))
+    assert t2sp_b200.q4_unpack(buf(Q), buf(S), buf(w), Q4Desc(group, int(trans))) == 0
+    return w
+
+
+def check_rows(x, values, index, y, group, untouched=None):
+    """values: (E, K, N) in 64 bits; index: a list, or None."""
+    import torch
+    R, K = y.shape[0], x.shape[1]
+    per = R // x.shape[0]
+    index = index if index is not None else [0] * R
+    for r in range(R):
+        if not 0 <= index[r] < values.shape[0]:
+            assert torch.equal(y[r], untouched[r])
+            continue
+        v, w = x[r // per].double(), values[index[r]]
+        ref, mag = v @ w, v.abs() @ w.abs()
+        tol = ((group // 16 + 16) + (K // group + 16)) * 2.0 ** -23 * mag + 1e-30
+        if y.dtype != torch.float32:
+            tol = tol * (1 + eps_half(y.dtype)) + eps_half(y.dtype) * ref.abs() + (2.0 ** -25 if y.dtype == torch.float16 else 0)
+        bad = ~((y[r].double() - ref).abs() <= tol)
+        assert not bad.any(), (r, int(bad.sum()), bad.nonzero()[:4].tolist())
+
+
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("E,K,N,group", [(1, 64, 16, 64), (2, 100, 40, 32), (1, 1, 1, 128), (3, 130, 70, 128), (1, 1001, 777, 64),
+                                         (2, 256, 128, 32), (1, 192, 33, 128), (5, 63, 17, 32)])
+def test_pack_and_unpack_exactly(lib, E, K, N, group, dtype, trans):
+    import torch
+    dt = getattr(torch, dtype)
+    w = matrices(E, K, N, dt, seed=K + N)
+    w[:, : K // 3] *= 0.01
+    stored = w.transpose(1, 2).contiguous() if trans else w
+    with on_stream():
+        Q, S = packed(stored, group, trans)
+        back = unpacked(Q, S, stored, group, trans)
+    want = quantised64(w, group).to(dt)
+    assert torch.equal(back.transpose(1, 2) if trans else back, want)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_pack_borders(lib, dtype):
+    """Ties, zeros, the smallest and the largest values of the type."""
+    import torch
+    dt = getattr(torch, dtype)
+    fi = torch.finfo(dt)
+    w = torch.zeros(1, 64, 48, device="cuda")
+    w[0, :, 0] = torch.arange(64) % 15 - 7                     # scale 1: integers and ...
+    w[0, :, 1] = (torch.arange(64) % 28 - 14) / 2              # ... halves, ties to even
+    w[0, :, 2] = 0
+    w[0, 5, 3] = -7
+    w[0, :, 4] = fi.max
+    w[0, :, 5] = fi.smallest_normal
+    w[0, :, 6] = fi.smallest_normal * fi.eps                   # the smallest subnormal number: the scale rounds to zero or not
+    w[0, ::2, 7] = fi.smallest_normal * fi.eps * 9
+    w[0, :, 8] = -torch.arange(64, device="cuda") * fi.smallest_normal / 8
+    w = w.to(dt)
+    with on_stream():
+        Q, S = packed(w, 64)
+        back = unpacked(Q, S, w, 64)
+    assert torch.equal(back, quantised64(w, 64).to(dt))
+
+
+def test_pack_infinities_and_nan(lib):
+    """A group with a value that is not finite reads back as nothing finite; the others are as ever."""
+    import torch
+    w = matrices(1, 128, 40, torch.bfloat16)
+    bad = w.clone()
+    bad[0, 3, 7] = float("nan"); bad[0, 70, 8] = float("inf"); bad[0, 71, 39] = -float("inf")
+    x = torch.ones(1, 128, dtype=torch.bfloat16, device="cuda")
+    y = torch.zeros(1, 40, dtype=torch.float32, device="cuda")
+    with on_stream():
+        Q, S = packed(bad, 64)
+        back = unpacked(Q, S, bad, 64)
+        assert t2sp_b200.q4_gemv(buf(x), buf(Q), buf(S), None, buf(y), Q4Desc(64, 0)) == 0
+    want = quantised64(w, 64).to(torch.bfloat16)
+    hit = torch.zeros(1, 128, 40, dtype=torch.bool, device="cuda")
+    hit[0, :64, 7] = hit[0, 64:, 8] = hit[0, 64:, 39] = True
+    assert not back[hit].isfinite().any() and torch.equal(back[~hit], want[~hit])
+    columns = hit.any(1)[0]
+    assert not y[0][columns].isfinite().any() and y[0][~columns].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("R,K,N,group", [(1, 64, 16, 64), (1, 1, 1, 32), (1, 4096, 520, 64), (2, 100, 40, 32), (7, 1001, 777, 32), (8, 512, 48, 128),
+                                         (9, 130, 33, 128), (17, 192, 64, 64), (33, 256, 80, 32), (70, 64, 17, 64), (3, 8200, 24, 128)])
+def test_gemv_one_matrix(lib, R, K, N, group, dtype):
+    import torch
+    dt = getattr(torch, dtype)
+    w, x = matrices(1, K, N, dt, 1), matrices(1, R, K, dt, 2)[0]
+    with on_stream():
+        Q, S = packed(w, group)
+        for out in (dt, torch.float32):
+            y = torch.full((R, N), float("nan"), dtype=out, device="cuda")
+            assert t2sp_b200.q4_gemv(buf(x), buf(Q), buf(S), None, buf(y), Q4Desc(group, 0)) == 0
+            check_rows(x, quantised64(w, group), None, y, group)
+
+
+@pytest.mark.parametrize("E,T,per,K,N,group", [(4, 3, 2, 128, 64, 32), (64, 8, 2, 512, 96, 64), (3, 40, 1, 96, 40, 32), (5, 1, 1, 1000, 24, 128),
+                                               (2, 30, 4, 70, 35, 64), (200, 70, 4, 64, 16, 64)])
+def test_gemv_by_expert(lib, E, T, per, K, N, group):
+    import torch
+    dt = torch.bfloat16
+    w, x = matrices(E, K, N, dt, 1), matrices(1, T, K, dt, 2)[0]
+    R = T * per
+    rng = np.random.default_rng(E)
+    index = rng.integers(0, E, R)
+    index[rng.random(R) < 0.2] = -1            # rows without an expert
+    index[0] = E - 1
+    idx = torch.tensor(index, dtype=torch.int32, device="cuda")
+    y = torch.full((R, N), 7.0, dtype=dt, device="cuda")
+    with on_stream():
+        Q, S = packed(w, group)
+        assert t2sp_b200.q4_gemv(buf(x), buf(Q), buf(S), buf(idx), buf(y), Q4Desc(group, 0)) == 0
+    check_rows(x, quantised64(w, group), index.tolist(), y, group, torch.full_like(y, 7.0))
+
+
+def test_gemv_all_rows_without_or_with_one_expert(lib):
+    import torch
+    w, x = matrices(3, 64, 32, torch.float16, 1), matrices(1, 20, 64, torch.float16, 2)[0]
+    with on_stream():
+        Q, S = packed(w, 64)
+        for value in (-1, 2):
+            idx = torch.full((20,), value, dtype=torch.int32, device="cuda")
+            y = torch.full((20, 32), 7.0, dtype=torch.float32, device="cuda")
+            assert t2sp_b200.q4_gemv(buf(x), buf(Q), buf(S), buf(idx), buf(y), Q4Desc(64, 0)) == 0
+            check_rows(x, quantised64(w, 64), [value] * 20, y, 64, torch.full_like(y, 7.0))
+
+
+def test_gemv_index_beyond_the_last_matrix(lib):
+    import torch
+    w, x = matrices(3, 64, 32, torch.bfloat16, 1), matrices(1, 4, 64, torch.bfloat16, 2)[0]
+    index = [0, 3, 2 ** 31 - 1, 1]
+    idx = torch.tensor(index, dtype=torch.int32, device="cuda")
+    y = torch.full((4, 32), 7.0, dtype=torch.bfloat16, device="cuda")
+    with on_stream():
+        Q, S = packed(w, 64)
+        assert t2sp_b200.q4_gemv(buf(x), buf(Q), buf(S), buf(idx), buf(y), Q4Desc(64, 0)) == -4
+        check_rows(x, quantised64(w, 64), index, y, 64, torch.full_like(y, 7.0))
+    with on_stream(asynchronous=True) as L:
+        assert t2sp_b200.q4_gemv(buf(x), buf(Q), buf(S), buf(idx), buf(y), Q4Desc(64, 0)) == 0
+        assert L.t2sp_b200_sync() == -4 and L.t2sp_b200_sync() == 0
+
+
+@pytest.mark.parametrize("first,pad", [(0, 8), (1, 0), (1, 3), (8, 5)])
+def test_gemv_strides(lib, first, pad):
+    """Rows of x and y with a pitch, starting inside an allocation; what lies between the rows stays."""
+    import torch
+    R, K, N, group = 5, 200, 56, 64
+    w = matrices(1, K, N, torch.bfloat16, 1)
+    x0 = matrices(1, R, K, torch.bfloat16, 2)[0]
+    bx = torch.full((R * (K + pad) + 64,), float("nan"), dtype=torch.bfloat16, device="cuda")
+    by = torch.full((R * (N + pad) + 64,), 9.0, dtype=torch.bfloat16, device="cuda")
+    x = bx[first:].as_strided((R, K), (K + pad, 1))
+    y = by[first:].as_strided((R, N), (N + pad, 1))
+    x.copy_(x0)
+    y.zero_()
+    with on_stream():
+        Q, S = packed(w, group)
+        assert t2sp_b200.q4_gemv(buf(x), buf(Q), buf(S), None, buf(y), Q4Desc(group, 0)) == 0
+    check_rows(x0, quantised64(w, group), None, y, group)
+    y.fill_(9.0)
+    assert (by == 9).all()
+
+
+def test_pack_strides(lib):
+    """Matrices that are parts of a larger tensor, both ways round."""
+    import torch
+    big = matrices(3, 90, 70, torch.float16, 4)
+    part = big[1:3, 5:83, 3:60]
+    for trans in (False, True):
+        stored = part if not trans else big.transpose(1, 2).contiguous().transpose(1, 2)[1:3, 5:83, 3:60].transpose(1, 2)
+        with on_stream():
+            Q, S = packed(stored, 32, trans)
+            out = torch.full((3, 80, 80), 5.0, dtype=torch.float16, device="cuda")
+            view = out[:2, 1:1 + stored.shape[1], 2:2 + stored.shape[2]]
+            assert t2sp_b200.q4_unpack(buf(Q), buf(S), buf(view), Q4Desc(32, int(trans))) == 0
+        want = quantised64(part, 32).half()
+        assert torch.equal(view.transpose(1, 2) if trans else view, want)
+        view.fill_(5.0)
+        assert (out == 5).all()
+
+
+def test_gemv_empty_contraction(lib):
+    import torch
+    y = torch.full((2, 24), 7.0, dtype=torch.bfloat16, device="cuda")
+    X = Buffer((0, 2), "bf16", host=y.data_ptr())
+    Q = Buffer((512, 0, 2, 1), "u8", host=y.data_ptr())
+    S = Buffer((16, 0, 2, 1), "bf16", host=y.data_ptr())
+    with on_stream():
+        assert t2sp_b200.q4_gemv(X, Q, S, None, buf(y), Q4Desc(64, 0)) == 0
+    assert not y.any()
+
+
+def test_host_buffers(lib):
+    import torch
+    w = matrices(2, 70, 20, torch.float16, 3)
+    x = matrices(1, 3, 70, torch.float16, 4)[0]
+    W, X = Buffer.from_numpy(w.cpu().numpy()), Buffer.from_numpy(x.cpu().numpy())
+    q, s = Buffer.query(4, "u8"), Buffer.query(4, "f16")
+    assert t2sp_b200.q4_pack(W, q, s, Q4Desc(32, 0)) == 0
+    Q = Buffer.from_numpy(np.zeros([e for _, e, _ in reversed(q.shape())], np.uint8))
+    S = Buffer.from_numpy(np.zeros([e for _, e, _ in reversed(s.shape())], np.float16))
+    Y = Buffer.from_numpy(np.full((3, 20), 7.0, np.float32))
+    assert t2sp_b200.q4_pack(W, Q, S, Q4Desc(32, 0)) == 0
+    assert t2sp_b200.q4_gemv(X, Q, S, Buffer.from_numpy(np.array([1, -1, 0], np.int32)), Y, Q4Desc(32, 0)) == 0
+    y = torch.from_numpy(Y.keepalive).cuda()
+    check_rows(x, quantised64(w, 32), [1, -1, 0], y, 32, torch.full_like(y, 7.0))
+
+
+def test_experts_of_a_layer_together(lib):
+    """A layer's experts as a host program uses them: a training step with the grouped products, the weights quantised once, a prompt
+    with the values read back, and single tokens from the packed form, captured into a graph and replayed; both give the prompt's rows."""
+    import torch
+    E, K, N, group, dt = 6, 192, 320, 64, torch.bfloat16
+    w = matrices(E, K, N, dt, 1, K ** -0.5)
+    counts = [9, 0, 30, 1, 64, 12]
+    M = sum(counts)
+    off = torch.tensor(np.concatenate([[0], np.cumsum(counts)]), dtype=torch.int32, device="cuda")
+    x = matrices(1, M, K, dt, 2)[0]
+    d = matrices(1, M, N, dt, 3)[0]
+    dx, dw = torch.empty_like(x), torch.empty(E, K, N, dtype=torch.float32, device="cuda")
+    prompt = torch.empty(M, N, dtype=torch.float32, device="cuda")
+    with on_stream(asynchronous=True) as L:
+        assert t2sp_b200.grouped_gemm(buf(d), buf(w), buf(off), buf(dx), GroupedDesc(1)) == 0
+        assert t2sp_b200.grouped_gemm_grad(buf(x), buf(d), buf(off), buf(dw)) == 0
+        w -= (0.01 * dw).to(dt)                                        # on the same stream
+        Q, S = packed(w, group)
+        back = unpacked(Q, S, w, group)
+        assert t2sp_b200.grouped_gemm(buf(x), buf(back), buf(off), buf(prompt)) == 0
+        assert L.t2sp_b200_sync() == 0
+    expert = torch.repeat_interleave(torch.arange(E), torch.tensor(counts)).to(torch.int32).cuda()
+    pick = torch.tensor([M - 1, 0, 9, 39, 40, 38], device="cuda")
+    token, index = x[pick].contiguous(), expert[pick].contiguous()
+    y = torch.zeros(6, N, dtype=torch.float32, device="cuda")
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    T, I, Y, QB, SB = (buf(t) for t in (token, index, y, Q, S))
+    torch.cuda.synchronize()
+    with on_stream(side, asynchronous=True):
+        assert t2sp_b200.q4_gemv(T, QB, SB, I, Y, Q4Desc(group, 0)) == 0
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            rc = t2sp_b200.q4_gemv(T, QB, SB, I, Y, Q4Desc(group, 0))
+    assert rc == 0
+    for rows in (pick, torch.tensor([3, 50, 51, 100, 8, 7], device="cuda")):
+        token.copy_(x[rows])
+        index.copy_(expert[rows])
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_rows(token, quantised64(w, group), index.tolist(), y, group)
+        # the prompt used values rounded to bf16: half a step of 2^-8 of each product's magnitude
+        mag = torch.stack([token[i].double().abs() @ back[index[i]].double().abs() for i in range(6)])
+        assert ((y.double() - prompt[rows].double()).abs() <= mag * (eps_half(dt) + 64 * 2.0 ** -23)).all()
