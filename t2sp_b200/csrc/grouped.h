@@ -1,5 +1,6 @@
 // Products whose matrix depends on the row: parameter blocks and launchers (definitions in launch_grouped.cu).
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -9,24 +10,32 @@ namespace t2sp {
 
 constexpr int kMaxGroups = 1024;  // the kernels keep the groups' tables in shared memory
 
+enum : int { GR_FWD_MN = 0, GR_FWD_K = 1, GR_GRAD = 2 };  // B with n innermost, B with k innermost, gradient of B
+enum : int { GR_OUT_F32 = 0, GR_OUT_BF16 = 1, GR_OUT_F16 = 2 };
+
 // Forward: C[t][n] = sum_k A[t][k] * B[e][k][n] for offsets[e] <= t < offsets[e+1]; rows outside every group are not
 // touched. Gradient of B: G[e][k][n] = sum_{t in e} A[t][k] * D[t][n], zero for an empty group.
-// Strides in elements; the innermost stride of every operand is 1.
+// The inputs are read through tensor maps; strides in elements.
 struct GroupedParams {
-    const void* a;         // A: rows x K
-    const void* b;         // forward: B, E x K x N (trans_b: E x N x K); gradient: D, rows x N
     void* c;               // forward: C, rows x N; gradient: G, E x K x N
     const int* offsets;    // E + 1
-    long long lda, ldb, ldc;
-    long long bs_b, bs_c;  // strides between the matrices of B and of G
+    long long ldc, bs_c;   // row pitch of C or G, stride between the matrices of G
     int rows, E, K, N;
-    int trans_b;
-    int grad;
     int bf16;              // element type of the inputs: 1 bf16, 0 f16
-    int out_f32;           // output element: 1 fp32, 0 the inputs' type
+    long long wait_cycles; // limit of every mbarrier wait in SM cycles, 0: kWaitTimeoutCycles
     unsigned* status;
 };
 
-cudaError_t grouped_launch(const GroupedParams& p, cudaStream_t stream);
+struct GroupedMaps {
+    CUtensorMap p;      // B (n, k, e), box 64 x 64, or (k, n, e), box 64 k x 128 n; gradient: D (n, t, 1), box 64 x 64
+    CUtensorMap q;      // A: forward (k, t), 64 k x 128 rows a box; gradient (k, t), 64 k x 64 rows
+    CUtensorMap q16;    // forward: 16 rows a box, for tiles narrower than 256 rows
+};
+
+cudaError_t grouped_launch(int mode, int out, const GroupedParams& p, const GroupedMaps& maps, cudaStream_t stream);
+
+// dst[m][r][i] (row pitch ld_dst, dense matrices) = src[m * bs_src + r * ld_src + i], 16-bit elements; ld_dst is a multiple of 8.
+cudaError_t repack16_launch(const void* src, long long ld_src, long long bs_src, void* dst, long long ld_dst, int inner, int rows,
+                            int matrices, cudaStream_t stream);
 
 }  // namespace t2sp

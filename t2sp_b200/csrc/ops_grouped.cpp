@@ -15,12 +15,65 @@ int check_offsets(const Arg& a) {
     return 0;
 }
 
-// Launch with the timing and the error report of the other operators.
-int run_grouped(const char* who, GroupedParams& p, bool sync_after) {
+// A matrix operand as TMA reads it: 16-byte aligned base, strides that are multiples of 16 bytes.
+struct Operand {
+    char* ptr;
+    int64_t ld, bs;              // elements between rows and between matrices
+    int inner, rows, matrices;
+    bool fits() const {
+        return !(reinterpret_cast<uintptr_t>(ptr) & 15) && (rows <= 1 || ld % 8 == 0) && (matrices <= 1 || bs % 8 == 0);
+    }
+};
+
+// Copies an operand that TMA cannot read in place into scratch memory with padded rows.
+int fit_operand(Views& vw, Operand& o) {
+    if (o.inner == 0 || o.rows == 0 || o.matrices == 0 || o.fits()) return 0;
+    const int64_t ld = (int64_t(o.inner) + 7) / 8 * 8;
+    void* q = rt_alloc(size_t(ld) * o.rows * o.matrices * 2);
+    if (!q) return halide_error_code_device_malloc_failed;
+    vw.v[vw.n].ptr = q; vw.v[vw.n].borrowed = false; vw.n++;
+    if (repack16_launch(o.ptr, o.ld, o.bs, q, ld, o.inner, o.rows, o.matrices, rt_stream()) != cudaSuccess) {
+        cudaGetLastError();
+        return halide_error_code_device_run_failed;
+    }
+    rt_count_launch(1);
+    o.ptr = static_cast<char*>(q);
+    o.ld = ld;
+    o.bs = ld * o.rows;
+    return 0;
+}
+
+bool encode(CUtensorMap* map, uint32_t type, const Operand& o, int rank, uint32_t box_inner, uint32_t box_rows) {
+    // strides of dimensions of one element are never used, but have to be multiples of 16 bytes
+    const uint64_t ld = o.rows > 1 ? uint64_t(o.ld) * 2 : (uint64_t(o.inner) * 2 + 15) / 16 * 16;
+    const uint64_t bs = o.matrices > 1 ? uint64_t(o.bs) * 2 : ld * o.rows;
+    const uint64_t dims[3] = {uint64_t(o.inner), uint64_t(o.rows), uint64_t(o.matrices)}, str[3] = {2, ld, bs};
+    const uint32_t box[3] = {box_inner, box_rows, 1};
+    return rt_encode_tmap(map, type == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, o.ptr, dims,
+                          str, box);
+}
+
+// Lowering and launch, with the timing and the error report of the other operators. `p_op` holds the columns n (B, or D),
+// `q_op` the rows (A).
+int run_grouped(const char* who, int mode, uint32_t type, uint32_t out, GroupedParams& p, Operand p_op, Operand q_op, Views& vw,
+                bool sync_after) {
+    if (int e = check_capture(who, false, !p_op.fits() || !q_op.fits())) return e;
     cudaStream_t s = rt_stream();
     p.status = rt_status_word();
+    p.wait_cycles = rt_env().wait_cycles;
+    p.bf16 = type == kBF16;
     if (sync_after) cudaEventRecord(rt_event(0), s);
-    const cudaError_t e = grouped_launch(p, s);
+    GroupedMaps maps;
+    memset(&maps, 0, sizeof(maps));
+    if (p.K > 0 && p.rows > 0) {   // else nothing is read
+        if (int e = fit_operand(vw, p_op)) return e;
+        if (int e = fit_operand(vw, q_op)) return e;
+        bool ok = encode(&maps.p, type, p_op, 3, 64, mode == GR_FWD_K ? 128 : 64) &&
+                  encode(&maps.q, type, q_op, 2, 64, mode == GR_GRAD ? 64 : 128);
+        if (ok && mode != GR_GRAD) ok = encode(&maps.q16, type, q_op, 2, 64, 16);
+        if (!ok) return tma_unsupported(mode == GR_GRAD ? "A or D" : "A or B");
+    }
+    const cudaError_t e = grouped_launch(mode, out == kF32 ? GR_OUT_F32 : (out == kBF16 ? GR_OUT_BF16 : GR_OUT_F16), p, maps, s);
     if (e != cudaSuccess) {
         fprintf(stderr, "t2sp_b200: %s: kernel launch failed: %s\n", who, cudaGetErrorString(e));
         return halide_error_code_device_run_failed;
@@ -96,17 +149,13 @@ extern "C" int t2sp_b200_grouped_gemm(halide_buffer_t* A, halide_buffer_t* B, ha
     vw.n++;
     if (int e = preload_output(C, &vw.v[3])) return e;   // rows outside the groups keep their values
     GroupedParams p = {};
-    p.a = vw.v[0].ptr;
-    p.b = vw.v[1].ptr;
     p.offsets = static_cast<const int*>(vw.v[2].ptr);
     p.c = static_cast<char*>(vw.v[3].ptr) + origin_offset(C) * (out_f32 ? 4 : 2);
-    p.lda = A->dim[1].stride;
-    p.ldb = B->dim[1].stride;
-    p.bs_b = B->dim[2].stride;
     p.ldc = C->dim[1].stride;
     p.rows = M; p.E = E; p.K = K; p.N = N;
-    p.trans_b = tb; p.bf16 = in_t == kBF16; p.out_f32 = out_f32;
-    if (int e = run_grouped("grouped_gemm", p, sync_after)) return e;
+    const Operand b = {static_cast<char*>(vw.v[1].ptr), B->dim[1].stride, B->dim[2].stride, B->dim[0].extent, B->dim[1].extent, E};
+    const Operand a = {static_cast<char*>(vw.v[0].ptr), A->dim[1].stride, 0, K, M, 1};
+    if (int e = run_grouped("grouped_gemm", tb ? GR_FWD_K : GR_FWD_MN, in_t, out_f32 ? kF32 : in_t, p, b, a, vw, sync_after)) return e;
     if (int e = rt_finish_output(C, "C", &vw.v[3])) return e;
     return finish_call("grouped_gemm", "kernel_Out", sync_after);
 }
@@ -169,17 +218,14 @@ extern "C" int t2sp_b200_grouped_gemm_grad(halide_buffer_t* A, halide_buffer_t* 
     vw.n++;
     if (int e = preload_output(G, &vw.v[3])) return e;   // what G holds beyond (N, K, E) keeps its values
     GroupedParams p = {};
-    p.a = vw.v[0].ptr;
-    p.b = vw.v[1].ptr;
     p.offsets = static_cast<const int*>(vw.v[2].ptr);
     p.c = static_cast<char*>(vw.v[3].ptr) + origin_offset(G) * (out_f32 ? 4 : 2);
-    p.lda = A->dim[1].stride;
-    p.ldb = D->dim[1].stride;
     p.ldc = G->dim[1].stride;
     p.bs_c = G->dim[2].stride;
     p.rows = M; p.E = E; p.K = K; p.N = N;
-    p.grad = 1; p.bf16 = in_t == kBF16; p.out_f32 = out_f32;
-    if (int e = run_grouped("grouped_gemm_grad", p, sync_after)) return e;
+    const Operand d = {static_cast<char*>(vw.v[1].ptr), D->dim[1].stride, 0, N, M, 1};
+    const Operand a = {static_cast<char*>(vw.v[0].ptr), A->dim[1].stride, 0, K, M, 1};
+    if (int e = run_grouped("grouped_gemm_grad", GR_GRAD, in_t, out_f32 ? kF32 : in_t, p, d, a, vw, sync_after)) return e;
     if (int e = rt_finish_output(G, "G", &vw.v[3])) return e;
     return finish_call("grouped_gemm_grad", "kernel_Out", sync_after);
 }

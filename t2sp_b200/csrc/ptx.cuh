@@ -162,6 +162,14 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const void* map, uin
         "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster_addr), "r"(c0), "r"(c1)
         : "memory");
 }
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const void* map, uint32_t bar_cluster_addr, int c0, int c1,
+                                                 int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster_addr), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
 
 // ---------------------------------------------------------------- TMA stores (shared -> global, tiled mode)
 // The box is clipped to the tensor's extents, so ragged edges need no masking. The issuing

@@ -296,6 +296,32 @@ def test_graph_and_streams(lib):
         check_forward(x, w, o, z, False, z)
 
 
+def test_capture_refuses_what_it_cannot_hold(lib):
+    """A synchronous call, and a call that needs scratch memory, are refused inside a capture, which goes on."""
+    import torch
+    a, b, _, off = make(2, 37, 64, [10, 20], torch.bfloat16)
+    good, wide, _, _ = make(2, 64, 64, [10, 20], torch.bfloat16)
+    c = torch.zeros(30, 64, dtype=torch.bfloat16, device="cuda")
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    bufs = [buf(t) for t in (a, b, off, c, good, wide)]
+    torch.cuda.synchronize()
+    with on_stream(side, asynchronous=True) as L:
+        assert t2sp_b200.grouped_gemm(bufs[4], bufs[5], bufs[2], bufs[3]) == 0
+        side.synchronize()
+        c.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            rc_scratch = t2sp_b200.grouped_gemm(bufs[0], bufs[1], bufs[2], bufs[3])
+            L.t2sp_b200_set_async(0)
+            rc_sync = t2sp_b200.grouped_gemm(bufs[4], bufs[5], bufs[2], bufs[3])
+            L.t2sp_b200_set_async(1)
+            rc_ok = t2sp_b200.grouped_gemm(bufs[4], bufs[5], bufs[2], bufs[3])
+    assert (rc_scratch, rc_sync, rc_ok) == (-8, -8, 0)
+    graph.replay()
+    torch.cuda.synchronize()
+    check_forward(good, wide, off, c, False, c)
+
+
 def test_repeatable(lib):
     import torch
     a, b, d, off = make(5, 520, 776, [100, 3, 0, 900, 77], torch.bfloat16)
