@@ -2,7 +2,7 @@
 //
 // A matrix W(n, k) is held as w = (nibble - 8) * scale(n, k / group). The nibbles are laid out for the tensor cores'
 // m16n8k16 instruction: blocks of 16 n x 64 k of 512 bytes, a lane's 16 bytes one after the other. Lane 4 g + t holds
-// rows g and g + 8 and k = 16 t .. 16 t + 15 of the block; its 32-bit word s holds k = 16 t + 4 s + j, j = 0 .. 3, one
+// rows g and g + 8; its 32-bit word s (the instruction's step s, 16 consecutive k) holds k = 16 s + 4 t + j, j = 0 .. 3, one
 // byte each in the order j = 0, 2, 1, 3, row g in the low nibble and row g + 8 in the high one. So
 // (word >> 4 i) & 0x000f000f is the pair of 16-bit values of operand register i of the instruction (registers 0, 1:
 // j = 0, 1 of rows g, g + 8; registers 2, 3: j = 2, 3). Blocks run along k, then n, then the matrices.
