@@ -223,7 +223,7 @@ int t2sp_b200_grouped_gemm_grad(halide_buffer_t *A, halide_buffer_t *D, halide_b
  *              summed in fp32 within a group and scaled in fp32.
  * W: 3-D (N, K, E) or, with trans_b, (K, N, E); bf16 or f16. Q: 4-D uint8 (512, ceil(K/64), ceil(N/16), E), S: 4-D of W's
  * type (16, groups, ceil(N/16), E), both dense and in an order of the library's own (a bounds query on Q and S
- * gives their shapes; Q 16-byte aligned). X: 2-D (K, T), Y: 2-D (N, R) with R a multiple of T, of X's type or fp32;
+ * gives their shapes; both 16-byte aligned). X: 2-D (K, T), Y: 2-D (N, R) with R a multiple of T, of X's type or fp32;
  * X and S have one type. index: 1-D (R) int32, or NULL with E = 1. A row with a negative index is left as it was; an index
  * of E or more leaves the row as it was and reports halide_error_code_access_out_of_bounds (for asynchronous calls
  * at t2sp_b200_sync). For many rows, q4_unpack and grouped_gemm are faster. */

@@ -5,7 +5,9 @@
 #include <type_traits>
 
 #include "launch_util.cuh"
+#include "ptx.cuh"
 #include "q4.h"
+#include "umma_launch.h"
 
 namespace t2sp {
 
@@ -97,44 +99,52 @@ __global__ void q4_unpack_kernel(const Q4Params p) {
 }
 
 // ---------------------------------------------------------------- products of a few rows
-constexpr int kGemvWarps = 8;
-constexpr int kGemvUnroll = 4;                                 // 64-k blocks a warp has in flight for each of its strips
-constexpr int kGemvChunk = kGemvWarps * kGemvUnroll * 64;      // k values the CTA takes at a time
-constexpr int kGemvStrips = 2;                                 // strips of 16 n a CTA computes
+constexpr int kGemvWarps = 16;
+constexpr int kGemvBlocks = 4;                        // blocks of 64 k a warp's copy brings at a time
+constexpr int kGemvSlot = kGemvBlocks * (512 + 64);   // bytes of a slot: the blocks, then up to two groups' scales for each
+constexpr int kGemvMaxShared = 227 << 10;
+constexpr int kGemvTries = 1 << 17;                   // a wait gives up after this many tests of up to 16 us
 
-// Two 16-bit values q - 8 from the nibbles at bits 0..3 and 16..19 of `w`: the nibble becomes the low mantissa bits of
-// 1024 (fp16) or 128 (bf16), where a unit is 1, and 1032 or 136 is subtracted; both steps are exact.
-template <class T> __device__ __forceinline__ uint32_t q4_pair(uint32_t w);
-template <> __device__ __forceinline__ uint32_t q4_pair<__half>(uint32_t w) {
-    const uint32_t v = (w & 0x000f000fu) | 0x64006400u;
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408)));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-template <> __device__ __forceinline__ uint32_t q4_pair<__nv_bfloat16>(uint32_t w) {
-    const uint32_t v = (w & 0x000f000fu) | 0x43004300u;
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v),
-                                     __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308)));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
+// The sixteen integers of a lane's word as A-fragment registers, each times or plus a constant that the caller takes
+// out again: no conversion instruction is needed, which is what bounds the kernel otherwise (one and a half ALU operations a weight).
+//   fp16: the nibble is left where it is, as a subnormal number: q * 2^-24 in rows g, q * 2^-20 in rows g + 8
+//         (mantissa bits 0..3 and 4..7). The tensor core multiplies subnormal numbers exactly.
+//   bf16: the nibble goes to mantissa bits 3..6 of 1.0: 1 + q / 16. (Subnormal bf16 products would leave fp32's range.)
+// kOffset is what the integer q - 8 is offset by in units of kUnitLo / kUnitHi; offset times the sum of x over the group is subtracted in fp32.
+template <class T> struct Q4Frag;
+template <> struct Q4Frag<__half> {
+    static constexpr float kOffset = 8.f, kUnitLo = 16777216.f, kUnitHi = 1048576.f;   // 2^24, 2^20
+    static __device__ __forceinline__ void expand(uint32_t w, uint32_t (&a)[4]) {
+        const uint32_t v = w >> 8;
+        a[0] = w & 0x000f000fu;
+        a[1] = w & 0x00f000f0u;
+        a[2] = v & 0x000f000fu;
+        a[3] = v & 0x00f000f0u;
+    }
+};
+template <> struct Q4Frag<__nv_bfloat16> {
+    static constexpr float kOffset = 24.f, kUnitLo = 16.f, kUnitHi = 16.f;
+    static __device__ __forceinline__ void expand(uint32_t w, uint32_t (&a)[4]) {
+        a[0] = ((w << 3) & 0x00780078u) | 0x3f803f80u;
+        a[1] = ((w >> 1) & 0x00780078u) | 0x3f803f80u;
+        a[2] = ((w >> 5) & 0x00780078u) | 0x3f803f80u;
+        a[3] = ((w >> 9) & 0x00780078u) | 0x3f803f80u;
+    }
+};
 
 template <class T>
-__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
     if constexpr (std::is_same<T, __half>::value)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-__device__ __forceinline__ uint4 load_stream(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
+__device__ __forceinline__ void bar_group(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 template <class T> __device__ __forceinline__ float2 pair_f32(uint32_t w);
 template <> __device__ __forceinline__ float2 pair_f32<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
@@ -142,101 +152,150 @@ template <> __device__ __forceinline__ float2 pair_f32<__nv_bfloat16>(uint32_t w
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
 }
 
+// Shared memory of q4_gemv_kernel. A staged row of x holds, for each block of 64 k and each t = 0 .. 3, the 32 bytes that
+// lanes 4 g + t of the B fragments take (steps s = 0 .. 3, k = 16 s + 4 t + j): two 16-byte loads. The pitch is 16 modulo 128, so
+// that eight lanes of a load (two rows, four t) meet every bank once.
 template <int NT>
-struct GemvShared {
-    static constexpr int kPitch = kGemvChunk * 2 + 32;   // bytes of a staged row: rows 32 bytes apart modulo 128, so that a
-                                                         // fragment load of 8 rows x 32 bytes meets every bank once
-    uint8_t x[8 * NT * kPitch];
-    float part[kGemvWarps][kGemvStrips * 16][8 * NT + 1];
-    int rows[8 * NT];                                    // rows of y that this pass computes
-    int count;
+struct GemvLayout {
+    int pitch, xs, part, ring, bars, rows, units, idx, bytes;   // byte offsets
+    __host__ __device__ GemvLayout(int kblocks, int groups, int unit_rows, int depth, int R, bool indexed) {
+        pitch = kblocks * 128 + 16;
+        xs = unit_rows * pitch;
+        part = (xs + groups * 8 * NT * 4 + 15) & ~15;
+        ring = part + ((2 * kGemvWarps * 16 * (8 * NT + 1) * 4 + 127) & ~127);
+        bars = ring + kGemvWarps * depth * kGemvSlot;
+        rows = bars + kGemvWarps * depth * 8;
+        units = rows + 8 * NT * 4 + 16;
+        idx = units + (indexed ? R * 4 : 0);
+        bytes = idx + (indexed ? R * 4 : 0);
+    }
 };
 
-// Y[r] = X[r / per] x W[index[r]]. A CTA computes kGemvStrips strips of 16 n for the rows of one matrix: blockIdx.y is a row of y, and
-// the CTA of the first row that names a matrix takes all rows that name it, so a matrix is read once however many
-// rows share it (up to 8 NT rows at a time). The warps divide k; each turns 16-byte pieces of packed weights into A fragments of
-// m16n8k16 (16 n x 16 k of integers, exact in 16 bits) against B fragments of x (8 rows), sums a group in the instruction's fp32
-// accumulator, scales it in fp32 and adds it up; the eight partial sums meet in shared memory in a fixed order.
-template <class T, class O, int NT, bool G32>
-__global__ void __launch_bounds__(kGemvWarps * 32) q4_gemv_kernel(const Q4Params p) {
-    extern __shared__ __align__(16) uint8_t smem_raw[];
-    GemvShared<NT>& sh = *reinterpret_cast<GemvShared<NT>*>(smem_raw);
-    const int kblocks = q4_kblocks(p.K), strips = q4_strips(p.N), groups = q4_groups(p.K, p.group);
+// Y[r] = X[r / per] x W[index[r]]. Work items are (unit, strip of 16 n), where a unit is up to `unit_rows` (8 NT at most) rows that name one matrix:
+// a matrix is read once for all of them. Every CTA takes an equal run of consecutive items, stages a unit's rows of x in shared memory once, with
+// the sums of x over each group of k, and lets groups of `gs` warps compute a strip each, each warp a run of its k. A warp brings its own
+// packed weights and scales through a private ring of `depth` slots with bulk copies that run ahead over strip ends, turns 16 bytes a lane
+// into A fragments of m16n8k16, sums a group of k in the instruction's fp32 accumulators and adds scale * (sum - offset * sum of x) in
+// fp32. The gs partial sums of a strip meet in shared memory in a fixed order.
+template <class T, int NT, int G>
+__global__ void __launch_bounds__(kGemvWarps * 32, 1) q4_gemv_kernel(const Q4Params p, int gs, int unit_rows, int depth) {
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    constexpr int kCols = 8 * NT;
+    const int kblocks = q4_kblocks(p.K), strips = q4_strips(p.N), groups = q4_groups(p.K, G);
+    const GemvLayout<NT> lay(kblocks, groups, unit_rows, depth, p.R, p.index != nullptr);
+    float* xs = reinterpret_cast<float*>(smem_raw + lay.xs);
+    float* part = reinterpret_cast<float*>(smem_raw + lay.part);
+    int* rows = reinterpret_cast<int*>(smem_raw + lay.rows);
+    int* units = reinterpret_cast<int*>(smem_raw + lay.units);
+    int* idx = reinterpret_cast<int*>(smem_raw + lay.idx);
+    int* count_slot = rows + kCols;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int lead = blockIdx.y;
-    int e = 0;
-    if (p.index) {
-        e = p.index[lead];
-        if (e >= p.E) {
-            if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(p.status, ST_BAD_INDEX);
-            return;
-        }
-        if (e < 0) return;
-        int earlier = 0;
-        for (int r = threadIdx.x; r < lead; r += blockDim.x) earlier |= p.index[r] == e;
-        if (__syncthreads_or(earlier)) return;
+    uint8_t* ring = smem_raw + lay.ring + warp * depth * kGemvSlot;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + lay.bars) + warp * depth;
+    if (lane == 0) {
+        for (int d = 0; d < depth; ++d) ptx::mbar_init(&bars[d], 1);
+        ptx::fence_mbar_init();
     }
-    const int strip0 = blockIdx.x * kGemvStrips;
-    const uint8_t* qbase = p.q + (static_cast<long long>(e) * strips + strip0) * kblocks * 512 + lane * 16;
-    const T* sbase = reinterpret_cast<const T*>(p.s) + (static_cast<long long>(e) * strips + strip0) * groups * 16 + g * 2;
-    const int nstrips = min(kGemvStrips, strips - strip0);
-    const int chunks = (kblocks * 64 + kGemvChunk - 1) / kGemvChunk;
-    const int gsh = p.group == 128 ? 1 : 0;
+    __syncwarp();
 
-    uint4 q[kGemvStrips][kGemvUnroll];
-    uint32_t sc[kGemvStrips][kGemvUnroll][G32 ? 2 : 1];
-    auto fetch = [&](int chunk, int u) {
-        const int kb = (chunk * kGemvWarps + warp) * kGemvUnroll + u;
-#pragma unroll
-        for (int i = 0; i < kGemvStrips; ++i) {
-            q[i][u] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
-#pragma unroll
-            for (int h = 0; h < (G32 ? 2 : 1); ++h) sc[i][u][h] = 0;
-            if (kb < kblocks && i < nstrips) {
-                q[i][u] = load_stream(qbase + (static_cast<long long>(i) * kblocks + kb) * 512);
-#pragma unroll
-                for (int h = 0; h < (G32 ? 2 : 1); ++h)
-                    sc[i][u][h] = *reinterpret_cast<const uint32_t*>(
-                        sbase + (static_cast<long long>(i) * groups + (G32 ? kb * 2 + h : kb >> gsh)) * 16);
-            }
-        }
-    };
-    const bool x_aligned = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldx % 8 == 0;
-
-    for (int pass = 0;; ++pass) {
-        // the rows of this pass
-        if (warp == 0) {
-            const int base = pass * 8 * NT;   // rows that earlier passes took
-            int found;
-            if (p.index) {
-                int seen = 0;
-                for (int r0 = lead; r0 < p.R && seen < base + 8 * NT; r0 += 32) {
-                    const int r = r0 + lane;
-                    const unsigned hit = __ballot_sync(0xffffffffu, r < p.R && p.index[r] == e);
-                    const int slot = seen + __popc(hit & ((1u << lane) - 1)) - base;
-                    if ((hit >> lane & 1) && slot >= 0 && slot < 8 * NT) sh.rows[slot] = r;
-                    seen += __popc(hit);
-                }
-                found = max(0, min(8 * NT, seen - base));
-            } else {
-                found = max(0, min(8 * NT, p.R - base));
-                for (int i = lane; i < found; i += 32) sh.rows[i] = base + i;
-            }
-            if (lane == 0) sh.count = found;
+    // units: the rows whose number among the rows of their matrix is a multiple of unit_rows start one
+    int num_units;
+    if (p.index) {
+        for (int r = threadIdx.x; r < p.R; r += blockDim.x) idx[r] = p.index[r];
+        __syncthreads();
+        for (int r = threadIdx.x; r < p.R; r += blockDim.x) {
+            const int e = idx[r];
+            int before = 0;
+            for (int i = 0; i < r; ++i) before += idx[i] == e;
+            units[r] = e >= 0 && e < p.E && before % unit_rows == 0;
+            if (e >= p.E && blockIdx.x == 0) atomicOr(p.status, ST_BAD_INDEX);
         }
         __syncthreads();
-        const int count = sh.count;
-        if (count == 0) return;
-        float acc[kGemvStrips][NT][4] = {};
-#pragma unroll
-        for (int u = 0; u < kGemvUnroll; ++u) fetch(0, u);
-        for (int chunk = 0; chunk < chunks; ++chunk) {
-            // the chunk of x, zero beyond K
-            for (int i = threadIdx.x; i < count * (kGemvChunk / 8); i += blockDim.x) {
-                const int row = i / (kGemvChunk / 8), k8 = (i % (kGemvChunk / 8)) * 8;
-                const long long k = chunk * static_cast<long long>(kGemvChunk) + k8;
-                const uint16_t* src = static_cast<const uint16_t*>(p.x) + (sh.rows[row] / p.per) * p.ldx + k;
-                uint4 v = make_uint4(0, 0, 0, 0);
+        if (warp == 0) {   // the marks become the list of rows, in place: its end never passes the marks still to be read
+            int n = 0;
+            for (int r0 = 0; r0 < p.R; r0 += 32) {
+                const unsigned starts = __ballot_sync(0xffffffffu, r0 + lane < p.R && units[r0 + lane]);
+                if (starts >> lane & 1) units[n + __popc(starts & ((1u << lane) - 1))] = r0 + lane;
+                n += __popc(starts);
+                __syncwarp();
+            }
+            if (lane == 0) *count_slot = n;
+        }
+        __syncthreads();
+        num_units = *count_slot;
+    } else {
+        num_units = (p.R + unit_rows - 1) / unit_rows;
+    }
+
+    const long long items = static_cast<long long>(num_units) * strips;
+    long long item = items * blockIdx.x / gridDim.x;
+    const long long item_end = items * (blockIdx.x + 1) / gridDim.x;
+    const int wig = warp % gs, group = warp / gs, num_groups = kGemvWarps / gs;
+    // blocks of a strip that a warp takes, whole slots: kb_begin .. kb_end - 1
+    const int per_warp = (kblocks + gs * kGemvBlocks - 1) / (gs * kGemvBlocks) * kGemvBlocks;
+    const int kb_begin = min(kblocks, wig * per_warp), kb_end = min(kblocks, kb_begin + per_warp);
+    const bool x_aligned = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldx % 8 == 0;
+    int flip = 0, tries = kGemvTries;
+    int f_slot = 0, c_slot = 0;          // next slot to fill and to read
+    uint32_t c_phase = 0;
+
+    while (item < item_end) {
+        const int unit = static_cast<int>(item / strips);
+        const int s_begin = static_cast<int>(item % strips);
+        const int s_end = static_cast<int>(min(static_cast<long long>(strips), s_begin + (item_end - item)));
+        item += s_end - s_begin;
+        const int lead = p.index ? units[unit] : unit * unit_rows;
+        const int e = p.index ? idx[lead] : 0;
+
+        int f_strip = s_begin + group, f_kb = kb_begin;   // next copy
+        auto fetch = [&]() {
+            if (f_strip < s_end && f_kb < kb_end) {
+                if (lane == 0) {
+                    const int nb = min(kGemvBlocks, kb_end - f_kb);
+                    const int g0 = f_kb * 64 / G, ng = ((f_kb + nb) * 64 + G - 1) / G - g0;
+                    const long long strip = static_cast<long long>(e) * strips + f_strip;
+                    uint8_t* dst = ring + f_slot * kGemvSlot;
+                    ptx::mbar_expect_tx(&bars[f_slot], nb * 512 + ng * 32);
+                    ptx::bulk_load(dst, p.q + (strip * kblocks + f_kb) * 512, nb * 512, &bars[f_slot]);
+                    ptx::bulk_load(dst + kGemvBlocks * 512, p.s + (strip * groups + g0) * 16, ng * 32, &bars[f_slot]);
+                }
+                f_slot = f_slot + 1 == depth ? 0 : f_slot + 1;
+                f_kb += kGemvBlocks;
+                if (f_kb >= kb_end) { f_kb = kb_begin; f_strip += num_groups; }
+            }
+        };
+        for (int d = 0; d < depth; ++d) fetch();
+
+        // the rows of the unit, their x and its sums
+        __syncthreads();   // the previous unit's x and rows have been read
+        if (warp == 0) {
+            int found = 0;
+            if (p.index) {
+                for (int r0 = lead; r0 < p.R && found < unit_rows; r0 += 32) {
+                    const int r = r0 + lane;
+                    const unsigned hit = __ballot_sync(0xffffffffu, r < p.R && idx[r] == e);
+                    const int slot = found + __popc(hit & ((1u << lane) - 1));
+                    if ((hit >> lane & 1) && slot < unit_rows) rows[slot] = r;
+                    found = min(unit_rows, found + __popc(hit));
+                }
+            } else {
+                found = min(unit_rows, p.R - lead);
+                for (int i = lane; i < found; i += 32) rows[i] = lead + i;
+            }
+            if (lane == 0) *count_slot = found;
+        }
+        __syncthreads();
+        const int count = *count_slot;
+        const int pieces = kblocks * 8, padded = (pieces + 15) & ~15;   // of 8 k; a row's lanes start on a group of lanes
+        constexpr int kLanes = G / 8;                                   // lanes that hold a group
+        for (int i0 = 0; i0 < count * padded; i0 += blockDim.x) {
+            const int i = i0 + threadIdx.x;
+            const int row = i / padded, k8 = i % padded;
+            const bool real = row < count && k8 < pieces;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (real) {
+                const long long k = k8 * 8ll;
+                const uint16_t* src = static_cast<const uint16_t*>(p.x) + (rows[row] / p.per) * p.ldx + k;
                 if (x_aligned && k + 8 <= p.K) {
                     v = *reinterpret_cast<const uint4*>(src);
                 } else {
@@ -245,79 +304,151 @@ __global__ void __launch_bounds__(kGemvWarps * 32) q4_gemv_kernel(const Q4Params
                     for (int j = 0; j < 8; ++j)
                         if (k + j < p.K) w[j >> 1] |= uint32_t(src[j]) << (16 * (j & 1));
                 }
-                *reinterpret_cast<uint4*>(sh.x + row * GemvShared<NT>::kPitch + k8 * 2) = v;
+                // k = 16 s + 4 t + j of block k8 / 8: s = (k8 % 8) / 2, t = 2 (k8 % 2) and the next
+                uint8_t* dst = smem_raw + row * lay.pitch + (k8 >> 3) * 128 + (k8 & 1) * 64 + ((k8 >> 1) & 3) * 8;
+                *reinterpret_cast<uint2*>(dst) = make_uint2(v.x, v.y);
+                *reinterpret_cast<uint2*>(dst + 32) = make_uint2(v.z, v.w);
             }
-            __syncthreads();
+            const float2 a = pair_f32<T>(v.x), b = pair_f32<T>(v.y), c = pair_f32<T>(v.z), d = pair_f32<T>(v.w);
+            float sum = ((a.x + a.y) + (b.x + b.y)) + ((c.x + c.y) + (d.x + d.y));
 #pragma unroll
-            for (int u = 0; u < kGemvUnroll; ++u) {
-                const int kk = (warp * kGemvUnroll + u) * 64;
-                float c[kGemvStrips][NT][4] = {};
+            for (int m = 1; m < kLanes; m <<= 1) sum += __shfl_down_sync(0xffffffffu, sum, m);
+            // in the unit of the low rows' fragments, so that the sums need no factor of their own
+            if (real && k8 % kLanes == 0) xs[(k8 / kLanes) * kCols + row] = sum * (Q4Frag<T>::kOffset / Q4Frag<T>::kUnitLo);
+        }
+        __syncthreads();
+
+        for (int strip = s_begin + group; strip < s_end; strip += num_groups) {
+            float acc[NT][4] = {};
+            for (int kb0 = kb_begin; kb0 < kb_end; kb0 += kGemvBlocks) {
+                // a wait that runs out is reported and the rest of the call's waits do not block (its results are lost)
+                while (!ptx::mbar_try_wait(&bars[c_slot], c_phase)) {
+                    if (tries <= 0) break;
+                    if (--tries == 0 && lane == 0) atomicOr(p.status, ST_TIMEOUT_PRODUCER);
+                }
+                const uint8_t* slot = ring + c_slot * kGemvSlot;
+                const int nb = kb_end - kb0;
+                float c[NT][4] = {};
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    uint2 b[NT];
+                for (int u = 0; u < kGemvBlocks; ++u) {
+                    if (u < nb) {
+                        const uint4 q = *reinterpret_cast<const uint4*>(slot + u * 512 + lane * 16);
+                        const uint8_t* xrow = smem_raw + g * lay.pitch + (kb0 + u) * 128 + t * 32;
+                        uint4 b[NT][2];
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        b[n] = make_uint2(0, 0);
-                        if (n * 8 + g < count) b[n] = *reinterpret_cast<const uint2*>(sh.x + (n * 8 + g) * GemvShared<NT>::kPitch + (kk + 16 * s + 4 * t) * 2);
-                    }
+                        for (int n = 0; n < NT; ++n) {
+                            b[n][0] = b[n][1] = make_uint4(0, 0, 0, 0);
+                            if (n * 8 + g < count) {
+                                b[n][0] = *reinterpret_cast<const uint4*>(xrow + n * 8 * lay.pitch);
+                                b[n][1] = *reinterpret_cast<const uint4*>(xrow + n * 8 * lay.pitch + 16);
+                            }
+                        }
+                        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int i = 0; i < kGemvStrips; ++i) {
-                        const uint32_t w = (&q[i][u].x)[s];
-                        const uint32_t a[4] = {q4_pair<T>(w), q4_pair<T>(w >> 4), q4_pair<T>(w >> 8), q4_pair<T>(w >> 12)};
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) mma_16816<T>(c[i][n], a, b[n].x, b[n].y);
-                    }
-                    if (s == 3 || (G32 && s == 1)) {
-#pragma unroll
-                        for (int i = 0; i < kGemvStrips; ++i) {
-                            const float2 f = pair_f32<T>(sc[i][u][G32 ? s >> 1 : 0]);
+                        for (int s = 0; s < 4; ++s) {
+                            uint32_t a[4];
+                            Q4Frag<T>::expand((&q.x)[s], a);
+                            const bool begins = (s == 0 && (G != 128 || u % 2 == 0)) || (G == 32 && s == 2);
+                            const bool ends = (s == 3 && (G != 128 || u % 2 == 1 || u + 1 == nb)) || (G == 32 && s == 1);
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
-                                acc[i][n][0] += f.x * c[i][n][0];
-                                acc[i][n][1] += f.x * c[i][n][1];
-                                acc[i][n][2] += f.y * c[i][n][2];
-                                acc[i][n][3] += f.y * c[i][n][3];
-                                c[i][n][0] = c[i][n][1] = c[i][n][2] = c[i][n][3] = 0.f;
+                                const uint32_t b0 = (&b[n][s >> 1].x)[2 * (s & 1)], b1 = (&b[n][s >> 1].x)[2 * (s & 1) + 1];
+                                if (begins) mma_16816<T>(c[n], a, b0, b1, zero);
+                                else mma_16816<T>(c[n], a, b0, b1, c[n]);
+                            }
+                            if (ends) {
+                                const int in_slot = G == 32 ? u * 2 + (s >> 1) : (G == 64 ? u : u >> 1);
+                                const float2 f = pair_f32<T>(*reinterpret_cast<const uint32_t*>(slot + kGemvBlocks * 512 + in_slot * 32 + g * 4));
+                                const float* xg = xs + (kb0 * 64 / G + in_slot) * kCols + 2 * t;
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    const float2 x = *reinterpret_cast<const float2*>(xg + n * 8);
+                                    constexpr float kUp = Q4Frag<T>::kUnitLo / Q4Frag<T>::kUnitHi;   // the high rows' unit, a power of two
+                                    acc[n][0] += f.x * (c[n][0] - x.x);
+                                    acc[n][1] += f.x * (c[n][1] - x.y);
+                                    acc[n][2] += f.y * (c[n][2] - x.x * kUp);
+                                    acc[n][3] += f.y * (c[n][3] - x.y * kUp);
+                                }
                             }
                         }
                     }
                 }
-                if (chunk + 1 < chunks) fetch(chunk + 1, u);
+                c_slot = c_slot + 1 == depth ? 0 : c_slot + 1;
+                c_phase ^= c_slot == 0 ? 1u : 0u;
+                __syncwarp();   // every lane has read the slot
+                fetch();
             }
-            __syncthreads();
-        }
-#pragma unroll
-        for (int i = 0; i < kGemvStrips; ++i)
+            float* mine = part + (flip * kGemvWarps + warp) * 16 * (kCols + 1);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) sh.part[warp][i * 16 + g + (j >> 1) * 8][n * 8 + 2 * t + (j & 1)] = acc[i][n][j];
-        __syncthreads();
-        for (int i = threadIdx.x; i < kGemvStrips * 16 * count; i += blockDim.x) {
-            const int n = strip0 * 16 + i % (kGemvStrips * 16), row = i / (kGemvStrips * 16);
-            float v = 0.f;
-#pragma unroll
-            for (int w = 0; w < kGemvWarps; ++w) v += sh.part[w][i % (kGemvStrips * 16)][row];
-            if (n < p.N) static_cast<O*>(p.y)[sh.rows[row] * p.ldy + n] = rounded<O>(v);
+                for (int j = 0; j < 4; ++j)
+                    mine[(g + (j >> 1) * 8) * (kCols + 1) + n * 8 + 2 * t + (j & 1)] =
+                        acc[n][j] * (j >> 1 ? Q4Frag<T>::kUnitHi : Q4Frag<T>::kUnitLo);
+            bar_group(1 + group, gs * 32);
+            // two buffers in turn: this one is written again only after the barrier of the next strip
+            for (int i = wig * 32 + lane; i < 16 * count; i += gs * 32) {
+                const int n = i & 15, col = i >> 4;
+                const float* from = part + (flip * kGemvWarps + group * gs) * 16 * (kCols + 1) + n * (kCols + 1) + col;
+                float v = 0.f;
+                for (int w = 0; w < gs; ++w) v += from[w * 16 * (kCols + 1)];
+                if (strip * 16 + n < p.N) {
+                    const long long at = rows[col] * p.ldy + strip * 16 + n;
+                    if (p.out_f32) static_cast<float*>(p.y)[at] = v;
+                    else static_cast<T*>(p.y)[at] = rounded<T>(v);
+                }
+            }
+            flip ^= 1;
         }
-        __syncthreads();   // the next pass writes the shared rows
     }
 }
 
-template <class T, class O, int NT, bool G32>
+// How a call is cut: rows of x that a CTA stages at a time (as many as the instruction's columns and shared memory take; 0 when
+// not one fits) and slots of the warps' rings.
+struct GemvPlan {
+    int unit_rows, depth, bytes;
+};
+template <int NT>
+GemvPlan gemv_plan(int K, int group, int R, bool indexed) {
+    GemvPlan plan = {R < 8 * NT ? R : 8 * NT, 0, 0};
+    for (; plan.unit_rows > 0; --plan.unit_rows)
+        for (plan.depth = 4; plan.depth >= 2; --plan.depth) {
+            plan.bytes = GemvLayout<NT>(q4_kblocks(K), q4_groups(K, group), plan.unit_rows, plan.depth, R, indexed).bytes;
+            if (plan.bytes <= kGemvMaxShared) return plan;
+        }
+    return plan;
+}
+
+template <class T, int NT, int G>
 cudaError_t gemv_launch(const Q4Params& p, cudaStream_t stream) {
-    auto kern = q4_gemv_kernel<T, O, NT, G32>;
+    auto kern = q4_gemv_kernel<T, NT, G>;
     static std::atomic<bool> configured[kMaxDev];
-    if (cudaError_t e = allow_smem(kern, sizeof(GemvShared<NT>), configured)) return e;
-    const dim3 grid((q4_strips(p.N) + kGemvStrips - 1) / kGemvStrips, p.index ? p.R : 1);
-    kern<<<grid, kGemvWarps * 32, sizeof(GemvShared<NT>), stream>>>(p);
+    if (cudaError_t e = allow_smem(kern, kGemvMaxShared, configured)) return e;
+    const GemvPlan plan = gemv_plan<NT>(p.K, G, p.R, p.index != nullptr);
+    if (plan.unit_rows <= 0) return cudaErrorInvalidValue;   // the entry point has checked q4_gemv_fits
+    const int sms = core_sm_count(), kblocks = q4_kblocks(p.K);
+    const long long units = p.index ? (p.R < p.E ? p.R : p.E) : (p.R + plan.unit_rows - 1) / plan.unit_rows;   // about
+    const long long items = units * q4_strips(p.N);
+    const int grid = static_cast<int>(items < 1 ? 1 : (items < sms ? items : sms));
+    // warps to a strip: all of them where a CTA has one strip at a time, fewer where it has several or k gives them nothing to do
+    const long long per_cta = (items + grid - 1) / grid;
+    int gs = per_cta >= 8 ? 4 : (per_cta >= 3 ? 8 : 16);
+    while (gs > 4 && kblocks <= gs / 2 * kGemvBlocks && per_cta > 1) gs /= 2;
+    kern<<<grid, kGemvWarps * 32, plan.bytes, stream>>>(p, gs, plan.unit_rows, plan.depth);
     return cudaGetLastError();
 }
 
-template <class T, class O>
+template <class T, int NT>
+cudaError_t gemv_group(const Q4Params& p, cudaStream_t stream) {
+    if (p.group == 32) return gemv_launch<T, NT, 32>(p, stream);
+    return p.group == 64 ? gemv_launch<T, NT, 64>(p, stream) : gemv_launch<T, NT, 128>(p, stream);
+}
+
+template <class T>
 cudaError_t gemv_typed(const Q4Params& p, cudaStream_t stream) {
-    if (p.R <= 8) return p.group == 32 ? gemv_launch<T, O, 1, true>(p, stream) : gemv_launch<T, O, 1, false>(p, stream);
-    return p.group == 32 ? gemv_launch<T, O, 2, true>(p, stream) : gemv_launch<T, O, 2, false>(p, stream);
+    // 16 rows at a time where rows are likely to share a matrix and their x fits
+    const bool two = p.R > 8 && p.R > 4 * p.E && gemv_plan<2>(p.K, p.group, p.R, p.index != nullptr).unit_rows > 8;
+    return two ? gemv_group<T, 2>(p, stream) : gemv_group<T, 1>(p, stream);
 }
 
 unsigned blocks_for(long long work) { return static_cast<unsigned>((work + 127) / 128); }
@@ -338,9 +469,10 @@ cudaError_t q4_unpack_launch(const Q4Params& p, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
+bool q4_gemv_fits(int K, int group, int R, bool indexed) { return gemv_plan<1>(K, group, R, indexed).unit_rows > 0; }
+
 cudaError_t q4_gemv_launch(const Q4Params& p, cudaStream_t stream) {
-    if (p.bf16) return p.out_f32 ? gemv_typed<__nv_bfloat16, float>(p, stream) : gemv_typed<__nv_bfloat16, __nv_bfloat16>(p, stream);
-    return p.out_f32 ? gemv_typed<__half, float>(p, stream) : gemv_typed<__half, __half>(p, stream);
+    return p.bf16 ? gemv_typed<__nv_bfloat16>(p, stream) : gemv_typed<__half>(p, stream);
 }
 
 }  // namespace t2sp

@@ -70,7 +70,7 @@ int check_w_q_s(Arg* args, int w, int q, int s, int tb, int group) {
     int qe[4], se[4];
     packed_extents(W->dim[tb ? 1 : 0].extent, W->dim[tb ? 0 : 1].extent, W->dim[2].extent, group, qe, se);
     if (int e = check_packed(args[q], qe, 16)) return e;
-    if (int e = check_packed(args[s], se, 4)) return e;
+    if (int e = check_packed(args[s], se, 16)) return e;
     for (int i = 0; i < 3; ++i)
         if (int e = check_host(args[i])) return e;
     return 0;
@@ -174,7 +174,8 @@ extern "C" int t2sp_b200_q4_gemv(halide_buffer_t* X, halide_buffer_t* Q, halide_
     if (p.R == 0 || p.N == 0) return 0;
     if (!index && p.E != 1) return constraint("Q.extent.3", p.E, "one matrix where no index is given", 1);
     if (index && index->dim[0].extent != p.R) return constraint("index.extent.0", index->dim[0].extent, "Y.extent.1", p.R);
-    if (index && p.R > 65535) return constraint("Y.extent.1", p.R, "at most 65535 where an index is given", 65535);
+    if (index && p.R > 1024) return constraint("Y.extent.1", p.R, "at most 1024 rows where an index is given", 1024);
+    if (!q4_gemv_fits(p.K, group, p.R, index != nullptr)) return constraint("X.extent.0", p.K, "at most about", 32768);   // a row of x is staged whole in shared memory
     if (T == 0 || p.R % T) return constraint("Y.extent.1", p.R, "a multiple of X.extent.1", T);
     for (int i = 0; i < n_args; ++i)
         if (int e = check_min0(args[i])) return e;
@@ -187,7 +188,7 @@ extern "C" int t2sp_b200_q4_gemv(halide_buffer_t* X, halide_buffer_t* Q, halide_
     int qe[4], se[4];
     packed_extents(p.N, p.K, p.E, group, qe, se);
     if (int e = check_packed(args[1], qe, 16)) return e;
-    if (int e = check_packed(args[2], se, 4)) return e;
+    if (int e = check_packed(args[2], se, 16)) return e;
     for (int i = 0; i < n_args; ++i)
         if (int e = check_host(args[i])) return e;
 

@@ -42,6 +42,8 @@ struct Q4Params {
 
 cudaError_t q4_pack_launch(const Q4Params& p, cudaStream_t stream);
 cudaError_t q4_unpack_launch(const Q4Params& p, cudaStream_t stream);
+// Whether the rows' x and index fit the kernel's shared memory.
+bool q4_gemv_fits(int K, int group, int R, bool indexed);
 cudaError_t q4_gemv_launch(const Q4Params& p, cudaStream_t stream);
 
 }  // namespace t2sp

@@ -147,6 +147,8 @@ def test_q4_refusals(lib):
     assert t2sp_b200.wrap_device(b, 4096 + 8) == 0     # the packed matrices start on 16 bytes
     assert gemv(Q=b) == -8
     assert gemv(R=0, T=1) == 0
+    assert gemv(K=100000, N=16, E=1, R=1, T=1) == -8   # a row of x has to fit in shared memory
+    assert gemv(R=1025, T=1025) == -8                  # rows that name their matrix: at most 1024
     if no_device():
         assert gemv() == -36 and gemv(E=1, index=None) == -36 and gemv(Y=f32(6, 40)) == -36
     W = h16(2, 100, 40)

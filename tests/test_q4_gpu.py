@@ -108,7 +108,8 @@ def test_pack_infinities_and_nan(lib):
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 @pytest.mark.parametrize("R,K,N,group", [(1, 64, 16, 64), (1, 1, 1, 32), (1, 4096, 520, 64), (2, 100, 40, 32), (7, 1001, 777, 32), (8, 512, 48, 128),
-                                         (9, 130, 33, 128), (17, 192, 64, 64), (33, 256, 80, 32), (70, 64, 17, 64), (3, 8200, 24, 128)])
+                                         (9, 130, 33, 128), (17, 192, 64, 64), (33, 256, 80, 32), (70, 64, 17, 64), (3, 8200, 24, 128), (9, 30000, 20, 64),
+                                         (1, 32000, 16, 128), (1100, 64, 16, 64)])
 def test_gemv_one_matrix(lib, R, K, N, group, dtype):
     import torch
     dt = getattr(torch, dtype)
@@ -122,7 +123,8 @@ def test_gemv_one_matrix(lib, R, K, N, group, dtype):
 
 
 @pytest.mark.parametrize("E,T,per,K,N,group", [(4, 3, 2, 128, 64, 32), (64, 8, 2, 512, 96, 64), (3, 40, 1, 96, 40, 32), (5, 1, 1, 1000, 24, 128),
-                                               (2, 30, 4, 70, 35, 64), (200, 70, 4, 64, 16, 64)])
+                                               (2, 30, 4, 70, 35, 64), (200, 70, 4, 64, 16, 64),
+                                               (1, 100, 1, 192, 40, 128), (7, 512, 2, 64, 20, 32)])
 def test_gemv_by_expert(lib, E, T, per, K, N, group):
     import torch
     dt = torch.bfloat16
