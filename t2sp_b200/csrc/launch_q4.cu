@@ -99,9 +99,10 @@ __global__ void q4_unpack_kernel(const Q4Params p) {
 }
 
 // ---------------------------------------------------------------- products of a few rows
-constexpr int kGemvWarps = 16;
-constexpr int kGemvBlocks = 4;                        // blocks of 64 k a warp's copy brings at a time
-constexpr int kGemvSlot = kGemvBlocks * (512 + 64);   // bytes of a slot: the blocks, then up to two groups' scales for each
+constexpr int kGemvWarps = 16;                        // that compute; one more brings the weights
+constexpr int kGemvThreads = (kGemvWarps + 1) * 32;
+constexpr int kGemvBlocks = 4;                        // blocks of 64 k that a warp computes at a time
+constexpr int kGemvSlot = kGemvBlocks * (512 + 64);   // a warp's share of a slot: its blocks, and up to two groups' scales for each
 constexpr int kGemvMaxShared = 227 << 10;
 constexpr int kGemvTries = 1 << 17;                   // a wait gives up after this many tests of up to 16 us
 
@@ -164,7 +165,7 @@ struct GemvLayout {
         part = (xs + groups * 8 * NT * 4 + 15) & ~15;
         ring = part + ((2 * kGemvWarps * 16 * (8 * NT + 1) * 4 + 127) & ~127);
         bars = ring + kGemvWarps * depth * kGemvSlot;
-        rows = bars + kGemvWarps * depth * 8;
+        rows = bars + kGemvWarps * depth * 16;
         units = rows + 8 * NT * 4 + 16;
         idx = units + (indexed ? R * 4 : 0);
         bytes = idx + (indexed ? R * 4 : 0);
@@ -173,12 +174,13 @@ struct GemvLayout {
 
 // Y[r] = X[r / per] x W[index[r]]. Work items are (unit, strip of 16 n), where a unit is up to `unit_rows` (8 NT at most) rows that name one matrix:
 // a matrix is read once for all of them. Every CTA takes an equal run of consecutive items, stages a unit's rows of x in shared memory once, with
-// the sums of x over each group of k, and lets groups of `gs` warps compute a strip each, each warp a run of its k. A warp brings its own
-// packed weights and scales through a private ring of `depth` slots with bulk copies that run ahead over strip ends, turns 16 bytes a lane
-// into A fragments of m16n8k16, sums a group of k in the instruction's fp32 accumulators and adds scale * (sum - offset * sum of x) in
-// fp32. The gs partial sums of a strip meet in shared memory in a fixed order.
+// the sums of x over each group of k, and lets groups of `gs` warps compute a strip each. One warp
+// brings packed weights and scales with bulk copies, gs * kGemvBlocks blocks of a strip at a time into a ring of `depth` slots for each
+// group, and runs ahead over strip and unit ends. A computing warp turns 16 bytes a lane into A fragments of m16n8k16, sums a group of k in the
+// instruction's fp32 accumulators and adds scale * (sum - offset * sum of x) in fp32. The gs partial sums of a strip meet in shared
+// memory in a fixed order.
 template <class T, int NT, int G>
-__global__ void __launch_bounds__(kGemvWarps * 32, 1) q4_gemv_kernel(const Q4Params p, int gs, int unit_rows, int depth) {
+__global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params p, int gs, int unit_rows, int depth) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
     constexpr int kCols = 8 * NT;
     const int kblocks = q4_kblocks(p.K), strips = q4_strips(p.N), groups = q4_groups(p.K, G);
@@ -190,13 +192,16 @@ __global__ void __launch_bounds__(kGemvWarps * 32, 1) q4_gemv_kernel(const Q4Par
     int* idx = reinterpret_cast<int*>(smem_raw + lay.idx);
     int* count_slot = rows + kCols;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    uint8_t* ring = smem_raw + lay.ring + warp * depth * kGemvSlot;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + lay.bars) + warp * depth;
-    if (lane == 0) {
-        for (int d = 0; d < depth; ++d) ptx::mbar_init(&bars[d], 1);
+    const int group = warp / gs, wig = warp % gs, num_groups = kGemvWarps / gs;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + lay.bars);   // [group][depth] filled, then [group][depth] free
+    const int slot_bytes = gs * kGemvSlot;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < num_groups * depth; ++i) {
+            ptx::mbar_init(&bars[i], 1);
+            ptx::mbar_init(&bars[num_groups * depth + i], gs);
+        }
         ptx::fence_mbar_init();
     }
-    __syncwarp();
 
     // units: the rows whose number among the rows of their matrix is a multiple of unit_rows start one
     int num_units;
@@ -219,24 +224,64 @@ __global__ void __launch_bounds__(kGemvWarps * 32, 1) q4_gemv_kernel(const Q4Par
                 n += __popc(starts);
                 __syncwarp();
             }
-            if (lane == 0) *count_slot = n;
+            if (lane == 0) count_slot[1] = n;   // a word of its own: the other one is written again while the copying warp reads this
         }
         __syncthreads();
-        num_units = *count_slot;
+        num_units = count_slot[1];
     } else {
         num_units = (p.R + unit_rows - 1) / unit_rows;
+        __syncthreads();
     }
 
     const long long items = static_cast<long long>(num_units) * strips;
     long long item = items * blockIdx.x / gridDim.x;
     const long long item_end = items * (blockIdx.x + 1) / gridDim.x;
-    const int wig = warp % gs, group = warp / gs, num_groups = kGemvWarps / gs;
-    // blocks of a strip that a warp takes, whole slots: kb_begin .. kb_end - 1
-    const int per_warp = (kblocks + gs * kGemvBlocks - 1) / (gs * kGemvBlocks) * kGemvBlocks;
-    const int kb_begin = min(kblocks, wig * per_warp), kb_end = min(kblocks, kb_begin + per_warp);
+    const int chunk = gs * kGemvBlocks;                         // blocks of a slot
+    const int chunks = (kblocks + chunk - 1) / chunk;           // slots of a strip
+    int tries = kGemvTries;   // a wait that runs out is reported, and the rest of the call's waits do not block (its results are lost)
+
+    if (warp == kGemvWarps) {
+        // ------------------------------------------------------------ brings the weights, group after group as slots become free
+        if (lane != 0) return;
+        uint32_t fill[4] = {0, 0, 0, 0};   // slots filled so far, by group
+        const int q_last = (kblocks - (chunks - 1) * chunk) * 512;
+        const int s_full = chunk * 64 / G * 32, s_last = (groups - (chunks - 1) * (chunk * 64 / G)) * 32;
+        while (item < item_end) {
+            const int unit = static_cast<int>(item / strips);
+            const int s_begin = static_cast<int>(item % strips);
+            const int s_end = static_cast<int>(min(static_cast<long long>(strips), s_begin + (item_end - item)));
+            item += s_end - s_begin;
+            const int e = p.index ? idx[units[unit]] : 0;
+            // strips s_begin + i go to group i % num_groups; the groups' slots are filled in turn
+            for (int s0 = s_begin; s0 < s_end; s0 += num_groups)
+                for (int c = 0; c < chunks; ++c) {
+                    const int qb = c + 1 == chunks ? q_last : chunk * 512, sb = c + 1 == chunks ? s_last : s_full;
+                    for (int gr = 0; gr < num_groups && s0 + gr < s_end; ++gr) {
+                        const long long strip = static_cast<long long>(e) * strips + s0 + gr;
+                        const int slot = gr * depth + static_cast<int>(fill[gr] % depth);
+                        const uint32_t phase = (fill[gr] / depth) & 1;
+                        ++fill[gr];
+                        while (!ptx::mbar_try_wait(&bars[num_groups * depth + slot], phase ^ 1)) {
+                            if (tries <= 0) break;
+                            if (--tries == 0) atomicOr(p.status, ST_TIMEOUT_PRODUCER);
+                        }
+                        uint8_t* dst = smem_raw + lay.ring + slot * slot_bytes;
+                        ptx::mbar_expect_tx(&bars[slot], qb + sb);
+                        ptx::bulk_load(dst, p.q + (strip * kblocks + c * chunk) * 512, qb, &bars[slot]);
+                        ptx::bulk_load(dst + chunk * 512, p.s + (strip * groups + c * (chunk * 64 / G)) * 16, sb, &bars[slot]);
+                    }
+                }
+        }
+        return;
+    }
+
+    // ---------------------------------------------------------------- computing warps
     const bool x_aligned = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldx % 8 == 0;
-    int flip = 0, tries = kGemvTries;
-    int f_slot = 0, c_slot = 0;          // next slot to fill and to read
+    const uint8_t* ring = smem_raw + lay.ring + group * depth * slot_bytes;
+    uint64_t* full = bars + group * depth;
+    uint64_t* freed = full + num_groups * depth;
+    int flip = 0;
+    int c_slot = 0;          // next slot to read
     uint32_t c_phase = 0;
 
     while (item < item_end) {
@@ -247,27 +292,8 @@ __global__ void __launch_bounds__(kGemvWarps * 32, 1) q4_gemv_kernel(const Q4Par
         const int lead = p.index ? units[unit] : unit * unit_rows;
         const int e = p.index ? idx[lead] : 0;
 
-        int f_strip = s_begin + group, f_kb = kb_begin;   // next copy
-        auto fetch = [&]() {
-            if (f_strip < s_end && f_kb < kb_end) {
-                if (lane == 0) {
-                    const int nb = min(kGemvBlocks, kb_end - f_kb);
-                    const int g0 = f_kb * 64 / G, ng = ((f_kb + nb) * 64 + G - 1) / G - g0;
-                    const long long strip = static_cast<long long>(e) * strips + f_strip;
-                    uint8_t* dst = ring + f_slot * kGemvSlot;
-                    ptx::mbar_expect_tx(&bars[f_slot], nb * 512 + ng * 32);
-                    ptx::bulk_load(dst, p.q + (strip * kblocks + f_kb) * 512, nb * 512, &bars[f_slot]);
-                    ptx::bulk_load(dst + kGemvBlocks * 512, p.s + (strip * groups + g0) * 16, ng * 32, &bars[f_slot]);
-                }
-                f_slot = f_slot + 1 == depth ? 0 : f_slot + 1;
-                f_kb += kGemvBlocks;
-                if (f_kb >= kb_end) { f_kb = kb_begin; f_strip += num_groups; }
-            }
-        };
-        for (int d = 0; d < depth; ++d) fetch();
-
         // the rows of the unit, their x and its sums
-        __syncthreads();   // the previous unit's x and rows have been read
+        bar_group(15, kGemvWarps * 32);   // the previous unit's x and rows have been read
         if (warp == 0) {
             int found = 0;
             if (p.index) {
@@ -284,11 +310,11 @@ __global__ void __launch_bounds__(kGemvWarps * 32, 1) q4_gemv_kernel(const Q4Par
             }
             if (lane == 0) *count_slot = found;
         }
-        __syncthreads();
+        bar_group(15, kGemvWarps * 32);
         const int count = *count_slot;
         const int pieces = kblocks * 8, padded = (pieces + 15) & ~15;   // of 8 k; a row's lanes start on a group of lanes
         constexpr int kLanes = G / 8;                                   // lanes that hold a group
-        for (int i0 = 0; i0 < count * padded; i0 += blockDim.x) {
+        for (int i0 = 0; i0 < count * padded; i0 += kGemvWarps * 32) {
             const int i = i0 + threadIdx.x;
             const int row = i / padded, k8 = i % padded;
             const bool real = row < count && k8 < pieces;
@@ -316,67 +342,73 @@ __global__ void __launch_bounds__(kGemvWarps * 32, 1) q4_gemv_kernel(const Q4Par
             // in the unit of the low rows' fragments, so that the sums need no factor of their own
             if (real && k8 % kLanes == 0) xs[(k8 / kLanes) * kCols + row] = sum * (Q4Frag<T>::kOffset / Q4Frag<T>::kUnitLo);
         }
-        __syncthreads();
+        bar_group(15, kGemvWarps * 32);
 
-        for (int strip = s_begin + group; strip < s_end; strip += num_groups) {
-            float acc[NT][4] = {};
-            for (int kb0 = kb_begin; kb0 < kb_end; kb0 += kGemvBlocks) {
-                // a wait that runs out is reported and the rest of the call's waits do not block (its results are lost)
-                while (!ptx::mbar_try_wait(&bars[c_slot], c_phase)) {
-                    if (tries <= 0) break;
-                    if (--tries == 0 && lane == 0) atomicOr(p.status, ST_TIMEOUT_PRODUCER);
-                }
-                const uint8_t* slot = ring + c_slot * kGemvSlot;
-                const int nb = kb_end - kb0;
-                float c[NT][4] = {};
+        // lanes of columns without a row read row 0 of x: what they compute is in columns that are not stored
+        const uint8_t* xlane[NT];
 #pragma unroll
-                for (int u = 0; u < kGemvBlocks; ++u) {
-                    if (u < nb) {
-                        const uint4 q = *reinterpret_cast<const uint4*>(slot + u * 512 + lane * 16);
-                        const uint8_t* xrow = smem_raw + g * lay.pitch + (kb0 + u) * 128 + t * 32;
-                        uint4 b[NT][2];
+        for (int n = 0; n < NT; ++n) xlane[n] = smem_raw + (n * 8 + g < count ? n * 8 + g : 0) * lay.pitch + t * 32;
+        const float* xslane = xs + 2 * t;
+        float acc[NT][4];
+        // the warp's blocks of one slot, kGemvBlocks of them or `nb` at the strip's end
+        auto compute = [&](auto full_slot, const uint8_t* blocks, const uint8_t* scales, int kb0, int nb) {
+            float c[NT][4] = {};
+#pragma unroll
+            for (int u = 0; u < kGemvBlocks; ++u) {
+                if (!full_slot.value && u >= nb) break;
+                const uint4 q = *reinterpret_cast<const uint4*>(blocks + u * 512);
+                uint4 b[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    b[n][0] = *reinterpret_cast<const uint4*>(xlane[n] + kb0 * 128 + u * 128);
+                    b[n][1] = *reinterpret_cast<const uint4*>(xlane[n] + kb0 * 128 + u * 128 + 16);
+                }
+                const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    uint32_t a[4];
+                    Q4Frag<T>::expand((&q.x)[s], a);
+                    const bool begins = (s == 0 && (G != 128 || u % 2 == 0)) || (G == 32 && s == 2);
+                    const bool ends = (s == 3 && (G != 128 || u % 2 == 1 || (!full_slot.value && u + 1 == nb))) || (G == 32 && s == 1);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const uint32_t b0 = (&b[n][s >> 1].x)[2 * (s & 1)], b1 = (&b[n][s >> 1].x)[2 * (s & 1) + 1];
+                        if (begins) mma_16816<T>(c[n], a, b0, b1, zero);
+                        else mma_16816<T>(c[n], a, b0, b1, c[n]);
+                    }
+                    if (ends) {
+                        const int in_slot = G == 32 ? u * 2 + (s >> 1) : (G == 64 ? u : u >> 1);
+                        const float2 f = pair_f32<T>(*reinterpret_cast<const uint32_t*>(scales + in_slot * 32));
+                        const float* xg = xslane + kb0 * (64 * kCols / G) + in_slot * kCols;
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            b[n][0] = b[n][1] = make_uint4(0, 0, 0, 0);
-                            if (n * 8 + g < count) {
-                                b[n][0] = *reinterpret_cast<const uint4*>(xrow + n * 8 * lay.pitch);
-                                b[n][1] = *reinterpret_cast<const uint4*>(xrow + n * 8 * lay.pitch + 16);
-                            }
-                        }
-                        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int s = 0; s < 4; ++s) {
-                            uint32_t a[4];
-                            Q4Frag<T>::expand((&q.x)[s], a);
-                            const bool begins = (s == 0 && (G != 128 || u % 2 == 0)) || (G == 32 && s == 2);
-                            const bool ends = (s == 3 && (G != 128 || u % 2 == 1 || u + 1 == nb)) || (G == 32 && s == 1);
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) {
-                                const uint32_t b0 = (&b[n][s >> 1].x)[2 * (s & 1)], b1 = (&b[n][s >> 1].x)[2 * (s & 1) + 1];
-                                if (begins) mma_16816<T>(c[n], a, b0, b1, zero);
-                                else mma_16816<T>(c[n], a, b0, b1, c[n]);
-                            }
-                            if (ends) {
-                                const int in_slot = G == 32 ? u * 2 + (s >> 1) : (G == 64 ? u : u >> 1);
-                                const float2 f = pair_f32<T>(*reinterpret_cast<const uint32_t*>(slot + kGemvBlocks * 512 + in_slot * 32 + g * 4));
-                                const float* xg = xs + (kb0 * 64 / G + in_slot) * kCols + 2 * t;
-#pragma unroll
-                                for (int n = 0; n < NT; ++n) {
-                                    const float2 x = *reinterpret_cast<const float2*>(xg + n * 8);
-                                    constexpr float kUp = Q4Frag<T>::kUnitLo / Q4Frag<T>::kUnitHi;   // the high rows' unit, a power of two
-                                    acc[n][0] += f.x * (c[n][0] - x.x);
-                                    acc[n][1] += f.x * (c[n][1] - x.y);
-                                    acc[n][2] += f.y * (c[n][2] - x.x * kUp);
-                                    acc[n][3] += f.y * (c[n][3] - x.y * kUp);
-                                }
-                            }
+                            const float2 x = *reinterpret_cast<const float2*>(xg + n * 8);
+                            constexpr float kUp = Q4Frag<T>::kUnitLo / Q4Frag<T>::kUnitHi;   // the high rows' unit, a power of two
+                            acc[n][0] += f.x * (c[n][0] - x.x);
+                            acc[n][1] += f.x * (c[n][1] - x.y);
+                            acc[n][2] += f.y * (c[n][2] - x.x * kUp);
+                            acc[n][3] += f.y * (c[n][3] - x.y * kUp);
                         }
                     }
                 }
-                c_slot = c_slot + 1 == depth ? 0 : c_slot + 1;
-                c_phase ^= c_slot == 0 ? 1u : 0u;
+            }
+        };
+        for (int strip = s_begin + group; strip < s_end; strip += num_groups) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+            for (int kb0 = wig * kGemvBlocks; kb0 < chunks * chunk; kb0 += chunk) {
+                while (!ptx::mbar_try_wait(&full[c_slot], c_phase)) {
+                    if (tries <= 0) break;
+                    if (--tries == 0 && lane == 0) atomicOr(p.status, ST_TIMEOUT_MMA);
+                }
+                const uint8_t* slot = ring + c_slot * slot_bytes;
+                const uint8_t* blocks = slot + wig * (kGemvBlocks * 512) + lane * 16;
+                const uint8_t* scales = slot + chunk * 512 + wig * (kGemvBlocks * 64 / G * 32) + g * 4;
+                if (kb0 + kGemvBlocks <= kblocks) compute(std::true_type(), blocks, scales, kb0, kGemvBlocks);
+                else if (kb0 < kblocks) compute(std::false_type(), blocks, scales, kb0, kblocks - kb0);
                 __syncwarp();   // every lane has read the slot
-                fetch();
+                if (lane == 0) ptx::mbar_arrive(&freed[c_slot]);
+                if (++c_slot == depth) { c_slot = 0; c_phase ^= 1u; }
             }
             float* mine = part + (flip * kGemvWarps + warp) * 16 * (kCols + 1);
 #pragma unroll
@@ -430,11 +462,16 @@ cudaError_t gemv_launch(const Q4Params& p, cudaStream_t stream) {
     const long long units = p.index ? (p.R < p.E ? p.R : p.E) : (p.R + plan.unit_rows - 1) / plan.unit_rows;   // about
     const long long items = units * q4_strips(p.N);
     const int grid = static_cast<int>(items < 1 ? 1 : (items < sms ? items : sms));
-    // warps to a strip: all of them where a CTA has one strip at a time, fewer where it has several or k gives them nothing to do
+    // Warps to a strip: the number that needs the fewest slot times, where the groups of a CTA share its strips and a strip's end costs about
+    // half a slot (8192 x 32768, 14 strips a CTA: 4 groups take 4 strips one after another, 2 groups 7 of half the length).
     const long long per_cta = (items + grid - 1) / grid;
-    int gs = per_cta >= 8 ? 4 : (per_cta >= 3 ? 8 : 16);
-    while (gs > 4 && kblocks <= gs / 2 * kGemvBlocks && per_cta > 1) gs /= 2;
-    kern<<<grid, kGemvWarps * 32, plan.bytes, stream>>>(p, gs, plan.unit_rows, plan.depth);
+    int gs = 16;
+    long long best = 0;
+    for (int n = 16; n >= 4; n /= 2) {
+        const long long cost = (per_cta * n + 15) / 16 * (2 * ((kblocks + n * kGemvBlocks - 1) / (n * kGemvBlocks)) + 1);
+        if (n == 16 || cost < best) { best = cost; gs = n; }
+    }
+    kern<<<grid, kGemvThreads, plan.bytes, stream>>>(p, gs, plan.unit_rows, plan.depth);
     return cudaGetLastError();
 }
 
