@@ -24,7 +24,7 @@ template <> __device__ __forceinline__ __half rounded<__half>(float v) { return 
 __device__ __forceinline__ long long q4_byte(int e, int strip, int g, int k, int kblocks, int strips) {
     const int kk = k & 63, j = kk & 3;
     return ((static_cast<long long>(e) * strips + strip) * kblocks + (k >> 6)) * 512 + (g * 4 + ((kk >> 2) & 3)) * 16 +
-           (kk >> 4) * 4 + ((j & 1) << 1) + (j >> 1);
+           (kk >> 4) * 4 + j;
 }
 
 // The nearest of -7 .. 7 to v / scale, ties to even. The quotient of two 16-bit values cannot round onto a tie that
@@ -106,32 +106,49 @@ constexpr int kGemvSlot = kGemvBlocks * (512 + 64);   // a warp's share of a slo
 constexpr int kGemvMaxShared = 227 << 10;
 constexpr int kGemvTries = 1 << 17;                   // a wait gives up after this many tests of up to 16 us
 
-// The sixteen integers of a lane's word as A-fragment registers, each times or plus a constant that the caller takes
-// out again: no conversion instruction is needed, which is what bounds the kernel otherwise (one and a half ALU operations a weight).
-//   fp16: the nibble is left where it is, as a subnormal number: q * 2^-24 in rows g, q * 2^-20 in rows g + 8
-//         (mantissa bits 0..3 and 4..7). The tensor core multiplies subnormal numbers exactly.
-//   bf16: the nibble goes to mantissa bits 3..6 of 1.0: 1 + q / 16. (Subnormal bf16 products would leave fp32's range.)
-// kOffset is what the integer q - 8 is offset by in units of kUnitLo / kUnitHi; offset times the sum of x over the group is subtracted in fp32.
+// The sixteen integers q - 8 of a lane's word as 16-bit floating-point A-fragment registers, exactly: the nibbles become low mantissa
+// bits of a number whose last bit counts 1 (128 in bf16, 1024 in fp16; fp16 has room for the second nibble as it stands, counting
+// 16), and one packed operation takes the constant off. (Leaving fp16 nibbles as subnormal numbers and the constant to the sums of x
+// saves that operation, but the tensor core aligns a subnormal product by its exponent field and drops seven to ten bits of it.)
 template <class T> struct Q4Frag;
 template <> struct Q4Frag<__half> {
-    static constexpr float kOffset = 8.f, kUnitLo = 16777216.f, kUnitHi = 1048576.f;   // 2^24, 2^20
+    static __device__ __forceinline__ uint32_t low(uint32_t w) {
+        const uint32_t v = (w & 0x000f000fu) | 0x64006400u, o = 0x64086408u;   // 1024 + q, 1032
+        const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&o));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+    static __device__ __forceinline__ uint32_t high(uint32_t w) {
+        const uint32_t v = (w & 0x00f000f0u) | 0x64006400u, m = 0x2c002c00u, o = 0xd480d480u;   // 1024 + 16 q, 1 / 16, -72
+        const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&m), *reinterpret_cast<const __half2*>(&o));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
     static __device__ __forceinline__ void expand(uint32_t w, uint32_t (&a)[4]) {
-        const uint32_t v = w >> 8;
-        a[0] = w & 0x000f000fu;
-        a[1] = w & 0x00f000f0u;
-        a[2] = v & 0x000f000fu;
-        a[3] = v & 0x00f000f0u;
+        a[0] = low(w);
+        a[1] = high(w);
+        a[2] = low(w >> 8);
+        a[3] = high(w >> 8);
     }
 };
 template <> struct Q4Frag<__nv_bfloat16> {
-    static constexpr float kOffset = 24.f, kUnitLo = 16.f, kUnitHi = 16.f;
+    static __device__ __forceinline__ uint32_t low(uint32_t w) {
+        const uint32_t v = (w & 0x000f000fu) | 0x43004300u, o = 0x43084308u;   // 128 + q, 136
+        const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&o));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
     static __device__ __forceinline__ void expand(uint32_t w, uint32_t (&a)[4]) {
-        a[0] = ((w << 3) & 0x00780078u) | 0x3f803f80u;
-        a[1] = ((w >> 1) & 0x00780078u) | 0x3f803f80u;
-        a[2] = ((w >> 5) & 0x00780078u) | 0x3f803f80u;
-        a[3] = ((w >> 9) & 0x00780078u) | 0x3f803f80u;
+        a[0] = low(w);
+        a[1] = low(w >> 4);
+        a[2] = low(w >> 8);
+        a[3] = low(w >> 12);
     }
 };
+
+// Integers: sixteen k of unsigned nibbles against signed bytes of x, exact in 32 bits.
+__device__ __forceinline__ void mma_16832(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 
 template <class T>
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
@@ -153,39 +170,56 @@ template <> __device__ __forceinline__ float2 pair_f32<__nv_bfloat16>(uint32_t w
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
 }
 
-// Shared memory of q4_gemv_kernel. A staged row of x holds, for each block of 64 k and each t = 0 .. 3, the 32 bytes that
-// lanes 4 g + t of the B fragments take (steps s = 0 .. 3, k = 16 s + 4 t + j): two 16-byte loads. The pitch is 16 modulo 128, so
-// that eight lanes of a load (two rows, four t) meet every bank once.
-template <int NT>
+// Two ways to multiply, by the number of rows that share a pass over the weights.
+//   INT  a few rows: the weights stay unsigned nibbles, whose offset 8 the sum of x over the group takes out, and x is written, group by group of k, as 24-bit integers times a power of two, in three signed bytes, and each byte is a column of
+//        m16n8k32: two operations turn a word of weights into operands, half as many instructions as with 16-bit products, and the sums of
+//        a group are exact. A value of x down to 2^-11 of its group's largest is held exactly (bf16: 2^-14); a smaller one is off by at
+//        most 2^-23 of the largest, about what an fp32 sum over the group rounds away at each step.
+//   else x stays in 16 bits, one column of m16n8k16 a row, with the nibbles as 16-bit numbers (Q4Frag).
+template <int NT, bool INT>
+struct GemvShape {
+    static constexpr int kCols = 8 * NT;
+    static constexpr int kPerRow = INT ? 3 : 1;                 // columns of a row
+    static constexpr int kRows = kCols / kPerRow;               // rows of a pass
+    static constexpr int kBlockBytes = INT ? 64 : 128;          // of a column, for 64 k
+    static constexpr int kSumBytes = INT ? 8 : 0;               // of a column, for a group
+};
+
+// Shared memory of q4_gemv_kernel. A staged column of x holds, for each block of 64 k and each t = 0 .. 3, the bytes that lanes 4 g + t
+// of the B fragments take: one 16-byte load (INT; pitch 64 modulo 128) or two (pitch 16 modulo 128), where eight
+// lanes of a load (two columns, four t) meet every bank once.
+template <int NT, bool INT>
 struct GemvLayout {
     int pitch, xs, part, ring, bars, rows, units, idx, bytes;   // byte offsets
     __host__ __device__ GemvLayout(int kblocks, int groups, int unit_rows, int depth, int R, bool indexed) {
-        pitch = kblocks * 128 + 16;
-        xs = unit_rows * pitch;
-        part = (xs + groups * 8 * NT * 4 + 15) & ~15;
-        ring = part + ((2 * kGemvWarps * 16 * (8 * NT + 1) * 4 + 127) & ~127);
+        using S = GemvShape<NT, INT>;
+        pitch = INT ? (kblocks | 1) * 64 : kblocks * 128 + 16;
+        xs = (unit_rows * S::kPerRow * pitch + 15) & ~15;
+        part = (xs + groups * S::kCols * S::kSumBytes + 15) & ~15;
+        ring = part + ((2 * kGemvWarps * 16 * (S::kCols + 1) * 4 + 127) & ~127);
         bars = ring + kGemvWarps * depth * kGemvSlot;
         rows = bars + kGemvWarps * depth * 16;
-        units = rows + 8 * NT * 4 + 16;
+        units = rows + S::kCols * 4 + 16;
         idx = units + (indexed ? R * 4 : 0);
         bytes = idx + (indexed ? R * 4 : 0);
     }
 };
 
-// Y[r] = X[r / per] x W[index[r]]. Work items are (unit, strip of 16 n), where a unit is up to `unit_rows` (8 NT at most) rows that name one matrix:
+// Y[r] = X[r / per] x W[index[r]]. Work items are (unit, strip of 16 n), where a unit is up to `unit_rows` rows that name one matrix:
 // a matrix is read once for all of them. Every CTA takes an equal run of consecutive items, stages a unit's rows of x in shared memory once, with
 // the sums of x over each group of k, and lets groups of `gs` warps compute a strip each. One warp
 // brings packed weights and scales with bulk copies, gs * kGemvBlocks blocks of a strip at a time into a ring of `depth` slots for each
-// group, and runs ahead over strip and unit ends. A computing warp turns 16 bytes a lane into A fragments of m16n8k16, sums a group of k in the
-// instruction's fp32 accumulators and adds scale * (sum - offset * sum of x) in fp32. The gs partial sums of a strip meet in shared
-// memory in a fixed order.
-template <class T, int NT, int G>
+// group, and runs ahead over strip and unit ends. A computing warp turns 16 bytes a lane into A fragments, sums a group of k in the
+// instruction's accumulators, and adds the scaled sum in fp32. The gs partial sums of a strip meet in shared memory in a fixed order.
+template <class T, int NT, int G, bool INT>
 __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params p, int gs, int unit_rows, int depth) {
+    using S = GemvShape<NT, INT>;
     extern __shared__ __align__(128) uint8_t smem_raw[];
-    constexpr int kCols = 8 * NT;
+    constexpr int kCols = S::kCols;
     const int kblocks = q4_kblocks(p.K), strips = q4_strips(p.N), groups = q4_groups(p.K, G);
-    const GemvLayout<NT> lay(kblocks, groups, unit_rows, depth, p.R, p.index != nullptr);
-    float* xs = reinterpret_cast<float*>(smem_raw + lay.xs);
+    const GemvLayout<NT, INT> lay(kblocks, groups, unit_rows, depth, p.R, p.index != nullptr);
+    int* xi = reinterpret_cast<int*>(smem_raw + lay.xs);        // INT, [group][column]: -8 times the sum of the bytes of x, and behind all of them
+    float* xf = reinterpret_cast<float*>(xi + groups * kCols);  // what a unit of the integer sums is worth
     float* part = reinterpret_cast<float*>(smem_raw + lay.part);
     int* rows = reinterpret_cast<int*>(smem_raw + lay.rows);
     int* units = reinterpret_cast<int*>(smem_raw + lay.units);
@@ -314,80 +348,159 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
         const int count = *count_slot;
         const int pieces = kblocks * 8, padded = (pieces + 15) & ~15;   // of 8 k; a row's lanes start on a group of lanes
         constexpr int kLanes = G / 8;                                   // lanes that hold a group
-        for (int i0 = 0; i0 < count * padded; i0 += kGemvWarps * 32) {
-            const int i = i0 + threadIdx.x;
-            const int row = i / padded, k8 = i % padded;
-            const bool real = row < count && k8 < pieces;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (real) {
-                const long long k = k8 * 8ll;
-                const uint16_t* src = static_cast<const uint16_t*>(p.x) + (rows[row] / p.per) * p.ldx + k;
-                if (x_aligned && k + 8 <= p.K) {
-                    v = *reinterpret_cast<const uint4*>(src);
-                } else {
-                    uint32_t* w = &v.x;
+        for (int row = 0; row < count; ++row)
+            for (int k0 = warp * 32; k0 < padded; k0 += kGemvWarps * 32) {   // whole warps: the shuffles need every lane
+                const int k8 = k0 + lane;
+                const bool real = k8 < pieces;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (real) {
+                    const long long k = k8 * 8ll;
+                    const uint16_t* src = static_cast<const uint16_t*>(p.x) + (rows[row] / p.per) * p.ldx + k;
+                    if (x_aligned && k + 8 <= p.K) {
+                        v = *reinterpret_cast<const uint4*>(src);
+                    } else {
+                        uint32_t* w = &v.x;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (k + j < p.K) w[j >> 1] |= uint32_t(src[j]) << (16 * (j & 1));
+                        for (int j = 0; j < 8; ++j)
+                            if (k + j < p.K) w[j >> 1] |= uint32_t(src[j]) << (16 * (j & 1));
+                    }
                 }
-                // k = 16 s + 4 t + j of block k8 / 8: s = (k8 % 8) / 2, t = 2 (k8 % 2) and the next
-                uint8_t* dst = smem_raw + row * lay.pitch + (k8 >> 3) * 128 + (k8 & 1) * 64 + ((k8 >> 1) & 3) * 8;
-                *reinterpret_cast<uint2*>(dst) = make_uint2(v.x, v.y);
-                *reinterpret_cast<uint2*>(dst + 32) = make_uint2(v.z, v.w);
-            }
-            const float2 a = pair_f32<T>(v.x), b = pair_f32<T>(v.y), c = pair_f32<T>(v.z), d = pair_f32<T>(v.w);
-            float sum = ((a.x + a.y) + (b.x + b.y)) + ((c.x + c.y) + (d.x + d.y));
+                const float2 a = pair_f32<T>(v.x), b = pair_f32<T>(v.y), c = pair_f32<T>(v.z), d = pair_f32<T>(v.w);
+                const float f[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+                // k = 16 w + 4 t + j of block k8 / 8: w = (k8 % 8) / 2, t = 2 (k8 % 2) and the next
+                if constexpr (INT) {
+                    float top = 0.f;
+                    bool bad = false;
 #pragma unroll
-            for (int m = 1; m < kLanes; m <<= 1) sum += __shfl_down_sync(0xffffffffu, sum, m);
-            // in the unit of the low rows' fragments, so that the sums need no factor of their own
-            if (real && k8 % kLanes == 0) xs[(k8 / kLanes) * kCols + row] = sum * (Q4Frag<T>::kOffset / Q4Frag<T>::kUnitLo);
-        }
+                    for (int j = 0; j < 8; ++j) {
+                        top = fmaxf(top, fabsf(f[j]));
+                        bad = bad || !(fabsf(f[j]) < __int_as_float(0x7f800000));
+                    }
+#pragma unroll
+                    for (int m = 1; m < kLanes; m <<= 1) {
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+                        bad = __shfl_xor_sync(0xffffffffu, bad, m) || bad;
+                    }
+                    // The largest power of two that keeps the integers within three signed bytes (127 * 65793): top < 2^(e + 1) has e in
+                    // its exponent bits. Subnormal numbers are taken for 2^-126, where nothing of a 16-bit type needs more.
+                    const int e = max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -126);
+                    int up = bad ? 0 : 22 - e;
+                    const int up1 = up >> 1;   // in two steps: 2^up itself may leave fp32's range
+                    float f1 = __uint_as_float(static_cast<uint32_t>(up1 + 127) << 23), f2 = __uint_as_float(static_cast<uint32_t>(up - up1 + 127) << 23);
+                    if (top * f1 * f2 > 8355711.f) { --up; f2 *= 0.5f; }
+                    // x + 0x808080 as an unsigned number: its bytes less 128 are the signed bytes
+                    uint32_t u[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) u[j] = bad ? 0x808080u : __float2int_rn(f[j] * f1 * f2) + 0x808080;
+                    uint32_t digits[3][2];
+                    int sums[3];
+#pragma unroll
+                    for (int n = 0; n < 3; ++n) {
+                        const uint32_t sel = n | ((4 + n) << 4);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            digits[n][h] = __byte_perm(__byte_perm(u[4 * h], u[4 * h + 1], sel), __byte_perm(u[4 * h + 2], u[4 * h + 3], sel), 0x5410) ^ 0x80808080u;
+                        sums[n] = __dp4a(static_cast<int>(digits[n][0]), 0x01010101, __dp4a(static_cast<int>(digits[n][1]), 0x01010101, 0));
+                    }
+                    // two sums to a word on the way over the lanes: each stays within 2^14
+                    int low = sums[0] + sums[1] * 65536;
+#pragma unroll
+                    for (int m = 1; m < kLanes; m <<= 1) {
+                        low += __shfl_xor_sync(0xffffffffu, low, m);
+                        sums[2] += __shfl_xor_sync(0xffffffffu, sums[2], m);
+                    }
+                    sums[0] = static_cast<int16_t>(low & 0xffff);
+                    sums[1] = (low - sums[0]) >> 16;
+                    const float back = __uint_as_float(static_cast<uint32_t>(127 - (up >> 1)) << 23) * __uint_as_float(static_cast<uint32_t>(127 - (up - (up >> 1))) << 23);
+                    if (real) {
+#pragma unroll
+                        for (int n = 0; n < 3; ++n) {
+                            uint8_t* dst = smem_raw + (row * 3 + n) * lay.pitch + (k8 >> 3) * 64 + (k8 & 1) * 32 + ((k8 >> 1) & 3) * 4;
+                            *reinterpret_cast<uint32_t*>(dst) = digits[n][0];
+                            *reinterpret_cast<uint32_t*>(dst + 16) = digits[n][1];
+                            if (k8 % kLanes == 0) {
+                                xi[(k8 / kLanes) * kCols + row * 3 + n] = -8 * sums[n];
+                                xf[(k8 / kLanes) * kCols + row * 3 + n] = bad ? __int_as_float(0x7fc00000) : back * static_cast<float>(1 << (8 * n));
+                            }
+                        }
+                    }
+                } else {
+                    if (real) {   // in the order j = 0, 2, 1, 3 of the weights' pairs
+                        uint8_t* dst = smem_raw + row * lay.pitch + (k8 >> 3) * 128 + (k8 & 1) * 64 + ((k8 >> 1) & 3) * 8;
+                        *reinterpret_cast<uint2*>(dst) = make_uint2(__byte_perm(v.x, v.y, 0x5410), __byte_perm(v.x, v.y, 0x7632));
+                        *reinterpret_cast<uint2*>(dst + 32) = make_uint2(__byte_perm(v.z, v.w, 0x5410), __byte_perm(v.z, v.w, 0x7632));
+                    }
+                }
+            }
         bar_group(15, kGemvWarps * 32);
 
-        // lanes of columns without a row read row 0 of x: what they compute is in columns that are not stored
+        // lanes of columns without a row read column 0 of x: what they compute is in columns that are not stored
         const uint8_t* xlane[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) xlane[n] = smem_raw + (n * 8 + g < count ? n * 8 + g : 0) * lay.pitch + t * 32;
-        const float* xslane = xs + 2 * t;
+        for (int n = 0; n < NT; ++n)
+            xlane[n] = smem_raw + (n * 8 + g < count * S::kPerRow ? n * 8 + g : 0) * lay.pitch + t * (S::kBlockBytes / 4);
         float acc[NT][4];
         // the warp's blocks of one slot, kGemvBlocks of them or `nb` at the strip's end
         auto compute = [&](auto full_slot, const uint8_t* blocks, const uint8_t* scales, int kb0, int nb) {
             float c[NT][4] = {};
+            int ci[NT][4] = {};
+            const int at0 = kb0 * 64 / G * kCols + 2 * t;
 #pragma unroll
             for (int u = 0; u < kGemvBlocks; ++u) {
                 if (!full_slot.value && u >= nb) break;
                 const uint4 q = *reinterpret_cast<const uint4*>(blocks + u * 512);
-                uint4 b[NT][2];
+                uint4 b[NT][INT ? 1 : 2];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    b[n][0] = *reinterpret_cast<const uint4*>(xlane[n] + kb0 * 128 + u * 128);
-                    b[n][1] = *reinterpret_cast<const uint4*>(xlane[n] + kb0 * 128 + u * 128 + 16);
-                }
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int h = 0; h < (INT ? 1 : 2); ++h)
+                        b[n][h] = *reinterpret_cast<const uint4*>(xlane[n] + (kb0 + u) * S::kBlockBytes + h * 16);
                 const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    uint32_t a[4];
-                    Q4Frag<T>::expand((&q.x)[s], a);
+                for (int s = 0; s < 4; ++s) {   // 16 k each
                     const bool begins = (s == 0 && (G != 128 || u % 2 == 0)) || (G == 32 && s == 2);
                     const bool ends = (s == 3 && (G != 128 || u % 2 == 1 || (!full_slot.value && u + 1 == nb))) || (G == 32 && s == 1);
+                    const int in_slot = G == 32 ? u * 2 + (s >> 1) : (G == 64 ? u : u >> 1);
+                    if constexpr (INT) {
+                        if (begins)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const uint32_t b0 = (&b[n][s >> 1].x)[2 * (s & 1)], b1 = (&b[n][s >> 1].x)[2 * (s & 1) + 1];
-                        if (begins) mma_16816<T>(c[n], a, b0, b1, zero);
-                        else mma_16816<T>(c[n], a, b0, b1, c[n]);
-                    }
-                    if (ends) {
-                        const int in_slot = G == 32 ? u * 2 + (s >> 1) : (G == 64 ? u : u >> 1);
-                        const float2 f = pair_f32<T>(*reinterpret_cast<const uint32_t*>(scales + in_slot * 32));
-                        const float* xg = xslane + kb0 * (64 * kCols / G) + in_slot * kCols;
+                            for (int n = 0; n < NT; ++n) {
+                                const int2 o = *reinterpret_cast<const int2*>(xi + at0 + in_slot * kCols + n * 8);
+                                ci[n][0] = ci[n][2] = o.x;
+                                ci[n][1] = ci[n][3] = o.y;
+                            }
+                        if (s % 2 == 0) {
+                            const uint32_t w0 = (&q.x)[s], w1 = (&q.x)[s + 1];
+                            const uint32_t a[4] = {w0 & 0x0f0f0f0fu, (w0 >> 4) & 0x0f0f0f0fu, w1 & 0x0f0f0f0fu, (w1 >> 4) & 0x0f0f0f0fu};
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma_16832(ci[n], a, (&b[n][0].x)[s], (&b[n][0].x)[s + 1]);
+                        }
+                    } else {
+                        uint32_t a[4];
+                        Q4Frag<T>::expand((&q.x)[s], a);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            const float2 x = *reinterpret_cast<const float2*>(xg + n * 8);
-                            constexpr float kUp = Q4Frag<T>::kUnitLo / Q4Frag<T>::kUnitHi;   // the high rows' unit, a power of two
-                            acc[n][0] += f.x * (c[n][0] - x.x);
-                            acc[n][1] += f.x * (c[n][1] - x.y);
-                            acc[n][2] += f.y * (c[n][2] - x.x * kUp);
-                            acc[n][3] += f.y * (c[n][3] - x.y * kUp);
+                            const uint32_t b0 = (&b[n][s >> 1].x)[2 * (s & 1)], b1 = (&b[n][s >> 1].x)[2 * (s & 1) + 1];
+                            if (begins) mma_16816<T>(c[n], a, b0, b1, zero);
+                            else mma_16816<T>(c[n], a, b0, b1, c[n]);
+                        }
+                    }
+                    if (ends) {
+                        const float2 f = pair_f32<T>(*reinterpret_cast<const uint32_t*>(scales + in_slot * 32));
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            if constexpr (INT) {
+                                const float2 m = *reinterpret_cast<const float2*>(xf + at0 + in_slot * kCols + n * 8);
+                                acc[n][0] += f.x * (m.x * ci[n][0]);
+                                acc[n][1] += f.x * (m.y * ci[n][1]);
+                                acc[n][2] += f.y * (m.x * ci[n][2]);
+                                acc[n][3] += f.y * (m.y * ci[n][3]);
+                            } else {
+                                acc[n][0] += f.x * c[n][0];
+                                acc[n][1] += f.x * c[n][1];
+                                acc[n][2] += f.y * c[n][2];
+                                acc[n][3] += f.y * c[n][3];
+                            }
                         }
                     }
                 }
@@ -415,15 +528,17 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    mine[(g + (j >> 1) * 8) * (kCols + 1) + n * 8 + 2 * t + (j & 1)] =
-                        acc[n][j] * (j >> 1 ? Q4Frag<T>::kUnitHi : Q4Frag<T>::kUnitLo);
+                    mine[(g + (j >> 1) * 8) * (kCols + 1) + n * 8 + 2 * t + (j & 1)] = acc[n][j];
             bar_group(1 + group, gs * 32);
             // two buffers in turn: this one is written again only after the barrier of the next strip
             for (int i = wig * 32 + lane; i < 16 * count; i += gs * 32) {
                 const int n = i & 15, col = i >> 4;
-                const float* from = part + (flip * kGemvWarps + group * gs) * 16 * (kCols + 1) + n * (kCols + 1) + col;
+                const float* from = part + (flip * kGemvWarps + group * gs) * 16 * (kCols + 1) + n * (kCols + 1) + col * S::kPerRow;
                 float v = 0.f;
-                for (int w = 0; w < gs; ++w) v += from[w * 16 * (kCols + 1)];
+                for (int w = 0; w < gs; ++w, from += 16 * (kCols + 1)) {
+                    if constexpr (INT) v += (from[0] + from[1]) + from[2];   // the smallest byte's sum first
+                    else v += from[0];
+                }
                 if (strip * 16 + n < p.N) {
                     const long long at = rows[col] * p.ldy + strip * 16 + n;
                     if (p.out_f32) static_cast<float*>(p.y)[at] = v;
@@ -440,23 +555,24 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
 struct GemvPlan {
     int unit_rows, depth, bytes;
 };
-template <int NT>
+template <int NT, bool INT>
 GemvPlan gemv_plan(int K, int group, int R, bool indexed) {
-    GemvPlan plan = {R < 8 * NT ? R : 8 * NT, 0, 0};
+    constexpr int most = GemvShape<NT, INT>::kRows;
+    GemvPlan plan = {R < most ? R : most, 0, 0};
     for (; plan.unit_rows > 0; --plan.unit_rows)
         for (plan.depth = 4; plan.depth >= 2; --plan.depth) {
-            plan.bytes = GemvLayout<NT>(q4_kblocks(K), q4_groups(K, group), plan.unit_rows, plan.depth, R, indexed).bytes;
+            plan.bytes = GemvLayout<NT, INT>(q4_kblocks(K), q4_groups(K, group), plan.unit_rows, plan.depth, R, indexed).bytes;
             if (plan.bytes <= kGemvMaxShared) return plan;
         }
     return plan;
 }
 
-template <class T, int NT, int G>
+template <class T, int NT, int G, bool INT>
 cudaError_t gemv_launch(const Q4Params& p, cudaStream_t stream) {
-    auto kern = q4_gemv_kernel<T, NT, G>;
+    auto kern = q4_gemv_kernel<T, NT, G, INT>;
     static std::atomic<bool> configured[kMaxDev];
     if (cudaError_t e = allow_smem(kern, kGemvMaxShared, configured)) return e;
-    const GemvPlan plan = gemv_plan<NT>(p.K, G, p.R, p.index != nullptr);
+    const GemvPlan plan = gemv_plan<NT, INT>(p.K, G, p.R, p.index != nullptr);
     if (plan.unit_rows <= 0) return cudaErrorInvalidValue;   // the entry point has checked q4_gemv_fits
     const int sms = core_sm_count(), kblocks = q4_kblocks(p.K);
     const long long units = p.index ? (p.R < p.E ? p.R : p.E) : (p.R + plan.unit_rows - 1) / plan.unit_rows;   // about
@@ -475,17 +591,21 @@ cudaError_t gemv_launch(const Q4Params& p, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
-template <class T, int NT>
+template <class T, int NT, bool INT>
 cudaError_t gemv_group(const Q4Params& p, cudaStream_t stream) {
-    if (p.group == 32) return gemv_launch<T, NT, 32>(p, stream);
-    return p.group == 64 ? gemv_launch<T, NT, 64>(p, stream) : gemv_launch<T, NT, 128>(p, stream);
+    if (p.group == 32) return gemv_launch<T, NT, 32, INT>(p, stream);
+    return p.group == 64 ? gemv_launch<T, NT, 64, INT>(p, stream) : gemv_launch<T, NT, 128, INT>(p, stream);
 }
 
 template <class T>
 cudaError_t gemv_typed(const Q4Params& p, cudaStream_t stream) {
-    // 16 rows at a time where rows are likely to share a matrix and their x fits
-    const bool two = p.R > 8 && p.R > 4 * p.E && gemv_plan<2>(p.K, p.group, p.R, p.index != nullptr).unit_rows > 8;
-    return two ? gemv_group<T, 2>(p, stream) : gemv_group<T, 1>(p, stream);
+    const bool indexed = p.index != nullptr;
+    // rows that may be expected to share a matrix: with an index the mean over the matrices
+    const int rows = indexed && p.E > 0 ? (p.R + p.E - 1) / p.E : p.R;
+    if (rows <= 2) return gemv_group<T, 1, true>(p, stream);
+    if (rows <= 5 && gemv_plan<2, true>(p.K, p.group, p.R, indexed).unit_rows >= rows) return gemv_group<T, 2, true>(p, stream);
+    const bool two = rows > 8 && gemv_plan<2, false>(p.K, p.group, p.R, indexed).unit_rows > 8;
+    return two ? gemv_group<T, 2, false>(p, stream) : gemv_group<T, 1, false>(p, stream);
 }
 
 unsigned blocks_for(long long work) { return static_cast<unsigned>((work + 127) / 128); }
@@ -506,7 +626,7 @@ cudaError_t q4_unpack_launch(const Q4Params& p, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
-bool q4_gemv_fits(int K, int group, int R, bool indexed) { return gemv_plan<1>(K, group, R, indexed).unit_rows > 0; }
+bool q4_gemv_fits(int K, int group, int R, bool indexed) { return gemv_plan<1, true>(K, group, 1, indexed).unit_rows > 0 && gemv_plan<1, false>(K, group, R, indexed).unit_rows > 0; }
 
 cudaError_t q4_gemv_launch(const Q4Params& p, cudaStream_t stream) {
     return p.bf16 ? gemv_typed<__nv_bfloat16>(p, stream) : gemv_typed<__half>(p, stream);

@@ -1,11 +1,10 @@
 // Matrices of 4-bit integers with group scales: layout, parameter blocks and launchers (launch_q4.cu).
 //
-// A matrix W(n, k) is held as w = (nibble - 8) * scale(n, k / group). The nibbles are laid out for the tensor cores'
-// m16n8k16 instruction: blocks of 16 n x 64 k of 512 bytes, a lane's 16 bytes one after the other. Lane 4 g + t holds
-// rows g and g + 8; its 32-bit word s (the instruction's step s, 16 consecutive k) holds k = 16 s + 4 t + j, j = 0 .. 3, one
-// byte each in the order j = 0, 2, 1, 3, row g in the low nibble and row g + 8 in the high one. So
-// (word >> 4 i) & 0x000f000f is the pair of 16-bit values of operand register i of the instruction (registers 0, 1:
-// j = 0, 1 of rows g, g + 8; registers 2, 3: j = 2, 3). Blocks run along k, then n, then the matrices.
+// A matrix W(n, k) is held as w = (nibble - 8) * scale(n, k / group). The nibbles are laid out for the A fragments of the tensor cores'
+// m16n8k32 (8-bit) and m16n8k16 (16-bit) instructions: blocks of 16 n x 64 k of 512 bytes, a lane's 16 bytes one after the other. Lane
+// 4 g + t holds rows g and g + 8; its 32-bit word w holds k = 16 w + 4 t + j in byte j, row g in the low nibble and row g + 8 in the high
+// one. So word & 0x0f0f0f0f is an operand register of four unsigned bytes, and word & 0x000f000f a pair of 16-bit values (j = 0, 2).
+// Blocks run along k, then n, then the matrices.
 // Scales: 16 for a strip of 16 n in the order g * 2 + (row >= 8), strips along the groups of k, then n, then the matrices.
 // What lies beyond N or K holds nibble 8 and scale 0, so it contributes nothing.
 #pragma once

@@ -279,3 +279,57 @@ def test_experts_of_a_layer_together(lib):
         # the prompt used values rounded to bf16: half a step of 2^-8 of each product's magnitude
         mag = torch.stack([token[i].double().abs() @ back[index[i]].double().abs() for i in range(6)])
         assert ((y.double() - prompt[rows].double()).abs() <= mag * (eps_half(dt) + 64 * 2.0 ** -23)).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("R", [1, 4, 8])
+def test_gemv_ranges_of_x(lib, R, dtype):
+    """Rows of x over the whole range of their type: outliers, numbers near the largest and the smallest, zeros, subnormal numbers.
+    A value may be held to 2^-23 of the largest one in its group of k: that is added to the tolerance."""
+    import torch
+    dt = getattr(torch, dtype)
+    fi = torch.finfo(dt)
+    K, N, group = 448, 48, 64
+    w = matrices(1, K, N, dt, 1, 1e-3)
+    x = matrices(1, R, K, dt, 2)[0].float()
+    x[:, 0:64] *= 2.0 ** -30 if dt == torch.bfloat16 else 2.0 ** -14
+    x[:, 70] = 1000.0
+    x[:, 128:192] = 0
+    x[:, 192:256] = float(fi.max) * 2.0 ** -12 * torch.sign(x[:, 192:256])
+    x[:, 256:320] = fi.smallest_normal * torch.sign(x[:, 256:320])
+    x[:, 320:384] = fi.smallest_normal * fi.eps * torch.sign(x[:, 320:384])
+    x = x.to(dt)
+    y = torch.empty(R, N, dtype=torch.float32, device="cuda")
+    for part in (slice(0, 192), slice(192, 256), slice(256, 448), slice(320, 384), slice(256, 320), slice(0, 448)):
+        only = torch.zeros_like(x)
+        only[:, part] = x[:, part]
+        with on_stream():
+            Q, S = packed(w, group)
+            assert t2sp_b200.q4_gemv(buf(only), buf(Q), buf(S), None, buf(y), Q4Desc(group, 0)) == 0
+        v, u = only.double(), quantised64(w, group)[0]
+        top = v.abs().view(R, K // group, group).amax(2)
+        tol = ((group // 16 + 16) + (K // group + 16)) * 2.0 ** -23 * (v.abs() @ u.abs())
+        tol = tol + 2.0 ** -23 * (top @ u.abs().view(K // group, group, N).sum(1)) + 2.0 ** -140
+        assert ((y.double() - v @ u).abs() <= tol).all(), part
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("R", [1, 8])
+def test_gemv_infinities_and_nan_of_x(lib, R, dtype):
+    """A value of x that is not finite leaves nothing finite in its row; the other rows are as ever."""
+    import torch
+    dt = getattr(torch, dtype)
+    w, x = matrices(1, 192, 40, dt, 1), matrices(1, R, 192, dt, 2)[0]
+    bad = x.clone()
+    bad[R - 1, 100] = float("inf")
+    if R > 1:
+        bad[2, 5] = float("nan")
+    y = torch.empty(R, 40, dtype=torch.float32, device="cuda")
+    with on_stream():
+        Q, S = packed(w, 64)
+        assert t2sp_b200.q4_gemv(buf(bad), buf(Q), buf(S), None, buf(y), Q4Desc(64, 0)) == 0
+    hit = ~bad.isfinite().all(1)
+    assert not y[hit].isfinite().any()
+    if R > 1:
+        rows = (~hit).nonzero().flatten()
+        check_rows(x[rows], quantised64(w, 64), None, y[rows], 64)
