@@ -99,8 +99,10 @@ __global__ void q4_unpack_kernel(const Q4Params p) {
 }
 
 // ---------------------------------------------------------------- products of a few rows
-constexpr int kGemvWarps = 16;                        // that compute; one more brings the weights
-constexpr int kGemvThreads = (kGemvWarps + 1) * 32;
+constexpr int kGemvWarps = 16;                        // that compute
+constexpr int kGemvCopiers = 4;                       // more, that bring the weights: one thread of one warp took longer to issue a
+                                                      // slot's copies, between the other warps' instructions, than the copies (4.0 TB/s)
+constexpr int kGemvThreads = (kGemvWarps + kGemvCopiers) * 32;
 constexpr int kGemvBlocks = 4;                        // blocks of 64 k that a warp computes at a time
 constexpr int kGemvSlot = kGemvBlocks * (512 + 64);   // a warp's share of a slot: its blocks, and up to two groups' scales for each
 constexpr int kGemvMaxShared = 227 << 10;
@@ -207,9 +209,9 @@ struct GemvLayout {
 
 // Y[r] = X[r / per] x W[index[r]]. Work items are (unit, strip of 16 n), where a unit is up to `unit_rows` rows that name one matrix:
 // a matrix is read once for all of them. Every CTA takes an equal run of consecutive items, stages a unit's rows of x in shared memory once, with
-// the sums of x over each group of k, and lets groups of `gs` warps compute a strip each. One warp
-// brings packed weights and scales with bulk copies, gs * kGemvBlocks blocks of a strip at a time into a ring of `depth` slots for each
-// group, and runs ahead over strip and unit ends. A computing warp turns 16 bytes a lane into A fragments, sums a group of k in the
+// the sums of x over each group of k, and lets groups of `gs` warps compute a strip each. Other warps
+// bring packed weights and scales with bulk copies, gs * kGemvBlocks blocks of a strip at a time into a ring of `depth` slots for each
+// group, and run ahead over strip and unit ends. A computing warp turns 16 bytes a lane into A fragments, sums a group of k in the
 // instruction's accumulators, and adds the scaled sum in fp32. The gs partial sums of a strip meet in shared memory in a fixed order.
 template <class T, int NT, int G, bool INT>
 __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params p, int gs, int unit_rows, int depth) {
@@ -258,7 +260,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
                 n += __popc(starts);
                 __syncwarp();
             }
-            if (lane == 0) count_slot[1] = n;   // a word of its own: the other one is written again while the copying warp reads this
+            if (lane == 0) count_slot[1] = n;   // a word of its own: the other one is written again while the copying warps read this
         }
         __syncthreads();
         num_units = count_slot[1];
@@ -274,37 +276,47 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
     const int chunks = (kblocks + chunk - 1) / chunk;           // slots of a strip
     int tries = kGemvTries;   // a wait that runs out is reported, and the rest of the call's waits do not block (its results are lost)
 
-    if (warp == kGemvWarps) {
-        // ------------------------------------------------------------ brings the weights, group after group as slots become free
+    if (warp >= kGemvWarps) {
+        // ------------------------------------------------------------ copying warps: each takes every `share`-th slot of one group
         if (lane != 0) return;
-        uint32_t fill[4] = {0, 0, 0, 0};   // slots filled so far, by group
-        const int q_last = (kblocks - (chunks - 1) * chunk) * 512;
-        const int s_full = chunk * 64 / G * 32, s_last = (groups - (chunks - 1) * (chunk * 64 / G)) * 32;
+        // a slot stays with one of them (`share` divides `depth`): a wait on the parity of its barrier must not miss a phase
+        const int gr = (warp - kGemvWarps) % num_groups, mine = (warp - kGemvWarps) / num_groups;
+        int share = kGemvCopiers / num_groups;
+        while (depth % share) --share;
+        if (mine >= share) return;
+        uint64_t* full = bars + gr * depth;
+        uint64_t* freed = full + num_groups * depth;
+        uint8_t* ring = smem_raw + lay.ring + gr * depth * slot_bytes;
+        const int q_full = chunk * 512, q_last = (kblocks - (chunks - 1) * chunk) * 512;
+        const int s_full = chunk * 64 / G * 32, s_last = groups * 32 - (chunks - 1) * s_full;
+        int turn = 0, slot = 0;          // slots of the group so far, modulo `share` and `depth`
+        uint32_t phase = 1;              // the first round finds every slot free
         while (item < item_end) {
             const int unit = static_cast<int>(item / strips);
             const int s_begin = static_cast<int>(item % strips);
             const int s_end = static_cast<int>(min(static_cast<long long>(strips), s_begin + (item_end - item)));
             item += s_end - s_begin;
             const int e = p.index ? idx[units[unit]] : 0;
-            // strips s_begin + i go to group i % num_groups; the groups' slots are filled in turn
-            for (int s0 = s_begin; s0 < s_end; s0 += num_groups)
-                for (int c = 0; c < chunks; ++c) {
-                    const int qb = c + 1 == chunks ? q_last : chunk * 512, sb = c + 1 == chunks ? s_last : s_full;
-                    for (int gr = 0; gr < num_groups && s0 + gr < s_end; ++gr) {
-                        const long long strip = static_cast<long long>(e) * strips + s0 + gr;
-                        const int slot = gr * depth + static_cast<int>(fill[gr] % depth);
-                        const uint32_t phase = (fill[gr] / depth) & 1;
-                        ++fill[gr];
-                        while (!ptx::mbar_try_wait(&bars[num_groups * depth + slot], phase ^ 1)) {
+            for (int strip = s_begin + gr; strip < s_end; strip += num_groups) {
+                const long long at = static_cast<long long>(e) * strips + strip;
+                const uint8_t* q = p.q + at * kblocks * 512;
+                const uint8_t* s = reinterpret_cast<const uint8_t*>(p.s) + at * groups * 32;
+                for (int c = 1; c <= chunks; ++c, q += q_full, s += s_full) {
+                    if (turn == mine) {
+                        while (!ptx::mbar_try_wait(&freed[slot], phase)) {
                             if (tries <= 0) break;
                             if (--tries == 0) atomicOr(p.status, ST_TIMEOUT_PRODUCER);
                         }
-                        uint8_t* dst = smem_raw + lay.ring + slot * slot_bytes;
-                        ptx::mbar_expect_tx(&bars[slot], qb + sb);
-                        ptx::bulk_load(dst, p.q + (strip * kblocks + c * chunk) * 512, qb, &bars[slot]);
-                        ptx::bulk_load(dst + chunk * 512, p.s + (strip * groups + c * (chunk * 64 / G)) * 16, sb, &bars[slot]);
+                        const int qb = c == chunks ? q_last : q_full, sb = c == chunks ? s_last : s_full;
+                        uint8_t* dst = ring + slot * slot_bytes;
+                        ptx::mbar_expect_tx(&full[slot], qb + sb);
+                        ptx::bulk_load(dst, q, qb, &full[slot]);
+                        ptx::bulk_load(dst + q_full, s, sb, &full[slot]);
                     }
+                    if (++turn == share) turn = 0;
+                    if (++slot == depth) { slot = 0; phase ^= 1u; }
                 }
+            }
         }
         return;
     }
