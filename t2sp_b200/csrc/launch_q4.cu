@@ -20,94 +20,6 @@ template <> __device__ __forceinline__ float rounded<float>(float v) { return v;
 template <> __device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half rounded<__half>(float v) { return __float2half_rn(v); }
 
-// Byte of (row pair g, g + 8; k) inside the packed matrices.
-__device__ __forceinline__ long long q4_byte(int e, int strip, int g, int k, int kblocks, int strips) {
-    const int kk = k & 63, j = kk & 3;
-    return ((static_cast<long long>(e) * strips + strip) * kblocks + (k >> 6)) * 512 + (g * 4 + ((kk >> 2) & 3)) * 16 +
-           (kk >> 4) * 4 + j;
-}
-
-// The nearest of -7 .. 7 to v / scale, ties to even. The quotient of two 16-bit values cannot round onto a tie that
-// the exact quotient does not hold: a tie (h + 1/2) * scale has at most 15 significant bits, so an unequal v differs
-// from it by more than 2^-17 relative, far above the division's 2^-24.
-__device__ __forceinline__ int q4_round(float v, float scale) {
-    if (!(scale > 0.f)) return 0;
-    const float q = rintf(__fdiv_rn(v, scale));
-    return static_cast<int>(fminf(fmaxf(q, -7.f), 7.f));  // a NaN becomes -7; its scale is not a number either
-}
-
-// One thread for the row pair (g, g + 8) of a strip and one group of k.
-template <class T>
-__global__ void q4_pack_kernel(const Q4Params p) {
-    const int kblocks = q4_kblocks(p.K), strips = q4_strips(p.N), groups = q4_groups(p.K, p.group);
-    const long long idx = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
-    const int g = static_cast<int>(idx & 7);
-    long long rest = idx >> 3;
-    const int strip = static_cast<int>(rest % strips);
-    rest /= strips;
-    const int grp = static_cast<int>(rest % groups), e = static_cast<int>(rest / groups);
-    if (e >= p.E) return;
-    const T* w = static_cast<const T*>(p.w) + e * p.bs_w;
-    auto load = [&](int n, long long k) {
-        if (n >= p.N || k >= p.K) return 0.f;
-        return to_f32(p.trans_b ? w[n * p.ldw + k] : w[k * p.ldw + n]);
-    };
-    const int k0 = grp * p.group, k1 = min(k0 + p.group, kblocks * 64);
-    float scale[2];
-    for (int h = 0; h < 2; ++h) {
-        float m = 0.f;
-        bool nan = false;
-        for (int k = k0; k < k1; ++k) {
-            const float v = fabsf(load(strip * 16 + g + 8 * h, k));
-            nan = nan || v != v;
-            m = fmaxf(m, v);
-        }
-        const T s = rounded<T>(nan ? __int_as_float(0x7fc00000) : __fdiv_rn(m, 7.f));
-        scale[h] = to_f32(s);
-        reinterpret_cast<T*>(p.s)[((static_cast<long long>(e) * strips + strip) * groups + grp) * 16 + g * 2 + h] = s;
-    }
-    for (int k = k0; k < k1; ++k) {
-        const int lo = q4_round(load(strip * 16 + g, k), scale[0]) + 8, hi = q4_round(load(strip * 16 + g + 8, k), scale[1]) + 8;
-        p.q[q4_byte(e, strip, g, k, kblocks, strips)] = static_cast<uint8_t>(lo | (hi << 4));
-    }
-}
-
-__device__ __forceinline__ int q4_value(const Q4Params& p, int e, int n, int k, int kblocks, int strips) {
-    const int row = n & 15;
-    const int b = p.q[q4_byte(e, n >> 4, row & 7, k, kblocks, strips)];
-    return ((row >> 3) ? b >> 4 : b & 15) - 8;
-}
-template <class T>
-__device__ __forceinline__ float q4_scale(const Q4Params& p, int e, int n, int k, int strips, int groups) {
-    const int row = n & 15;
-    return to_f32(reinterpret_cast<const T*>(p.s)[((static_cast<long long>(e) * strips + (n >> 4)) * groups + k / p.group) * 16 +
-                                                  (row & 7) * 2 + (row >> 3)]);
-}
-
-template <class T>
-__global__ void q4_unpack_kernel(const Q4Params p) {
-    const int kblocks = q4_kblocks(p.K), strips = q4_strips(p.N), groups = q4_groups(p.K, p.group);
-    const long long idx = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
-    const int inner = p.trans_b ? p.K : p.N, outer = p.trans_b ? p.N : p.K;
-    const int i = static_cast<int>(idx % inner);
-    const long long rest = idx / inner;
-    const int o = static_cast<int>(rest % outer), e = static_cast<int>(rest / outer);
-    if (e >= p.E) return;
-    const int n = p.trans_b ? o : i, k = p.trans_b ? i : o;
-    const float v = q4_value(p, e, n, k, kblocks, strips) * q4_scale<T>(p, e, n, k, strips, groups);
-    static_cast<T*>(p.wout)[e * p.bs_w + o * p.ldw + i] = rounded<T>(v);
-}
-
-// ---------------------------------------------------------------- products of a few rows
-constexpr int kGemvWarps = 16;                        // that compute
-constexpr int kGemvCopiers = 4;                       // more, that bring the weights: one thread of one warp took longer to issue a
-                                                      // slot's copies, between the other warps' instructions, than the copies (4.0 TB/s)
-constexpr int kGemvThreads = (kGemvWarps + kGemvCopiers) * 32;
-constexpr int kGemvBlocks = 4;                        // blocks of 64 k that a warp computes at a time
-constexpr int kGemvSlot = kGemvBlocks * (512 + 64);   // a warp's share of a slot: its blocks, and up to two groups' scales for each
-constexpr int kGemvMaxShared = 227 << 10;
-constexpr int kGemvTries = 1 << 17;                   // a wait gives up after this many tests of up to 16 us
-
 // The sixteen integers q - 8 of a lane's word as 16-bit floating-point A-fragment registers, exactly: the nibbles become low mantissa
 // bits of a number whose last bit counts 1 (128 in bf16, 1024 in fp16; fp16 has room for the second nibble as it stands, counting
 // 16), and one packed operation takes the constant off. (Leaving fp16 nibbles as subnormal numbers and the constant to the sums of x
@@ -145,6 +57,260 @@ template <> struct Q4Frag<__nv_bfloat16> {
     }
 };
 
+template <class T> __device__ __forceinline__ float2 pair_f32(uint32_t w);
+template <> __device__ __forceinline__ float2 pair_f32<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <> __device__ __forceinline__ float2 pair_f32<__nv_bfloat16>(uint32_t w) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+}
+
+// ---------------------------------------------------------------- quantising and reading back
+// Both kernels pass tiles of 128 k x 128 n through shared memory: whole rows of W on the one side, a warp's strip of 16 n with its
+// 16 bytes a lane on the other. They are bound by memory: 2 bytes a weight, and 0.5 + 2 / group.
+constexpr int kTile = 128;
+template <bool TRANS>
+struct Q4Tile {
+    // pitch in bytes, so that a strip's accesses (eight n, four k apart) meet different banks: [k][n], 2-byte accesses, four rows
+    // 32 bytes apart modulo 128; [n][k], 8-byte accesses, rows 32 bytes apart
+    static constexpr int kPitch = TRANS ? kTile * 2 + 32 : kTile * 2 + 8;
+};
+
+// Rows of W between global memory and the tile. Outside the matrix the tile holds zeros.
+template <bool TRANS, bool STORE>
+__device__ __forceinline__ void tile_rows(const Q4Params& p, uint16_t* w, uint8_t* tile, int n0, int k0) {
+    const int inner = TRANS ? p.K : p.N, outer = TRANS ? p.N : p.K, i0 = TRANS ? k0 : n0, o0 = TRANS ? n0 : k0;
+    const bool aligned = (reinterpret_cast<uintptr_t>(w) & 15) == 0 && p.ldw % 8 == 0;
+    constexpr int kSteps = kTile * 16 / 256;
+    uint4 v[kSteps];
+    if constexpr (!STORE) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int c = s * 256 + threadIdx.x, o = o0 + (c >> 4), i = i0 + (c & 15) * 8;
+            const uint16_t* src = w + o * p.ldw + i;
+            v[s] = make_uint4(0, 0, 0, 0);
+            if (o >= outer) continue;
+            if (aligned && i + 8 <= inner) {
+                asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(v[s].x), "=r"(v[s].y), "=r"(v[s].z), "=r"(v[s].w) : "l"(src));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (i + j < inner) (&v[s].x)[j >> 1] |= static_cast<uint32_t>(src[j]) << (16 * (j & 1));
+            }
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        const int c = s * 256 + threadIdx.x, o = o0 + (c >> 4), i = i0 + (c & 15) * 8;
+        uint2* at = reinterpret_cast<uint2*>(tile + (c >> 4) * Q4Tile<TRANS>::kPitch + (c & 15) * 16);   // 8-byte aligned rows
+        if constexpr (!STORE) {
+            at[0] = make_uint2(v[s].x, v[s].y);
+            at[1] = make_uint2(v[s].z, v[s].w);
+        } else {
+            if (o >= outer || i >= inner) continue;
+            const uint2 lo = at[0], hi = at[1];
+            uint16_t* dst = w + o * p.ldw + i;
+            if (aligned && i + 8 <= inner) {
+                *reinterpret_cast<uint4*>(dst) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            } else {
+                const uint32_t words[4] = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (i + j < inner) dst[j] = static_cast<uint16_t>(words[j >> 1] >> (16 * (j & 1)));
+            }
+        }
+    }
+}
+
+// Four consecutive k (16 w + 4 t .. + 3 of block b) of row n of the tile, as two packed pairs.
+template <bool TRANS>
+__device__ __forceinline__ uint2 tile_get(const uint8_t* tile, int n, int k) {
+    if constexpr (TRANS) {
+        return *reinterpret_cast<const uint2*>(tile + n * Q4Tile<TRANS>::kPitch + k * 2);
+    } else {
+        const uint16_t* c = reinterpret_cast<const uint16_t*>(tile + k * Q4Tile<TRANS>::kPitch) + n;
+        constexpr int kRow = Q4Tile<TRANS>::kPitch / 2;
+        return make_uint2(c[0] | (static_cast<uint32_t>(c[kRow]) << 16), c[2 * kRow] | (static_cast<uint32_t>(c[3 * kRow]) << 16));
+    }
+}
+template <bool TRANS>
+__device__ __forceinline__ void tile_put(uint8_t* tile, int n, int k, uint2 v) {
+    if constexpr (TRANS) {
+        *reinterpret_cast<uint2*>(tile + n * Q4Tile<TRANS>::kPitch + k * 2) = v;
+    } else {
+        uint16_t* c = reinterpret_cast<uint16_t*>(tile + k * Q4Tile<TRANS>::kPitch) + n;
+        constexpr int kRow = Q4Tile<TRANS>::kPitch / 2;
+        c[0] = static_cast<uint16_t>(v.x);
+        c[kRow] = static_cast<uint16_t>(v.x >> 16);
+        c[2 * kRow] = static_cast<uint16_t>(v.y);
+        c[3 * kRow] = static_cast<uint16_t>(v.y >> 16);
+    }
+}
+
+template <class T> struct Pair16;
+template <> struct Pair16<__half> { using type = __half2; };
+template <> struct Pair16<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <class T>
+__device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t v) {   // of each 16-bit half; a NaN stays
+    using P = typename Pair16<T>::type;
+    const P r = __hmax2_nan(*reinterpret_cast<const P*>(&m), __habs2(*reinterpret_cast<const P*>(&v)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// v / scale rounded to the nearest integer, ties to even, plus kNibble0, as the bits of a float: the integer is in the last bits. `inv` = 1 / scale,
+// or 0 for a scale of 0. v * inv is off the quotient by less than 2^-20, and a quotient that is no tie is at
+// least 2^-12 away from one: v and scale are integers a, b < 2^11 times powers of two, |v / scale - (h + 1/2)| = |2 v - (2 h + 1) scale| / (2
+// scale), and the numerator is a multiple of the scale's last bit. So the product rounded to a multiple of 2^-14 (by the first sum, whose last
+// bit that is) is a tie exactly where the quotient is one. A normal scale is at least (1 - 2^-8) max / 7, so the integer is within
+// -7 .. 7; subnormal scales, those whose inverse leaves fp32 and those that
+// are not finite take the division.
+constexpr uint32_t kNibble0 = 0x4b400008u;   // 1.5 * 2^23 + 8
+__device__ __forceinline__ uint32_t q4_nibble(float v, float inv) {
+    return __float_as_uint(__fadd_rn(__fmaf_rn(v, inv, 768.f), 12582920.f - 768.f));
+}
+__device__ __noinline__ uint32_t q4_nibble_any(float v, float scale) {
+    if (!(scale > 0.f) || scale == __int_as_float(0x7f800000)) return kNibble0;
+    const float r = fminf(fmaxf(rintf(__fdiv_rn(v, scale)), -7.f), 7.f);   // the quotient of 16-bit values cannot round onto a tie, see above
+    return __float_as_uint(__fadd_rn(r, 12582920.f));
+}
+
+template <class T, bool TRANS>
+__global__ void __launch_bounds__(256) q4_pack_kernel(const Q4Params p) {
+    __shared__ __align__(16) uint8_t tile[kTile * Q4Tile<TRANS>::kPitch];
+    const int kblocks = q4_kblocks(p.K), strips = q4_strips(p.N), groups = q4_groups(p.K, p.group);
+    const int ntiles = (strips + 7) / 8, ktiles = (kblocks + 1) / 2;
+    // tiles along W's rows run fastest
+    const int x = blockIdx.x % (TRANS ? ktiles : ntiles), y = blockIdx.x / (TRANS ? ktiles : ntiles);
+    const int kt = TRANS ? x : y % ktiles, nt = TRANS ? y % ntiles : x, e = y / (TRANS ? ntiles : ktiles);
+    tile_rows<TRANS, false>(p, const_cast<uint16_t*>(static_cast<const uint16_t*>(p.w)) + e * p.bs_w, tile, nt * kTile, kt * kTile);
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int strip = nt * 8 + warp;
+    if (strip >= strips) return;
+    uint2 v[2][4][2];          // [block][word][row g, g + 8]: four k
+    uint32_t top[2][2][2];     // [block][half of the block][row]: largest magnitude in either half of the word
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int w = 2 * h; w < 2 * h + 2; ++w) {
+                    v[b][w][r] = tile_get<TRANS>(tile, warp * 16 + g + 8 * r, b * 64 + 16 * w + 4 * t);
+                    m = max_abs2<T>(max_abs2<T>(m, v[b][w][r].x), v[b][w][r].y);
+                }
+                m = max_abs2<T>(m, __byte_perm(m, m, 0x1032));
+                m = max_abs2<T>(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                top[b][h][r] = max_abs2<T>(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            }
+    uint8_t* q = p.q + ((static_cast<long long>(e) * strips + strip) * kblocks + kt * 2) * 512 + lane * 16;
+    uint16_t* s = p.s + (static_cast<long long>(e) * strips + strip) * groups * 16;
+    float inv[2][2][2], scale[2][2][2];
+    bool any = false;   // a scale that needs the division
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t word = 0;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                uint32_t m = top[b][h][r];
+                if (p.group >= 64) m = max_abs2<T>(m, top[b][h ^ 1][r]);
+                if (p.group == 128) m = max_abs2<T>(max_abs2<T>(m, top[b ^ 1][0][r]), top[b ^ 1][1][r]);
+                const T sc = rounded<T>(__fdiv_rn(pair_f32<T>(m).x, 7.f));
+                word |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&sc)) << (16 * r);
+                const float f = to_f32(sc);
+                any = any || !(f < __int_as_float(0x7f800000)) || (f > 0.f && f < (std::is_same<T, __half>::value ? 0x1p-14f : 0x1p-100f));
+                inv[b][h][r] = f > 0.f ? __frcp_rn(f) : 0.f;
+                scale[b][h][r] = f;
+            }
+            const int group = (kt * 128 + b * 64 + h * 32) / p.group;
+            if (t == 0 && group < groups && (kt * 128 + b * 64 + h * 32) % p.group == 0)
+                *reinterpret_cast<uint32_t*>(s + group * 16 + g * 2) = word;
+        }
+    any = __any_sync(0xffffffffu, any);
+    // the words: integers shifted into place and added up, with the constant part of their bits taken off
+    auto words = [&](auto nibble, int b) {
+        uint4 out;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            uint32_t word = 0;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float2 lo = pair_f32<T>(v[b][w][r].x), hi = pair_f32<T>(v[b][w][r].y);
+                const float f[4] = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) word += (nibble(f[j], b, w >> 1, r) - (kNibble0 & ~15u)) << (8 * j + 4 * r);
+            }
+            (&out.x)[w] = word;
+        }
+        *reinterpret_cast<uint4*>(q + b * 512) = out;
+    };
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        if (kt * 2 + b >= kblocks) break;
+        if (!any) words([&](float f, int b, int h, int r) { return q4_nibble(f, inv[b][h][r]); }, b);
+        else words([&](float f, int b, int h, int r) { return q4_nibble_any(f, scale[b][h][r]); }, b);
+    }
+}
+
+template <class T, bool TRANS>
+__global__ void __launch_bounds__(256) q4_unpack_kernel(const Q4Params p) {
+    using P = typename Pair16<T>::type;
+    __shared__ __align__(16) uint8_t tile[kTile * Q4Tile<TRANS>::kPitch];
+    const int kblocks = q4_kblocks(p.K), strips = q4_strips(p.N), groups = q4_groups(p.K, p.group);
+    const int ntiles = (strips + 7) / 8, ktiles = (kblocks + 1) / 2;
+    const int x = blockIdx.x % (TRANS ? ktiles : ntiles), y = blockIdx.x / (TRANS ? ktiles : ntiles);
+    const int kt = TRANS ? x : y % ktiles, nt = TRANS ? y % ntiles : x, e = y / (TRANS ? ntiles : ktiles);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int strip = nt * 8 + warp;
+    if (strip < strips) {
+        const uint8_t* q = p.q + ((static_cast<long long>(e) * strips + strip) * kblocks + kt * 2) * 512 + lane * 16;
+        const uint16_t* s = p.s + (static_cast<long long>(e) * strips + strip) * groups * 16 + g * 2;
+        uint4 v[2];
+        uint32_t sc[2][2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            if (kt * 2 + b >= kblocks) break;
+            v[b] = *reinterpret_cast<const uint4*>(q + b * 512);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) sc[b][h] = *reinterpret_cast<const uint32_t*>(s + (kt * 128 + b * 64 + h * 32) / p.group * 16);
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            if (kt * 2 + b >= kblocks) break;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t a[4];   // rows g, g + 8 with k = 0, 2 and 1, 3 of the four
+                Q4Frag<T>::expand((&v[b].x)[w], a);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    // an integer of three bits times a 16-bit scale, rounded once
+                    const uint32_t f = __byte_perm(sc[b][w >> 1], 0, r ? 0x3232 : 0x1010);
+                    const P lo = __hmul2(*reinterpret_cast<const P*>(&a[r]), *reinterpret_cast<const P*>(&f));
+                    const P hi = __hmul2(*reinterpret_cast<const P*>(&a[2 + r]), *reinterpret_cast<const P*>(&f));
+                    const uint32_t l = *reinterpret_cast<const uint32_t*>(&lo), h = *reinterpret_cast<const uint32_t*>(&hi);
+                    tile_put<TRANS>(tile, warp * 16 + g + 8 * r, b * 64 + 16 * w + 4 * t,
+                                    make_uint2(__byte_perm(l, h, 0x5410), __byte_perm(l, h, 0x7632)));
+                }
+            }
+        }
+    }
+    __syncthreads();
+    tile_rows<TRANS, true>(p, static_cast<uint16_t*>(p.wout) + e * p.bs_w, tile, nt * kTile, kt * kTile);
+}
+
+// ---------------------------------------------------------------- products of a few rows
+constexpr int kGemvWarps = 16;                        // that compute
+constexpr int kGemvCopiers = 4;                       // more, that bring the weights: one thread of one warp took longer to issue a
+                                                      // slot's copies, between the other warps' instructions, than the copies (4.0 TB/s)
+constexpr int kGemvThreads = (kGemvWarps + kGemvCopiers) * 32;
+constexpr int kGemvBlocks = 4;                        // blocks of 64 k that a warp computes at a time
+constexpr int kGemvSlot = kGemvBlocks * (512 + 64);   // a warp's share of a slot: its blocks, and up to two groups' scales for each
+constexpr int kGemvMaxShared = 227 << 10;
+constexpr int kGemvTries = 1 << 17;                   // a wait gives up after this many tests of up to 16 us
+
 // Integers: sixteen k of unsigned nibbles against signed bytes of x, exact in 32 bits.
 __device__ __forceinline__ void mma_16832(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -165,12 +331,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
 }
 
 __device__ __forceinline__ void bar_group(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-
-template <class T> __device__ __forceinline__ float2 pair_f32(uint32_t w);
-template <> __device__ __forceinline__ float2 pair_f32<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
-template <> __device__ __forceinline__ float2 pair_f32<__nv_bfloat16>(uint32_t w) {
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
-}
 
 // Two ways to multiply, by the number of rows that share a pass over the weights.
 //   INT  a few rows: the weights stay unsigned nibbles, whose offset 8 the sum of x over the group takes out, and x is written, group by group of k, as 24-bit integers times a power of two, in three signed bytes, and each byte is a column of
@@ -620,21 +780,33 @@ cudaError_t gemv_typed(const Q4Params& p, cudaStream_t stream) {
     return two ? gemv_group<T, 2, false>(p, stream) : gemv_group<T, 1, false>(p, stream);
 }
 
-unsigned blocks_for(long long work) { return static_cast<unsigned>((work + 127) / 128); }
+unsigned tiles_for(const Q4Params& p) {
+    return static_cast<unsigned>(static_cast<long long>((q4_strips(p.N) + 7) / 8) * ((q4_kblocks(p.K) + 1) / 2) * p.E);
+}
 
 }  // namespace
 
 cudaError_t q4_pack_launch(const Q4Params& p, cudaStream_t stream) {
-    const long long work = 8ll * q4_strips(p.N) * q4_groups(p.K, p.group) * p.E;
-    if (p.bf16) q4_pack_kernel<__nv_bfloat16><<<blocks_for(work), 128, 0, stream>>>(p);
-    else q4_pack_kernel<__half><<<blocks_for(work), 128, 0, stream>>>(p);
+    const unsigned grid = tiles_for(p);
+    if (p.bf16) {
+        if (p.trans_b) q4_pack_kernel<__nv_bfloat16, true><<<grid, 256, 0, stream>>>(p);
+        else q4_pack_kernel<__nv_bfloat16, false><<<grid, 256, 0, stream>>>(p);
+    } else {
+        if (p.trans_b) q4_pack_kernel<__half, true><<<grid, 256, 0, stream>>>(p);
+        else q4_pack_kernel<__half, false><<<grid, 256, 0, stream>>>(p);
+    }
     return cudaGetLastError();
 }
 
 cudaError_t q4_unpack_launch(const Q4Params& p, cudaStream_t stream) {
-    const long long work = static_cast<long long>(p.E) * p.K * p.N;
-    if (p.bf16) q4_unpack_kernel<__nv_bfloat16><<<blocks_for(work), 128, 0, stream>>>(p);
-    else q4_unpack_kernel<__half><<<blocks_for(work), 128, 0, stream>>>(p);
+    const unsigned grid = tiles_for(p);
+    if (p.bf16) {
+        if (p.trans_b) q4_unpack_kernel<__nv_bfloat16, true><<<grid, 256, 0, stream>>>(p);
+        else q4_unpack_kernel<__nv_bfloat16, false><<<grid, 256, 0, stream>>>(p);
+    } else {
+        if (p.trans_b) q4_unpack_kernel<__half, true><<<grid, 256, 0, stream>>>(p);
+        else q4_unpack_kernel<__half, false><<<grid, 256, 0, stream>>>(p);
+    }
     return cudaGetLastError();
 }
 
