@@ -81,6 +81,30 @@ __device__ __forceinline__ void tile_rows(const Q4Params& p, uint16_t* w, uint8_
     const bool aligned = (reinterpret_cast<uintptr_t>(w) & 15) == 0 && p.ldw % 8 == 0;
     constexpr int kSteps = kTile * 16 / 256;
     uint4 v[kSteps];
+    const int c0 = threadIdx.x, step = 16 * Q4Tile<TRANS>::kPitch;
+    uint8_t* mine = tile + (c0 >> 4) * Q4Tile<TRANS>::kPitch + (c0 & 15) * 16;
+    if (aligned && o0 + kTile <= outer && i0 + kTile <= inner) {   // a whole tile
+        uint16_t* at = w + (o0 + (c0 >> 4)) * p.ldw + i0 + (c0 & 15) * 8;
+        const long long rows = 16 * p.ldw;
+        if constexpr (!STORE) {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+                asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(v[s].x), "=r"(v[s].y), "=r"(v[s].z), "=r"(v[s].w) : "l"(at + s * rows));
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            uint2* m = reinterpret_cast<uint2*>(mine + s * step);
+            if constexpr (!STORE) {
+                m[0] = make_uint2(v[s].x, v[s].y);
+                m[1] = make_uint2(v[s].z, v[s].w);
+            } else {
+                const uint2 lo = m[0], hi = m[1];
+                *reinterpret_cast<uint4*>(at + s * rows) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            }
+        }
+        return;
+    }
     if constexpr (!STORE) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
@@ -173,10 +197,10 @@ __device__ __noinline__ uint32_t q4_nibble_any(float v, float scale) {
     return __float_as_uint(__fadd_rn(r, 12582920.f));
 }
 
-template <class T, bool TRANS>
+template <class T, bool TRANS, int G>
 __global__ void __launch_bounds__(256) q4_pack_kernel(const Q4Params p) {
     __shared__ __align__(16) uint8_t tile[kTile * Q4Tile<TRANS>::kPitch];
-    const int kblocks = q4_kblocks(p.K), strips = q4_strips(p.N), groups = q4_groups(p.K, p.group);
+    const int kblocks = q4_kblocks(p.K), strips = q4_strips(p.N), groups = q4_groups(p.K, G);
     const int ntiles = (strips + 7) / 8, ktiles = (kblocks + 1) / 2;
     // tiles along W's rows run fastest
     const int x = blockIdx.x % (TRANS ? ktiles : ntiles), y = blockIdx.x / (TRANS ? ktiles : ntiles);
@@ -206,29 +230,27 @@ __global__ void __launch_bounds__(256) q4_pack_kernel(const Q4Params p) {
             }
     uint8_t* q = p.q + ((static_cast<long long>(e) * strips + strip) * kblocks + kt * 2) * 512 + lane * 16;
     uint16_t* s = p.s + (static_cast<long long>(e) * strips + strip) * groups * 16;
-    float inv[2][2][2], scale[2][2][2];
+    // [group of the tile's 128 k][row]. max / 7 in 16 bits: the fp32 product with 1 / 7 is off by 2^-23, and a quotient by 7 of a 16-bit number
+    // is at least 1 / 14 of a last place (2^-15 relative) away from where its rounding to 16 bits would change.
+    constexpr int kGroups = 128 / G;
+    float inv[kGroups][2], scale[kGroups][2];
     bool any = false;   // a scale that needs the division
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int i = 0; i < kGroups; ++i) {
+        uint32_t word = 0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            uint32_t word = 0;
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                uint32_t m = top[b][h][r];
-                if (p.group >= 64) m = max_abs2<T>(m, top[b][h ^ 1][r]);
-                if (p.group == 128) m = max_abs2<T>(max_abs2<T>(m, top[b ^ 1][0][r]), top[b ^ 1][1][r]);
-                const T sc = rounded<T>(__fdiv_rn(pair_f32<T>(m).x, 7.f));
-                word |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&sc)) << (16 * r);
-                const float f = to_f32(sc);
-                any = any || !(f < __int_as_float(0x7f800000)) || (f > 0.f && f < (std::is_same<T, __half>::value ? 0x1p-14f : 0x1p-100f));
-                inv[b][h][r] = f > 0.f ? __frcp_rn(f) : 0.f;
-                scale[b][h][r] = f;
-            }
-            const int group = (kt * 128 + b * 64 + h * 32) / p.group;
-            if (t == 0 && group < groups && (kt * 128 + b * 64 + h * 32) % p.group == 0)
-                *reinterpret_cast<uint32_t*>(s + group * 16 + g * 2) = word;
+        for (int r = 0; r < 2; ++r) {
+            uint32_t m = G == 32 ? top[i >> 1][i & 1][r] : max_abs2<T>(top[i % 2][0][r], top[i % 2][1][r]);
+            if (G == 128) m = max_abs2<T>(max_abs2<T>(m, top[1][0][r]), top[1][1][r]);
+            const T sc = rounded<T>(pair_f32<T>(m).x * (1.f / 7.f));
+            word |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&sc)) << (16 * r);
+            const float f = to_f32(sc);
+            any = any || !(f < __int_as_float(0x7f800000)) || (f > 0.f && f < (std::is_same<T, __half>::value ? 0x1p-14f : 0x1p-100f));
+            inv[i][r] = f > 0.f ? __fdividef(1.f, f) : 0.f;
+            scale[i][r] = f;
         }
+        if (t == 0 && kt * kGroups + i < groups) *reinterpret_cast<uint32_t*>(s + (kt * kGroups + i) * 16 + g * 2) = word;
+    }
     any = __any_sync(0xffffffffu, any);
     // the words: integers shifted into place and added up, with the constant part of their bits taken off
     auto words = [&](auto nibble, int b) {
@@ -241,7 +263,7 @@ __global__ void __launch_bounds__(256) q4_pack_kernel(const Q4Params p) {
                 const float2 lo = pair_f32<T>(v[b][w][r].x), hi = pair_f32<T>(v[b][w][r].y);
                 const float f[4] = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) word += (nibble(f[j], b, w >> 1, r) - (kNibble0 & ~15u)) << (8 * j + 4 * r);
+                for (int j = 0; j < 4; ++j) word += (nibble(f[j], G == 32 ? b * 2 + (w >> 1) : (G == 64 ? b : 0), r) - (kNibble0 & ~15u)) << (8 * j + 4 * r);
             }
             (&out.x)[w] = word;
         }
@@ -250,8 +272,8 @@ __global__ void __launch_bounds__(256) q4_pack_kernel(const Q4Params p) {
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
         if (kt * 2 + b >= kblocks) break;
-        if (!any) words([&](float f, int b, int h, int r) { return q4_nibble(f, inv[b][h][r]); }, b);
-        else words([&](float f, int b, int h, int r) { return q4_nibble_any(f, scale[b][h][r]); }, b);
+        if (!any) words([&](float f, int i, int r) { return q4_nibble(f, inv[i][r]); }, b);
+        else words([&](float f, int i, int r) { return q4_nibble_any(f, scale[i][r]); }, b);
     }
 }
 
@@ -784,18 +806,20 @@ unsigned tiles_for(const Q4Params& p) {
     return static_cast<unsigned>(static_cast<long long>((q4_strips(p.N) + 7) / 8) * ((q4_kblocks(p.K) + 1) / 2) * p.E);
 }
 
+template <class T, bool TRANS>
+cudaError_t pack_group(const Q4Params& p, cudaStream_t stream) {
+    const unsigned grid = tiles_for(p);
+    if (p.group == 32) q4_pack_kernel<T, TRANS, 32><<<grid, 256, 0, stream>>>(p);
+    else if (p.group == 64) q4_pack_kernel<T, TRANS, 64><<<grid, 256, 0, stream>>>(p);
+    else q4_pack_kernel<T, TRANS, 128><<<grid, 256, 0, stream>>>(p);
+    return cudaGetLastError();
+}
+
 }  // namespace
 
 cudaError_t q4_pack_launch(const Q4Params& p, cudaStream_t stream) {
-    const unsigned grid = tiles_for(p);
-    if (p.bf16) {
-        if (p.trans_b) q4_pack_kernel<__nv_bfloat16, true><<<grid, 256, 0, stream>>>(p);
-        else q4_pack_kernel<__nv_bfloat16, false><<<grid, 256, 0, stream>>>(p);
-    } else {
-        if (p.trans_b) q4_pack_kernel<__half, true><<<grid, 256, 0, stream>>>(p);
-        else q4_pack_kernel<__half, false><<<grid, 256, 0, stream>>>(p);
-    }
-    return cudaGetLastError();
+    if (p.bf16) return p.trans_b ? pack_group<__nv_bfloat16, true>(p, stream) : pack_group<__nv_bfloat16, false>(p, stream);
+    return p.trans_b ? pack_group<__half, true>(p, stream) : pack_group<__half, false>(p, stream);
 }
 
 cudaError_t q4_unpack_launch(const Q4Params& p, cudaStream_t stream) {
