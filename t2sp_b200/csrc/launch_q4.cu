@@ -69,104 +69,99 @@ template <> __device__ __forceinline__ float2 pair_f32<__nv_bfloat16>(uint32_t w
 constexpr int kTile = 128;
 template <bool TRANS>
 struct Q4Tile {
-    // pitch in bytes, so that a strip's accesses (eight n, four k apart) meet different banks: [k][n], 2-byte accesses, four rows
-    // 32 bytes apart modulo 128; [n][k], 8-byte accesses, rows 32 bytes apart
-    static constexpr int kPitch = TRANS ? kTile * 2 + 32 : kTile * 2 + 8;
+    // pitch in bytes, so that a strip's accesses (eight n, four k apart) meet different banks.
+    // [pair of k][n]: a 32-bit word holds k and k + 1 of one n; two rows of pairs are 32 bytes apart modulo 128
+    // TRANS, [n][k]: accesses of four k, rows 32 bytes apart
+    static constexpr int kPitch = TRANS ? kTile * 2 + 32 : (kTile + 4) * 4;
+    static constexpr int kBytes = (TRANS ? kTile : kTile / 2) * kPitch;
 };
 
-// Rows of W between global memory and the tile. Outside the matrix the tile holds zeros.
+// Eight elements of a row, zeros from the row's end on.
+__device__ __forceinline__ uint4 row_piece(const uint16_t* src, int left, bool aligned) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (aligned && left >= 8) {
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(src));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < left) (&v.x)[j >> 1] |= static_cast<uint32_t>(src[j]) << (16 * (j & 1));
+    }
+    return v;
+}
+__device__ __forceinline__ void row_piece_out(uint16_t* dst, uint4 v, int left, bool aligned) {
+    if (aligned && left >= 8) {
+        *reinterpret_cast<uint4*>(dst) = v;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < left) dst[j] = static_cast<uint16_t>((&v.x)[j >> 1] >> (16 * (j & 1)));
+    }
+}
+
+// Rows of W between global memory and the tile. Outside the matrix the tile holds zeros. Each thread moves eight pieces of eight elements:
+// two at a time, of rows k and k + 1 (TRANS: n and n + 1).
 template <bool TRANS, bool STORE>
 __device__ __forceinline__ void tile_rows(const Q4Params& p, uint16_t* w, uint8_t* tile, int n0, int k0) {
     const int inner = TRANS ? p.K : p.N, outer = TRANS ? p.N : p.K, i0 = TRANS ? k0 : n0, o0 = TRANS ? n0 : k0;
     const bool aligned = (reinterpret_cast<uintptr_t>(w) & 15) == 0 && p.ldw % 8 == 0;
-    constexpr int kSteps = kTile * 16 / 256;
-    uint4 v[kSteps];
-    const int c0 = threadIdx.x, step = 16 * Q4Tile<TRANS>::kPitch;
-    uint8_t* mine = tile + (c0 >> 4) * Q4Tile<TRANS>::kPitch + (c0 & 15) * 16;
-    if (aligned && o0 + kTile <= outer && i0 + kTile <= inner) {   // a whole tile
-        uint16_t* at = w + (o0 + (c0 >> 4)) * p.ldw + i0 + (c0 & 15) * 8;
-        const long long rows = 16 * p.ldw;
-        if constexpr (!STORE) {
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s)
-                asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(v[s].x), "=r"(v[s].y), "=r"(v[s].z), "=r"(v[s].w) : "l"(at + s * rows));
-        }
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            uint2* m = reinterpret_cast<uint2*>(mine + s * step);
-            if constexpr (!STORE) {
-                m[0] = make_uint2(v[s].x, v[s].y);
-                m[1] = make_uint2(v[s].z, v[s].w);
-            } else {
-                const uint2 lo = m[0], hi = m[1];
-                *reinterpret_cast<uint4*>(at + s * rows) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-            }
-        }
-        return;
-    }
+    constexpr int kSteps = kTile / 2 * 16 / 256;
+    const int pair = threadIdx.x >> 4, c = threadIdx.x & 15;      // pair of rows, piece of the row
+    const int left = inner - i0 - c * 8;
+    uint16_t* at = w + (o0 + 2 * pair) * p.ldw + i0 + c * 8;
+    const long long next = 32 * p.ldw;
+    uint4 v[kSteps][2];
     if constexpr (!STORE) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const int c = s * 256 + threadIdx.x, o = o0 + (c >> 4), i = i0 + (c & 15) * 8;
-            const uint16_t* src = w + o * p.ldw + i;
-            v[s] = make_uint4(0, 0, 0, 0);
-            if (o >= outer) continue;
-            if (aligned && i + 8 <= inner) {
-                asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(v[s].x), "=r"(v[s].y), "=r"(v[s].z), "=r"(v[s].w) : "l"(src));
-            } else {
+        for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (i + j < inner) (&v[s].x)[j >> 1] |= static_cast<uint32_t>(src[j]) << (16 * (j & 1));
-            }
-        }
+            for (int h = 0; h < 2; ++h)
+                v[s][h] = row_piece(at + s * next + h * p.ldw, o0 + 2 * pair + 32 * s + h < outer ? left : 0, aligned);
     }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-        const int c = s * 256 + threadIdx.x, o = o0 + (c >> 4), i = i0 + (c & 15) * 8;
-        uint2* at = reinterpret_cast<uint2*>(tile + (c >> 4) * Q4Tile<TRANS>::kPitch + (c & 15) * 16);   // 8-byte aligned rows
-        if constexpr (!STORE) {
-            at[0] = make_uint2(v[s].x, v[s].y);
-            at[1] = make_uint2(v[s].z, v[s].w);
-        } else {
-            if (o >= outer || i >= inner) continue;
-            const uint2 lo = at[0], hi = at[1];
-            uint16_t* dst = w + o * p.ldw + i;
-            if (aligned && i + 8 <= inner) {
-                *reinterpret_cast<uint4*>(dst) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-            } else {
-                const uint32_t words[4] = {lo.x, lo.y, hi.x, hi.y};
+        if constexpr (TRANS) {
+            uint8_t* m = tile + (2 * pair + 32 * s) * Q4Tile<TRANS>::kPitch + c * 16;
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (i + j < inner) dst[j] = static_cast<uint16_t>(words[j >> 1] >> (16 * (j & 1)));
+            for (int h = 0; h < 2; ++h) {
+                uint4* x = reinterpret_cast<uint4*>(m + h * Q4Tile<TRANS>::kPitch);
+                if constexpr (!STORE) *x = v[s][h];
+                else v[s][h] = *x;
             }
+        } else {
+            uint4* x = reinterpret_cast<uint4*>(tile + (pair + 16 * s) * Q4Tile<TRANS>::kPitch + c * 32);
+            if constexpr (!STORE) {
+                const uint4 a = v[s][0], b = v[s][1];
+                x[0] = make_uint4(__byte_perm(a.x, b.x, 0x5410), __byte_perm(a.x, b.x, 0x7632), __byte_perm(a.y, b.y, 0x5410), __byte_perm(a.y, b.y, 0x7632));
+                x[1] = make_uint4(__byte_perm(a.z, b.z, 0x5410), __byte_perm(a.z, b.z, 0x7632), __byte_perm(a.w, b.w, 0x5410), __byte_perm(a.w, b.w, 0x7632));
+            } else {
+                const uint4 a = x[0], b = x[1];
+                v[s][0] = make_uint4(__byte_perm(a.x, a.y, 0x5410), __byte_perm(a.z, a.w, 0x5410), __byte_perm(b.x, b.y, 0x5410), __byte_perm(b.z, b.w, 0x5410));
+                v[s][1] = make_uint4(__byte_perm(a.x, a.y, 0x7632), __byte_perm(a.z, a.w, 0x7632), __byte_perm(b.x, b.y, 0x7632), __byte_perm(b.z, b.w, 0x7632));
+            }
+        }
+        if constexpr (STORE) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                row_piece_out(at + s * next + h * p.ldw, v[s][h], o0 + 2 * pair + 32 * s + h < outer ? left : 0, aligned);
         }
     }
 }
 
-// Four consecutive k (16 w + 4 t .. + 3 of block b) of row n of the tile, as two packed pairs.
+// Four consecutive k of row n of the tile, as two packed pairs.
 template <bool TRANS>
 __device__ __forceinline__ uint2 tile_get(const uint8_t* tile, int n, int k) {
-    if constexpr (TRANS) {
-        return *reinterpret_cast<const uint2*>(tile + n * Q4Tile<TRANS>::kPitch + k * 2);
-    } else {
-        const uint16_t* c = reinterpret_cast<const uint16_t*>(tile + k * Q4Tile<TRANS>::kPitch) + n;
-        constexpr int kRow = Q4Tile<TRANS>::kPitch / 2;
-        return make_uint2(c[0] | (static_cast<uint32_t>(c[kRow]) << 16), c[2 * kRow] | (static_cast<uint32_t>(c[3 * kRow]) << 16));
-    }
+    if constexpr (TRANS) return *reinterpret_cast<const uint2*>(tile + n * Q4Tile<TRANS>::kPitch + k * 2);
+    const uint8_t* c = tile + (k >> 1) * Q4Tile<TRANS>::kPitch + n * 4;
+    return make_uint2(*reinterpret_cast<const uint32_t*>(c), *reinterpret_cast<const uint32_t*>(c + Q4Tile<TRANS>::kPitch));
 }
 template <bool TRANS>
 __device__ __forceinline__ void tile_put(uint8_t* tile, int n, int k, uint2 v) {
     if constexpr (TRANS) {
         *reinterpret_cast<uint2*>(tile + n * Q4Tile<TRANS>::kPitch + k * 2) = v;
     } else {
-        uint16_t* c = reinterpret_cast<uint16_t*>(tile + k * Q4Tile<TRANS>::kPitch) + n;
-        constexpr int kRow = Q4Tile<TRANS>::kPitch / 2;
-        c[0] = static_cast<uint16_t>(v.x);
-        c[kRow] = static_cast<uint16_t>(v.x >> 16);
-        c[2 * kRow] = static_cast<uint16_t>(v.y);
-        c[3 * kRow] = static_cast<uint16_t>(v.y >> 16);
+        uint8_t* c = tile + (k >> 1) * Q4Tile<TRANS>::kPitch + n * 4;
+        *reinterpret_cast<uint32_t*>(c) = v.x;
+        *reinterpret_cast<uint32_t*>(c + Q4Tile<TRANS>::kPitch) = v.y;
     }
 }
 
@@ -199,7 +194,7 @@ __device__ __noinline__ uint32_t q4_nibble_any(float v, float scale) {
 
 template <class T, bool TRANS, int G>
 __global__ void __launch_bounds__(256) q4_pack_kernel(const Q4Params p) {
-    __shared__ __align__(16) uint8_t tile[kTile * Q4Tile<TRANS>::kPitch];
+    __shared__ __align__(16) uint8_t tile[Q4Tile<TRANS>::kBytes];
     const int kblocks = q4_kblocks(p.K), strips = q4_strips(p.N), groups = q4_groups(p.K, G);
     const int ntiles = (strips + 7) / 8, ktiles = (kblocks + 1) / 2;
     // tiles along W's rows run fastest
@@ -280,7 +275,7 @@ __global__ void __launch_bounds__(256) q4_pack_kernel(const Q4Params p) {
 template <class T, bool TRANS>
 __global__ void __launch_bounds__(256) q4_unpack_kernel(const Q4Params p) {
     using P = typename Pair16<T>::type;
-    __shared__ __align__(16) uint8_t tile[kTile * Q4Tile<TRANS>::kPitch];
+    __shared__ __align__(16) uint8_t tile[Q4Tile<TRANS>::kBytes];
     const int kblocks = q4_kblocks(p.K), strips = q4_strips(p.N), groups = q4_groups(p.K, p.group);
     const int ntiles = (strips + 7) / 8, ktiles = (kblocks + 1) / 2;
     const int x = blockIdx.x % (TRANS ? ktiles : ntiles), y = blockIdx.x / (TRANS ? ktiles : ntiles);
