@@ -22,6 +22,7 @@ struct GroupedParams {
     long long ldc, bs_c;   // row pitch of C or G, stride between the matrices of G
     int rows, E, K, N;
     int bf16;              // element type of the inputs: 1 bf16, 0 f16
+    int wide_out;          // 16-bit results: rows of C and G start on 16 bytes and N is a multiple of 8
     long long wait_cycles; // limit of every mbarrier wait in SM cycles, 0: kWaitTimeoutCycles
     unsigned* status;
 };

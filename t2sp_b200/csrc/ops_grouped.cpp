@@ -62,6 +62,7 @@ int run_grouped(const char* who, int mode, uint32_t type, uint32_t out, GroupedP
     p.status = rt_status_word();
     p.wait_cycles = rt_env().wait_cycles;
     p.bf16 = type == kBF16;
+    p.wide_out = out != kF32 && !(reinterpret_cast<uintptr_t>(p.c) & 15) && p.ldc % 8 == 0 && p.bs_c % 8 == 0 && p.N % 8 == 0;
     if (sync_after) cudaEventRecord(rt_event(0), s);
     GroupedMaps maps;
     memset(&maps, 0, sizeof(maps));

@@ -35,7 +35,8 @@ struct GroupedCfg {
     static constexpr int kTmemCols = 512;                     // two 256-column accumulators
     static constexpr int kNumBars = 4 * kStages + 4;
     static constexpr int kTableBytes = 2 * (kMaxGroups + 4) * 4;  // offsets, first tile of each group
-    static constexpr int kSmemBytes = kStages * kStageBytes + kTableBytes + kNumBars * 8 + 16 + 1024;
+    static constexpr int kOutBytes = 4 * 2 * 2048;            // two 32 x 32 tiles of 16-bit results for each epilogue warp
+    static constexpr int kSmemBytes = kStages * kStageBytes + kOutBytes + kTableBytes + kNumBars * 8 + 16 + 1024;
     static_assert(kSmemBytes <= 232448, "shared memory budget exceeded");
 };
 
@@ -114,8 +115,53 @@ __device__ __forceinline__ bool grouped_tables(const GroupedParams& p, int* off,
     return true;   // the caller synchronises the CTA before the tables are used
 }
 
+template <class O> __device__ __forceinline__ uint32_t pack16(uint32_t lo, uint32_t hi);
+template <> __device__ __forceinline__ uint32_t pack16<__half>(uint32_t lo, uint32_t hi) {
+    const __half2 v = __floats2half2_rn(__uint_as_float(lo), __uint_as_float(hi));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(uint32_t lo, uint32_t hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(lo), __uint_as_float(hi));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// 16-bit results of 32 n x 32 columns through a transposed tile in shared memory ([column][n], 64 bytes a column, 16-byte pieces at
+// piece ^ (column / 2 % 4)): four instructions write it, four write it out, 16 bytes a lane and eight columns at a time. `n_left`, `cols`: what
+// exists of the 32 n (from the warp's first one on) and of the columns. (One 2-byte store a column and lane: a gradient tile of
+// 256 x 256 with little to add up took 5 us to leave, a multiple of its products.)
+template <class O>
+__device__ __forceinline__ void grouped_put(uint32_t taddr, bool zero, uint8_t* tile, O* dst, long long ld, int n_left, int cols, int lane) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t r[16];
+        if (!zero) {
+            ptx::tmem_ld_16x256b_x4(taddr + (static_cast<uint32_t>(h * 16) << 16), r);
+            ptx::tmem_ld_wait();
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) r[j] = 0u;
+        }
+        const int piece = 2 * h + ((lane >> 3) & 1);
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const int col = 8 * (i + (lane >> 4)) + (lane & 7);
+            ptx::stmatrix_x4_trans(ptx::smem_u32(tile) + col * 64 + ((piece ^ ((col >> 1) & 3)) << 4), pack16<O>(r[4 * i], r[4 * i + 1]),
+                                   pack16<O>(r[4 * i + 2], r[4 * i + 3]), pack16<O>(r[4 * i + 4], r[4 * i + 5]),
+                                   pack16<O>(r[4 * i + 6], r[4 * i + 7]));
+        }
+    }
+    __syncwarp();
+    const int piece = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int col = 8 * i + (lane >> 2);
+        const uint4 v = *reinterpret_cast<const uint4*>(tile + col * 64 + ((piece ^ ((col >> 1) & 3)) << 4));
+        if (col < cols && piece * 8 < n_left) *reinterpret_cast<uint4*>(dst + col * ld + piece * 8) = v;
+    }
+}
+
 // Writes 32 columns of the accumulator: lane = n, one output row (or k) for each column. Each store instruction writes 32
-// consecutive n.
+// consecutive n. For fp32 results, and for places that take no 16-byte stores.
 template <class O>
 __device__ __forceinline__ void grouped_store(O* dst, long long ld, int cols, const uint32_t (&r)[32]) {
 #pragma unroll
@@ -135,7 +181,7 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
     constexpr int STAGES = Cfg::kStages;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::kStageBytes);  // leader's: both CTAs' data landed
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::kStageBytes + Cfg::kOutBytes);  // leader's: both CTAs' data landed
     uint64_t* empty_bar = full_bar + STAGES;       // per CTA: the MMAs that read the stage retired
     uint64_t* tail_bar = empty_bar + STAGES;       // gradient, per CTA: its own part of a ragged block landed
     uint64_t* fixed_bar = tail_bar + STAGES;       // gradient, leader's: both CTAs have cleared the ragged block's end
@@ -143,6 +189,7 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
     uint64_t* tempty_bar = tfull_bar + 2;          // leader's: accumulator drained by both CTAs (2)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
     uint32_t* abort_slot = tmem_slot + 1;
+    uint8_t* out_tiles = smem + STAGES * Cfg::kStageBytes;
     int* off = reinterpret_cast<int*>(tmem_slot + 4);
     int* first = off + kMaxGroups + 4;
 
@@ -309,7 +356,7 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
         GroupedTile g;
         for (int t = pair; grouped_tile<MODE>(p, off, first, t, e, g); t += num_pairs) {
             const int acc = lt & 1;
-            const int n = g.n0 + static_cast<int>(rank) * 128 + q * 32 + lane;
+            const int n = g.n0 + static_cast<int>(rank) * 128 + q * 32;
             O* dst = static_cast<O*>(p.c) + (MODE == GR_GRAD ? g.e * p.bs_c : 0) + g.c0 * p.ldc + n;
             if (g.num_kb) {
                 if (!bounded_wait_warp(&tfull_bar[acc], (lt >> 1) & 1, ab, ST_TIMEOUT_EPILOGUE, lane)) break;
@@ -317,15 +364,22 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
             }
 #pragma unroll 1
             for (int c = 0; c < g.cols; c += 32) {
+                const uint32_t taddr = lane_base + acc * 256 + c;
+                if constexpr (sizeof(O) == 2) {
+                    if (p.wide_out) {
+                        grouped_put(taddr, g.num_kb == 0, out_tiles + (q * 2 + ((c >> 5) & 1)) * 2048, dst + c * p.ldc, p.ldc, p.N - n, g.cols - c, lane);
+                        continue;
+                    }
+                }
                 uint32_t r[32];
                 if (g.num_kb) {
-                    ptx::tmem_ld_32x32(lane_base + acc * 256 + c, r);
+                    ptx::tmem_ld_32x32(taddr, r);
                     ptx::tmem_ld_wait();
                 } else {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) r[j] = 0u;
                 }
-                if (n < p.N) grouped_store(dst + c * p.ldc, p.ldc, g.cols - c, r);
+                if (n + lane < p.N) grouped_store(dst + c * p.ldc + lane, p.ldc, g.cols - c, r);
             }
             if (g.num_kb) {
                 ptx::tc_fence_before_sync();
