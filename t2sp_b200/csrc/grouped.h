@@ -11,6 +11,7 @@ namespace t2sp {
 constexpr int kMaxGroups = 1024;  // the kernels keep the groups' tables in shared memory
 
 enum : int { GR_FWD_MN = 0, GR_FWD_K = 1, GR_GRAD = 2 };  // B with n innermost, B with k innermost, gradient of B
+enum : int { GR_TILE_128 = 0, GR_TILE_256 = 1, GR_TILE_512 = 2 };      // 128 x 128 by one CTA, 256 x 256 and 512 x 256 by a pair
 enum : int { GR_OUT_F32 = 0, GR_OUT_BF16 = 1, GR_OUT_F16 = 2 };
 
 // Forward: C[t][n] = sum_k A[t][k] * B[e][k][n] for offsets[e] <= t < offsets[e+1]; rows outside every group are not
@@ -29,8 +30,7 @@ struct GroupedParams {
 
 struct GroupedMaps {
     CUtensorMap p;      // B (n, k, e), box 64 x 64, or (k, n, e), box 64 k x 128 n; gradient: D (n, t, 1), box 64 x 64
-    CUtensorMap q;      // A: forward (k, t), 64 k x 128 rows a box; gradient (k, t), 64 k x 64 rows
-    CUtensorMap q16;    // forward: 16 rows a box, for tiles narrower than 256 rows
+    CUtensorMap q[4];   // A: forward (k, t), 64 k x 128, 64, 32 and 16 rows a box; gradient (k, t), 64 k x 64 rows (the first map)
 };
 
 cudaError_t grouped_launch(int mode, int out, const GroupedParams& p, const GroupedMaps& maps, cudaStream_t stream);

@@ -7,21 +7,67 @@ namespace t2sp {
 
 namespace {
 
-template <int MODE, class O>
-cudaError_t launch_typed(const GroupedParams& p, const GroupedMaps& maps, int grid, cudaStream_t stream) {
-    using Cfg = GroupedCfg<MODE>;
-    auto kern = grouped_kernel<MODE, O>;
+template <int MODE, int VAR, class O>
+cudaError_t launch_typed(const GroupedParams& p, const GroupedMaps& maps, int workers, cudaStream_t stream) {
+    using Cfg = GroupedCfg<MODE, VAR>;
+    auto kern = grouped_kernel<MODE, VAR, O>;
     static std::atomic<bool> configured[kMaxDev];
     if (cudaError_t e = allow_smem(kern, Cfg::kSmemBytes, configured)) return e;
-    kern<<<grid, Cfg::kThreads, Cfg::kSmemBytes, stream>>>(p, maps);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(workers * Cfg::kPair);
+    cfg.blockDim = dim3(Cfg::kThreads);
+    cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+    cfg.stream = stream;
+    // programmatic stream serialization: the launch is set up while the kernel before it ends; grouped_kernel waits for
+    // that one before it touches memory
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = Cfg::kPair;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, p, maps);
 }
 
+template <int MODE, int VAR>
+cudaError_t launch_var(int out, const GroupedParams& p, const GroupedMaps& maps, long long tiles, cudaStream_t stream) {
+    const long long slots = core_sm_count() / GroupedCfg<MODE, VAR>::kPair;
+    const int workers = static_cast<int>(tiles < slots ? (tiles > 0 ? tiles : 1) : slots);
+    if (out == GR_OUT_F32) return launch_typed<MODE, VAR, float>(p, maps, workers, stream);
+    if (out == GR_OUT_BF16) return launch_typed<MODE, VAR, __nv_bfloat16>(p, maps, workers, stream);
+    return launch_typed<MODE, VAR, __half>(p, maps, workers, stream);
+}
+
+// Tiles of a call: how the rows fall into the groups is known on the device only. `most`: an upper bound (a tile of each group
+// more than the rows alone would need); else as if the rows were spread evenly.
+long long count_tiles(int mode, const GroupedParams& p, int tn, int tc, bool most) {
+    const long long nblk = (p.N + tn - 1) / tn;
+    if (mode == GR_GRAD) return nblk * ((p.K + tc - 1) / tc) * p.E;
+    const int groups = p.rows < p.E ? p.rows : p.E;
+    if (most) return nblk * (p.rows / tc + groups);
+    const int mean = (p.rows + groups - 1) / groups;
+    return nblk * groups * ((mean + tc - 1) / tc);
+}
+
+// Which tiles: those that need the least time for whole rounds over the SMs. A 512 x 256 tile brings 48 KB a k-block into each SM for twice the products
+// of a 256 x 256 one's 32 KB, which is what bounds long contractions (16384 rows in 8 groups, K = 4096, N = 8192: 766 us against
+// 860), but has no second accumulator to drain under the next tile's products (64 groups of 128 rows, K = 1024, N = 2048: 64 us
+// against 57; gradient with 512 rows a group, 2048 x 2048: 69 against 67). 128 x 128 tiles of single CTAs where the larger ones would leave half the SMs idle
+// (8 groups of 2 rows, 1024 x 1024: 8.8 us against 10.0); the gradient's outputs are too large for that to pay (12.0 against 13.9).
 template <int MODE>
-cudaError_t launch_mode(int out, const GroupedParams& p, const GroupedMaps& maps, int grid, cudaStream_t stream) {
-    if (out == GR_OUT_F32) return launch_typed<MODE, float>(p, maps, grid, stream);
-    if (out == GR_OUT_BF16) return launch_typed<MODE, __nv_bfloat16>(p, maps, grid, stream);
-    return launch_typed<MODE, __half>(p, maps, grid, stream);
+cudaError_t launch_mode(int out, const GroupedParams& p, const GroupedMaps& maps, cudaStream_t stream) {
+    const long long pairs = core_sm_count() / 2;
+    const long long rounds256 = (count_tiles(MODE, p, 256, 256, false) + pairs - 1) / pairs;
+    const long long rounds512 = (count_tiles(MODE, p, 512, 256, false) + pairs - 1) / pairs;
+    const int kb = MODE == GR_GRAD ? p.rows / (p.E * 64) : (p.K + 63) / 64;
+    if (kb >= (MODE == GR_GRAD ? 12 : 32) && 200 * rounds512 <= 108 * rounds256)
+        return launch_var<MODE, GR_TILE_512>(out, p, maps, count_tiles(MODE, p, 512, 256, true), stream);
+    if constexpr (MODE != GR_GRAD)
+        if (2 * count_tiles(MODE, p, 256, 256, false) <= pairs)
+            return launch_var<MODE, GR_TILE_128>(out, p, maps, count_tiles(MODE, p, 128, 128, true), stream);
+    return launch_var<MODE, GR_TILE_256>(out, p, maps, count_tiles(MODE, p, 256, 256, true), stream);
 }
 
 __global__ void repack16_kernel(const uint16_t* __restrict__ src, long long ld_src, long long bs_src, uint16_t* __restrict__ dst,
@@ -44,15 +90,9 @@ __global__ void repack16_kernel(const uint16_t* __restrict__ src, long long ld_s
 }  // namespace
 
 cudaError_t grouped_launch(int mode, int out, const GroupedParams& p, const GroupedMaps& maps, cudaStream_t stream) {
-    // at most this many tiles: a tile of each group more than the rows alone would need
-    const long long nblk = (p.N + 255) / 256;
-    const long long tiles = mode == GR_GRAD ? nblk * ((p.K + 255) / 256) * p.E
-                                            : nblk * (p.rows / 256 + (p.rows < p.E ? p.rows : p.E));
-    const long long pairs = core_sm_count() / 2;
-    const int grid = 2 * static_cast<int>(tiles < pairs ? (tiles > 0 ? tiles : 1) : pairs);
-    if (mode == GR_FWD_MN) return launch_mode<GR_FWD_MN>(out, p, maps, grid, stream);
-    if (mode == GR_FWD_K) return launch_mode<GR_FWD_K>(out, p, maps, grid, stream);
-    return launch_mode<GR_GRAD>(out, p, maps, grid, stream);
+    if (mode == GR_FWD_MN) return launch_mode<GR_FWD_MN>(out, p, maps, stream);
+    if (mode == GR_FWD_K) return launch_mode<GR_FWD_K>(out, p, maps, stream);
+    return launch_mode<GR_GRAD>(out, p, maps, stream);
 }
 
 cudaError_t repack16_launch(const void* src, long long ld_src, long long bs_src, void* dst, long long ld_dst, int inner, int rows,

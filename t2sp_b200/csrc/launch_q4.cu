@@ -347,7 +347,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-__device__ __forceinline__ void bar_group(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 // Two ways to multiply, by the number of rows that share a pass over the weights.
 //   INT  a few rows: the weights stay unsigned nibbles, whose offset 8 the sum of x over the group takes out, and x is written, group by group of k, as 24-bit integers times a power of two, in three signed bytes, and each byte is a column of
@@ -516,7 +515,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
         const int e = p.index ? idx[lead] : 0;
 
         // the rows of the unit, their x and its sums
-        bar_group(15, kGemvWarps * 32);   // the previous unit's x and rows have been read
+        ptx::bar_sync(15, kGemvWarps * 32);   // the previous unit's x and rows have been read
         if (warp == 0) {
             int found = 0;
             if (p.index) {
@@ -533,7 +532,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
             }
             if (lane == 0) *count_slot = found;
         }
-        bar_group(15, kGemvWarps * 32);
+        ptx::bar_sync(15, kGemvWarps * 32);
         const int count = *count_slot;
         const int pieces = kblocks * 8, padded = (pieces + 15) & ~15;   // of 8 k; a row's lanes start on a group of lanes
         constexpr int kLanes = G / 8;                                   // lanes that hold a group
@@ -621,7 +620,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
                     }
                 }
             }
-        bar_group(15, kGemvWarps * 32);
+        ptx::bar_sync(15, kGemvWarps * 32);
 
         // lanes of columns without a row read column 0 of x: what they compute is in columns that are not stored
         const uint8_t* xlane[NT];
@@ -718,7 +717,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     mine[(g + (j >> 1) * 8) * (kCols + 1) + n * 8 + 2 * t + (j & 1)] = acc[n][j];
-            bar_group(1 + group, gs * 32);
+            ptx::bar_sync(1 + group, gs * 32);
             // two buffers in turn: this one is written again only after the barrier of the next strip
             for (int i = wig * 32 + lane; i < 16 * count; i += gs * 32) {
                 const int n = i & 15, col = i >> 4;

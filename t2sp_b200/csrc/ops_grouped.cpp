@@ -70,8 +70,9 @@ int run_grouped(const char* who, int mode, uint32_t type, uint32_t out, GroupedP
         if (int e = fit_operand(vw, p_op)) return e;
         if (int e = fit_operand(vw, q_op)) return e;
         bool ok = encode(&maps.p, type, p_op, 3, 64, mode == GR_FWD_K ? 128 : 64) &&
-                  encode(&maps.q, type, q_op, 2, 64, mode == GR_GRAD ? 64 : 128);
-        if (ok && mode != GR_GRAD) ok = encode(&maps.q16, type, q_op, 2, 64, 16);
+                  encode(&maps.q[0], type, q_op, 2, 64, mode == GR_GRAD ? 64 : 128);
+        if (mode != GR_GRAD)
+            for (int b = 1; b < 4; ++b) ok = ok && encode(&maps.q[b], type, q_op, 2, 64, 128 >> b);
         if (!ok) return tma_unsupported(mode == GR_GRAD ? "A or D" : "A or B");
     }
     const cudaError_t e = grouped_launch(mode, out == kF32 ? GR_OUT_F32 : (out == kBF16 ? GR_OUT_BF16 : GR_OUT_F16), p, maps, s);

@@ -94,6 +94,9 @@ __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 
+// Named barrier of `threads` threads (whole warps).
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
 // Generic-proxy writes to shared memory (st.shared) become visible to the async
 // proxy (UMMA operand reads, TMA stores) only after this fence.
 __device__ __forceinline__ void fence_proxy_async_smem() {

@@ -1,15 +1,15 @@
-// Grouped products on CTA pairs. The operands are exchanged against the other GEMM kernels: the 256 rows of a pair's
+// Grouped products on the tensor cores. The operands are exchanged against the other GEMM kernels: the 256 rows of an
 // MMA are columns n of the output and the MMA's columns are rows t of the group (forward) or indices k (gradient of B), so
-// that a group's ragged end costs an MMA of fewer columns (any multiple of 32) instead of rows computed in vain, and a
+// that a group's ragged end costs an MMA of fewer columns (any multiple of 16, of a pair 32) instead of rows computed in vain, and a
 // weight tile that meets a handful of rows is still fetched at full width.
 //
-//   forward   D[n][t] = sum_k B[e][k][n] A[t][k]       tiles of 256 n x up to 256 rows of one group
-//   gradient  D[n][k] = sum_t D[t][n] A[t][k]          tiles of 256 n x up to 256 k of one group's matrix; the contraction
+//   forward   D[n][t] = sum_k B[e][k][n] A[t][k]       tiles of up to 512 n x up to 256 rows of one group
+//   gradient  D[n][k] = sum_t D[t][n] A[t][k]          tiles of up to 512 n x up to 256 k of one group's matrix; the contraction
 //                                                      runs over the group's rows, whose last block is ragged
 //
 // The group boundaries are read here, on the device: every CTA loads the offsets, checks them and builds the table of
-// first tiles in its prologue. Roles per CTA as in umma_pair.cuh (warp 0 producer, 1 MMA, 2-5 epilogue); the gradient has a
-// warp 6 that clears the rows behind the group's end in its last block, in both operands (they belong to other groups or to nobody and may
+// first tiles in its prologue. Roles per CTA as in umma_pair.cuh (warp 0 producer, 1 MMA, 2-9 epilogue); the gradient has one more
+// warp that clears the rows behind the group's end in its last block, in both operands (they belong to other groups or to nobody and may
 // hold anything), before the MMA reads it.
 #pragma once
 #include <cuda_bf16.h>
@@ -22,20 +22,30 @@
 
 namespace t2sp {
 
-template <int MODE>
+// Tile variants: 128 n x 128 columns by one CTA, 256 x 256 by a CTA pair, 512 x 256 by a pair whose CTAs hold two sub-tiles
+// of 128 n each (grouped_launch says when each is taken).
+template <int MODE, int VAR>
 struct GroupedCfg {
     static constexpr bool kGrad = MODE == GR_GRAD;
     static constexpr bool kPMn = MODE != GR_FWD_K;           // the MMA's A operand (n) is MN-major
-    static constexpr int kStages = 6;
-    static constexpr int kBlockK = 64;
-    static constexpr int kPBytes = 128 * 128;                 // 128 n x 64 k of one CTA
+    static constexpr int kPair = VAR == GR_TILE_128 ? 1 : 2; // CTAs of a tile
+    static constexpr int kSub = VAR == GR_TILE_512 ? 2 : 1;  // sub-tiles of a CTA
+    static constexpr int kTileN = 128 * kPair * kSub;
+    static constexpr int kTileC = 128 * kPair;
+    // columns come in steps that both CTAs' parts can take: 16 rows of a K-major operand, 64 (a swizzle atom) of an MN-major one
+    static constexpr int kColStep = (kGrad ? 64 : 16) * kPair;
+    static constexpr int kAccs = 2;                           // accumulators of kTileC columns: two tiles in turn, or the two sub-tiles
+    static constexpr int kStages = kSub == 2 ? 4 : 6;
+    static constexpr int kSubBytes = 128 * 128;               // 128 n x 64 k
+    static constexpr int kPBytes = kSub * kSubBytes;
     static constexpr int kQBytes = 128 * 128;                 // up to 128 columns x 64 k of one CTA
     static constexpr int kStageBytes = kPBytes + kQBytes;
-    static constexpr int kThreads = kGrad ? 7 * 32 : 6 * 32;
-    static constexpr int kTmemCols = 512;                     // two 256-column accumulators
+    static constexpr int kEpiWarps = 8;                       // two for each quarter of the tensor memory's lanes
+    static constexpr int kThreads = (2 + kEpiWarps + (kGrad ? 1 : 0)) * 32;
+    static constexpr int kTmemCols = kAccs * kTileC;
     static constexpr int kNumBars = 4 * kStages + 4;
+    static constexpr int kOutBytes = kEpiWarps * 2048;        // a 64 x 32 tile of 16-bit results for two epilogue warps
     static constexpr int kTableBytes = 2 * (kMaxGroups + 4) * 4;  // offsets, first tile of each group
-    static constexpr int kOutBytes = 4 * 2 * 2048;            // two 32 x 32 tiles of 16-bit results for each epilogue warp
     static constexpr int kSmemBytes = kStages * kStageBytes + kOutBytes + kTableBytes + kNumBars * 8 + 16 + 1024;
     static_assert(kSmemBytes <= 232448, "shared memory budget exceeded");
 };
@@ -43,24 +53,43 @@ struct GroupedCfg {
 // One tile of the output and its contraction.
 struct GroupedTile {
     int e, n0, c0;      // group, first n, first column (row t of the group in the forward, k in the gradient)
-    int cols;           // columns that exist (up to 256)
-    int ncols;          // columns the MMA computes: cols rounded up to 32 (gradient: 128, whole swizzle atoms in both CTAs)
+    int cols;           // columns that exist
+    int ncols;          // columns the MMA computes
     int num_kb;         // k-blocks, 0: the result is zero
     int row0, tail;     // gradient: first row of the group; rows in its last block (64: not ragged)
 };
 
-template <int MODE>
+// n / d and n % d for 0 <= n, 0 < d, n / d < 2^21, through a reciprocal (the compiler's division takes several times as long, and every role
+// goes through a handful for each tile): the product is off the quotient by less than one.
+__device__ __forceinline__ int quick_div(int n, int d, int& rest) {
+    int q = static_cast<int>(__fdividef(static_cast<float>(n), static_cast<float>(d)));
+    rest = n - q * d;
+    if (rest < 0) { --q; rest += d; }
+    else if (rest >= d) { ++q; rest -= d; }
+    return q;
+}
+// tile_coords of umma_core.cuh: groups of G row-blocks sweep all column-blocks, rows fastest inside a group.
+__device__ __forceinline__ void quick_coords(int t, int tiles_m, int tiles_n, int G, int& mb, int& nb) {
+    int r;
+    const int g = quick_div(t, G * tiles_n, r);
+    nb = quick_div(r, min(G, tiles_m - g * G), mb);
+    mb += g * G;
+}
+
+template <int MODE, int VAR>
 __device__ __forceinline__ bool grouped_tile(const GroupedParams& p, const int* off, const int* first, int t, int& e, GroupedTile& g) {
-    const int nblk = (p.N + 255) >> 8;
+    using Cfg = GroupedCfg<MODE, VAR>;
+    constexpr int kRaster = 2048 / Cfg::kTileN;   // n-blocks that are swept together: 2048 n
+    const int nblk = (p.N + Cfg::kTileN - 1) / Cfg::kTileN;
     if constexpr (MODE == GR_GRAD) {
-        const int kblk = (p.K + 255) >> 8, per = nblk * kblk;
+        const int kblk = (p.K + Cfg::kTileC - 1) / Cfg::kTileC, per = nblk * kblk;
         if (t >= per * p.E) return false;
-        g.e = t / per;
-        int mb, kb;
-        tile_coords(t - g.e * per, nblk, kblk, 8, mb, kb);
-        g.n0 = mb * 256;
-        g.c0 = kb * 256;
-        g.cols = min(256, p.K - g.c0);
+        int mb, kb, rest;
+        g.e = quick_div(t, per, rest);
+        quick_coords(rest, nblk, kblk, kRaster, mb, kb);
+        g.n0 = mb * Cfg::kTileN;
+        g.c0 = kb * Cfg::kTileC;
+        g.cols = min(Cfg::kTileC, p.K - g.c0);
         g.row0 = off[g.e];
         const int rows = off[g.e + 1] - g.row0;
         g.num_kb = (rows + 63) >> 6;
@@ -70,25 +99,27 @@ __device__ __forceinline__ bool grouped_tile(const GroupedParams& p, const int* 
         while (t >= first[e + 1]) ++e;   // tiles are visited in increasing order
         g.e = e;
         const int lo = off[e], rows = off[e + 1] - lo;
-        const int tiles = (rows + 255) >> 8;
+        const int tiles = (rows + Cfg::kTileC - 1) / Cfg::kTileC;
         int mb, tb;
-        tile_coords(t - first[e], nblk, tiles, 8, mb, tb);
-        const int per = ((rows + tiles - 1) / tiles + 31) & ~31;   // near-equal tiles
-        g.n0 = mb * 256;
+        quick_coords(t - first[e], nblk, tiles, kRaster, mb, tb);
+        int rest;
+        const int per = quick_div(rows + tiles * Cfg::kColStep - 1, tiles * Cfg::kColStep, rest) * Cfg::kColStep;   // near-equal tiles
+        g.n0 = mb * Cfg::kTileN;
         g.c0 = lo + tb * per;
-        g.cols = min(per, lo + rows - g.c0);
+        g.cols = max(0, min(per, lo + rows - g.c0));
         g.num_kb = (p.K + 63) >> 6;
         g.row0 = 0;
         g.tail = 64;
     }
-    g.ncols = MODE == GR_GRAD ? (g.cols + 127) & ~127 : (g.cols + 31) & ~31;
+    g.ncols = max(Cfg::kColStep, (g.cols + Cfg::kColStep - 1) / Cfg::kColStep * Cfg::kColStep);
     return true;
 }
 
 // Offsets into shared memory, checked, and the number of the first tile of every group (forward). Returns false when the
 // offsets decrease or leave the rows; every thread of the CTA gets the verdict.
-template <int MODE>
+template <int MODE, int VAR>
 __device__ __forceinline__ bool grouped_tables(const GroupedParams& p, int* off, int* first) {
+    using Cfg = GroupedCfg<MODE, VAR>;
     int bad = 0;
     for (int e = threadIdx.x; e <= p.E; e += blockDim.x) off[e] = p.offsets[e];
     __syncthreads();
@@ -96,11 +127,11 @@ __device__ __forceinline__ bool grouped_tables(const GroupedParams& p, int* off,
     if (__syncthreads_or(bad)) return false;
     if (MODE != GR_GRAD) {
         if (threadIdx.x < 32) {
-            const int lane = threadIdx.x, nblk = (p.N + 255) >> 8;
+            const int lane = threadIdx.x, nblk = (p.N + Cfg::kTileN - 1) / Cfg::kTileN;
             int base = 0;
             for (int e0 = 0; e0 < p.E; e0 += 32) {
                 const int e = e0 + lane;
-                int v = e < p.E ? ((off[e + 1] - off[e] + 255) >> 8) * nblk : 0;
+                int v = e < p.E ? (off[e + 1] - off[e] + Cfg::kTileC - 1) / Cfg::kTileC * nblk : 0;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
                     const int u = __shfl_up_sync(0xffffffffu, v, d);
@@ -125,37 +156,41 @@ template <> __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(uint32_t l
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// 16-bit results of 32 n x 32 columns through a transposed tile in shared memory ([column][n], 64 bytes a column, 16-byte pieces at
-// piece ^ (column / 2 % 4)): four instructions write it, four write it out, 16 bytes a lane and eight columns at a time. `n_left`, `cols`: what
-// exists of the 32 n (from the warp's first one on) and of the columns. (One 2-byte store a column and lane: a gradient tile of
-// 256 x 256 with little to add up took 5 us to leave, a multiple of its products.)
+// 16-bit results of 64 n x 32 columns, by two warps with 32 n each, through a transposed tile in shared memory ([column][n], 128 bytes a column,
+// 16-byte pieces at piece ^ (column % 8)): each warp writes its half of every column with four instructions, then takes 16 columns out,
+// whole 128-byte lines and 16 bytes a lane. (One 2-byte store a column and lane: a gradient tile of 256 x 256 with little to add up
+// took 5 us to leave, a multiple of its products; 64-byte pieces of one warp: 15 bytes a cycle of the 32 that an SM can write.)
+// `half`: which warp of the two; `n_left`, `cols`: what exists of the 64 n and of the columns.
 template <class O>
-__device__ __forceinline__ void grouped_put(uint32_t taddr, bool zero, uint8_t* tile, O* dst, long long ld, int n_left, int cols, int lane) {
+__device__ __forceinline__ void grouped_put(uint32_t taddr, bool zero, uint8_t* tile, O* dst, long long ld, int n_left, int cols, int lane,
+                                            int half, int barrier) {
+    uint32_t r[2][16];
+    if (!zero) {
+        ptx::tmem_ld_16x256b_x4(taddr, r[0]);
+        ptx::tmem_ld_16x256b_x4(taddr + (16u << 16), r[1]);
+        ptx::tmem_ld_wait();
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[0][j] = r[1][j] = 0u;
+    }
+    ptx::bar_sync(barrier, 64);   // the tile's previous content has been read
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        uint32_t r[16];
-        if (!zero) {
-            ptx::tmem_ld_16x256b_x4(taddr + (static_cast<uint32_t>(h * 16) << 16), r);
-            ptx::tmem_ld_wait();
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) r[j] = 0u;
-        }
-        const int piece = 2 * h + ((lane >> 3) & 1);
+        const int piece = half * 4 + 2 * h + ((lane >> 3) & 1);
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
             const int col = 8 * (i + (lane >> 4)) + (lane & 7);
-            ptx::stmatrix_x4_trans(ptx::smem_u32(tile) + col * 64 + ((piece ^ ((col >> 1) & 3)) << 4), pack16<O>(r[4 * i], r[4 * i + 1]),
-                                   pack16<O>(r[4 * i + 2], r[4 * i + 3]), pack16<O>(r[4 * i + 4], r[4 * i + 5]),
-                                   pack16<O>(r[4 * i + 6], r[4 * i + 7]));
+            ptx::stmatrix_x4_trans(ptx::smem_u32(tile) + col * 128 + ((piece ^ (lane & 7)) << 4), pack16<O>(r[h][4 * i], r[h][4 * i + 1]),
+                                   pack16<O>(r[h][4 * i + 2], r[h][4 * i + 3]), pack16<O>(r[h][4 * i + 4], r[h][4 * i + 5]),
+                                   pack16<O>(r[h][4 * i + 6], r[h][4 * i + 7]));
         }
     }
-    __syncwarp();
-    const int piece = lane & 3;
+    ptx::bar_sync(barrier, 64);
+    const int piece = lane & 7;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int col = 8 * i + (lane >> 2);
-        const uint4 v = *reinterpret_cast<const uint4*>(tile + col * 64 + ((piece ^ ((col >> 1) & 3)) << 4));
+        const int col = 16 * half + 4 * i + (lane >> 3);
+        const uint4 v = *reinterpret_cast<const uint4*>(tile + col * 128 + ((piece ^ (col & 7)) << 4));
         if (col < cols && piece * 8 < n_left) *reinterpret_cast<uint4*>(dst + col * ld + piece * 8) = v;
     }
 }
@@ -174,114 +209,144 @@ __device__ __forceinline__ void grouped_store(O* dst, long long ld, int cols, co
         }
 }
 
-template <int MODE, class O>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedCfg<MODE>::kThreads, 1)
+template <int MODE, int VAR, class O>
+__global__ void __launch_bounds__(GroupedCfg<MODE, VAR>::kThreads, 1)
 grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ GroupedMaps maps) {
-    using Cfg = GroupedCfg<MODE>;
-    constexpr int STAGES = Cfg::kStages;
+    using Cfg = GroupedCfg<MODE, VAR>;
+    constexpr int STAGES = Cfg::kStages, kPair = Cfg::kPair, kSub = Cfg::kSub;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::kStageBytes + Cfg::kOutBytes);  // leader's: both CTAs' data landed
+    uint8_t* out_tiles = smem + STAGES * Cfg::kStageBytes;
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(out_tiles + Cfg::kOutBytes);  // leader's: all CTAs' data landed
     uint64_t* empty_bar = full_bar + STAGES;       // per CTA: the MMAs that read the stage retired
     uint64_t* tail_bar = empty_bar + STAGES;       // gradient, per CTA: its own part of a ragged block landed
-    uint64_t* fixed_bar = tail_bar + STAGES;       // gradient, leader's: both CTAs have cleared the ragged block's end
+    uint64_t* fixed_bar = tail_bar + STAGES;       // gradient, leader's: all CTAs have cleared the ragged block's end
     uint64_t* tfull_bar = fixed_bar + STAGES;      // per CTA: accumulator complete (2)
-    uint64_t* tempty_bar = tfull_bar + 2;          // leader's: accumulator drained by both CTAs (2)
+    uint64_t* tempty_bar = tfull_bar + 2;          // leader's: accumulator drained by all CTAs (2)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
     uint32_t* abort_slot = tmem_slot + 1;
-    uint8_t* out_tiles = smem + STAGES * Cfg::kStageBytes;
     int* off = reinterpret_cast<int*>(tmem_slot + 4);
     int* first = off + kMaxGroups + 4;
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const uint32_t rank = ptx::cluster_ctarank();
+    const int rank = kPair == 2 ? static_cast<int>(ptx::cluster_ctarank()) : 0;
     const AbortCtx ab{abort_slot, p.status, p.wait_cycles > 0 ? p.wait_cycles : kWaitTimeoutCycles};
-    const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+    const int worker = blockIdx.x / kPair, num_workers = gridDim.x / kPair;
 
-    // every CTA sees the same offsets, so all of them leave here or none does
-    if (!grouped_tables<MODE>(p, off, first)) {
-        if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(p.status, ST_BAD_OFFSETS);
-        return;
-    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             ptx::mbar_init(&full_bar[s], 1);
             ptx::mbar_init(&empty_bar[s], 1);
             ptx::mbar_init(&tail_bar[s], 1);
-            ptx::mbar_init(&fixed_bar[s], 2);
+            ptx::mbar_init(&fixed_bar[s], kPair);
         }
         for (int a = 0; a < 2; ++a) {
             ptx::mbar_init(&tfull_bar[a], 1);
-            ptx::mbar_init(&tempty_bar[a], 8);  // 4 epilogue warps in each CTA
+            ptx::mbar_init(&tempty_bar[a], Cfg::kEpiWarps * kPair);
         }
         *abort_slot = 0u;
         ptx::fence_mbar_init();
     }
     if (warp == 1) {
-        ptx::tmem_alloc<2>(tmem_slot, Cfg::kTmemCols);
-        ptx::tmem_relinquish<2>();
+        ptx::tmem_alloc<kPair>(tmem_slot, Cfg::kTmemCols);
+        ptx::tmem_relinquish<kPair>();
     }
+    ptx::grid_dep_launch();
+    ptx::grid_dep_wait();
+    const bool valid = grouped_tables<MODE, VAR>(p, off, first);
     ptx::tc_fence_before_sync();
     __syncthreads();
-    ptx::cluster_sync();
+    if constexpr (kPair == 2) ptx::cluster_sync();
     ptx::tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
+    if (!valid) {   // every CTA sees the same offsets, so all of them leave here or none does
+        if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(p.status, ST_BAD_OFFSETS);
+        if (warp == 1) ptx::tmem_dealloc<kPair>(tmem_base, Cfg::kTmemCols);
+        return;
+    }
+
+    // the forms for one CTA and for a pair
+    auto load2 = [&](void* dst, const void* map, uint64_t* bar, int owner, int c0, int c1) {
+        if constexpr (kPair == 2) ptx::tma_load_2d_pair(dst, map, ptx::map_to_cta(bar, owner), c0, c1);
+        else ptx::tma_load_2d(dst, map, bar, c0, c1);
+    };
+    auto load3 = [&](void* dst, const void* map, uint64_t* bar, int owner, int c0, int c1, int c2) {
+        if constexpr (kPair == 2) ptx::tma_load_3d_pair(dst, map, ptx::map_to_cta(bar, owner), c0, c1, c2);
+        else ptx::tma_load_3d(dst, map, bar, c0, c1, c2);
+    };
+    auto commit_all = [&](uint64_t* bar) {   // to this barrier of every CTA
+        if constexpr (kPair == 2) {
+            ptx::umma_commit_pair(ptx::map_to_cta(bar, 0));
+            ptx::umma_commit_pair(ptx::map_to_cta(bar, 1));
+        } else {
+            ptx::umma_commit(bar);
+        }
+    };
 
     if (warp == 0) {
-        // ------------------------------------------------------------ TMA producer (both CTAs)
+        // ------------------------------------------------------------ TMA producer (every CTA)
         if (lane == 0) {
             if (p.K > 0 && p.rows > 0) {   // else the maps describe nothing and no tile has a k-block
                 ptx::prefetch_tensormap(&maps.p);
-                ptx::prefetch_tensormap(&maps.q);
+                ptx::prefetch_tensormap(&maps.q[0]);
             }
             int it = 0, e = 0;
             bool ok = true;
             GroupedTile g;
-            for (int t = pair; ok && grouped_tile<MODE>(p, off, first, t, e, g); t += num_pairs) {
-                const int half = g.ncols >> 1;
-                const int n0 = g.n0 + static_cast<int>(rank) * 128;
-                const int c0 = g.c0 + static_cast<int>(rank) * half;
+            for (int t = worker; ok && grouped_tile<MODE, VAR>(p, off, first, t, e, g); t += num_workers) {
+                const int part = g.ncols / kPair;   // columns of this CTA
+                const int n0 = g.n0 + rank * 128;
+                const int c0 = g.c0 + rank * part;
                 for (int kb = 0; kb < g.num_kb; ++kb, ++it) {
                     const int s = it % STAGES;
                     const uint32_t ph = (it / STAGES) & 1;
                     if (!bounded_wait(&empty_bar[s], ph ^ 1, ab, ST_TIMEOUT_PRODUCER)) { ok = false; break; }
                     uint8_t* sp = smem + s * Cfg::kStageBytes;
                     uint8_t* sq = sp + Cfg::kPBytes;
-                    uint32_t bar;
+                    uint64_t* bar = &full_bar[s];
+                    int owner = 0;
                     if constexpr (MODE == GR_GRAD) {
-                        const int qboxes = half > 64 ? 2 : 1;
+                        const int qboxes = part > 64 ? 2 : 1;
                         const int bytes = Cfg::kPBytes + qboxes * 8192;
                         if (g.tail < 64 && kb == g.num_kb - 1) {
                             // ragged block: each CTA's part is credited to its own barrier, for its clearing warp; the
                             // stage's barrier only keeps its phase
                             ptx::mbar_expect_tx(&tail_bar[s], bytes);
                             if (rank == 0) ptx::mbar_arrive(&full_bar[s]);
-                            bar = ptx::map_to_cta(&tail_bar[s], rank);
-                        } else {
-                            if (rank == 0) ptx::mbar_expect_tx(&full_bar[s], 2 * bytes);
-                            bar = ptx::map_to_cta(&full_bar[s], 0);
+                            bar = &tail_bar[s];
+                            owner = rank;
+                        } else if (rank == 0) {
+                            ptx::mbar_expect_tx(&full_bar[s], kPair * bytes);
                         }
                         const int row = g.row0 + kb * 64;
-                        ptx::tma_load_3d_pair(sp, &maps.p, bar, n0, row, 0);
-                        ptx::tma_load_3d_pair(sp + 8192, &maps.p, bar, n0 + 64, row, 0);
-                        ptx::tma_load_2d_pair(sq, &maps.q, bar, c0, row);
-                        if (qboxes == 2) ptx::tma_load_2d_pair(sq + 8192, &maps.q, bar, c0 + 64, row);
+#pragma unroll
+                        for (int u = 0; u < kSub; ++u) {
+                            load3(sp + u * Cfg::kSubBytes, &maps.p, bar, owner, n0 + u * 256, row, 0);
+                            load3(sp + u * Cfg::kSubBytes + 8192, &maps.p, bar, owner, n0 + u * 256 + 64, row, 0);
+                        }
+                        load2(sq, &maps.q[0], bar, owner, c0, row);
+                        if (qboxes == 2) load2(sq + 8192, &maps.q[0], bar, owner, c0 + 64, row);
                     } else {
-                        if (rank == 0) ptx::mbar_expect_tx(&full_bar[s], 2 * (Cfg::kPBytes + half * 128));
-                        bar = ptx::map_to_cta(&full_bar[s], 0);
-                        if constexpr (MODE == GR_FWD_MN) {
-                            ptx::tma_load_3d_pair(sp, &maps.p, bar, n0, kb * 64, g.e);
-                            ptx::tma_load_3d_pair(sp + 8192, &maps.p, bar, n0 + 64, kb * 64, g.e);
-                        } else {
-                            ptx::tma_load_3d_pair(sp, &maps.p, bar, kb * 64, n0, g.e);
+                        if (rank == 0) ptx::mbar_expect_tx(&full_bar[s], kPair * (Cfg::kPBytes + part * 128));
+#pragma unroll
+                        for (int u = 0; u < kSub; ++u) {
+                            if constexpr (MODE == GR_FWD_MN) {
+                                load3(sp + u * Cfg::kSubBytes, &maps.p, bar, owner, n0 + u * 256, kb * 64, g.e);
+                                load3(sp + u * Cfg::kSubBytes + 8192, &maps.p, bar, owner, n0 + u * 256 + 64, kb * 64, g.e);
+                            } else {
+                                load3(sp + u * Cfg::kSubBytes, &maps.p, bar, owner, kb * 64, n0 + u * 256, g.e);
+                            }
                         }
-                        if (half == 128) {
-                            ptx::tma_load_2d_pair(sq, &maps.q, bar, kb * 64, c0);
-                        } else {
-                            for (int j = 0; j < half; j += 16)
-                                ptx::tma_load_2d_pair(sq + j * 128, &maps.q16, bar, kb * 64, c0 + j);
-                        }
+                        // boxes of 128, 64, 32 and 16 rows: at most three a block (eight boxes of 16 rows kept the thread busy for longer
+                        // than the block's MMAs)
+                        int j = 0;
+#pragma unroll
+                        for (int b = 0; b < 4; ++b)
+                            if (part & (128 >> b)) {
+                                load2(sq + j * 128, &maps.q[b], bar, owner, kb * 64, c0 + j);
+                                j += 128 >> b;
+                            }
                     }
                 }
             }
@@ -293,54 +358,99 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
             uint32_t fixed_ph = 0;
             bool ok = true;
             GroupedTile g;
+            uint32_t idesc = 0;
             constexpr uint32_t kStepMn = (16 * 128) >> 4, kStepK = 32 >> 4;
             constexpr uint32_t kStepP = Cfg::kPMn ? kStepMn : kStepK;
             constexpr uint32_t kStepQ = Cfg::kGrad ? kStepMn : kStepK;
-            for (int t = pair; ok && grouped_tile<MODE>(p, off, first, t, e, g); t += num_pairs) {
-                if (g.num_kb == 0) continue;   // nothing to add up: the epilogue writes zeros
-                const int acc = lt & 1;
-                if (!bounded_wait(&tempty_bar[acc], ((lt >> 1) & 1) ^ 1, ab, ST_TIMEOUT_MMA)) { ok = false; break; }
+            auto wait_block = [&](int i, int kb) -> bool {   // k-block kb of the tile, the i-th of this CTA
+                const int s = i % STAGES;
+                if (Cfg::kGrad && g.tail < 64 && kb == g.num_kb - 1) {
+                    if (!bounded_wait(&fixed_bar[s], (fixed_ph >> s) & 1, ab, ST_TIMEOUT_MMA)) return false;
+                    fixed_ph ^= 1u << s;
+                } else {
+                    if (!bounded_wait(&full_bar[s], (i / STAGES) & 1, ab, ST_TIMEOUT_MMA)) return false;
+                }
                 ptx::tc_fence_after_sync();
-                const uint32_t d_tmem = tmem_base + acc * 256;
-                const uint32_t idesc = make_instr_desc(1, p.bf16 ? 1 : 0, Cfg::kPMn, Cfg::kGrad, 256, g.ncols);
-                for (int kb = 0; kb < g.num_kb; ++kb, ++it) {
-                    const int s = it % STAGES;
-                    if (Cfg::kGrad && g.tail < 64 && kb == g.num_kb - 1) {
-                        if (!bounded_wait(&fixed_bar[s], (fixed_ph >> s) & 1, ab, ST_TIMEOUT_MMA)) { ok = false; break; }
-                        fixed_ph ^= 1u << s;
-                    } else {
-                        if (!bounded_wait(&full_bar[s], (it / STAGES) & 1, ab, ST_TIMEOUT_MMA)) { ok = false; break; }
-                    }
-                    ptx::tc_fence_after_sync();
-                    const uint32_t sp = ptx::smem_u32(smem + s * Cfg::kStageBytes);
-                    const uint64_t dp = ptx::make_smem_desc(sp, Cfg::kPMn ? 8192 : 16, 1024);
-                    const uint64_t dq = ptx::make_smem_desc(sp + Cfg::kPBytes, Cfg::kGrad ? 8192 : 16, 1024);
+                return true;
+            };
+            auto issue = [&](uint32_t d_tmem, int u, int kb, int i) {
+                const uint32_t sp = ptx::smem_u32(smem + (i % STAGES) * Cfg::kStageBytes);
+                const uint64_t dp = ptx::make_smem_desc(sp + u * Cfg::kSubBytes, Cfg::kPMn ? 8192 : 16, 1024);
+                const uint64_t dq = ptx::make_smem_desc(sp + Cfg::kPBytes, Cfg::kGrad ? 8192 : 16, 1024);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        ptx::umma<ptx::KIND_F16, 2>(d_tmem, dp + j * kStepP, dq + j * kStepQ, idesc, (kb | j) ? 1u : 0u);
-                    ptx::umma_commit_pair(ptx::map_to_cta(&empty_bar[s], 0));
-                    ptx::umma_commit_pair(ptx::map_to_cta(&empty_bar[s], 1));
+                for (int j = 0; j < 4; ++j)
+                    ptx::umma<ptx::KIND_F16, kPair>(d_tmem, dp + j * kStepP, dq + j * kStepQ, idesc, (kb | j) ? 1u : 0u);
+            };
+            for (int t = worker; ok && grouped_tile<MODE, VAR>(p, off, first, t, e, g); t += num_workers) {
+                if (g.num_kb == 0) continue;   // nothing to add up: the epilogue writes zeros
+                idesc = make_instr_desc(1, p.bf16 ? 1 : 0, Cfg::kPMn, Cfg::kGrad, 128 * kPair, g.ncols);
+                if constexpr (kSub == 1) {
+                    const int acc = lt & 1;
+                    ok = bounded_wait(&tempty_bar[acc], ((lt >> 1) & 1) ^ 1, ab, ST_TIMEOUT_MMA);
+                    ptx::tc_fence_after_sync();
+                    for (int kb = 0; kb < g.num_kb && ok; ++kb) {
+                        ok = wait_block(it + kb, kb);
+                        if (!ok) break;
+                        issue(tmem_base + acc * Cfg::kTileC, 0, kb, it + kb);
+                        commit_all(&empty_bar[(it + kb) % STAGES]);
+                    }
+                    if (ok) commit_all(&tfull_bar[acc]);
+                } else {
+                    // Both accumulators belong to this tile. Sub-tile 0 runs `lead` k-blocks ahead of sub-tile 1 at both ends of the tile, so that
+                    // its MMAs begin while accumulator 1 is still drained, and its own drain runs under sub-tile 1's last MMAs.
+                    const int n = g.num_kb, lead = min(STAGES - 1, n / 2);
+                    auto wait_drained = [&](int u) -> bool {
+                        if (!bounded_wait(&tempty_bar[u], (lt & 1) ^ 1, ab, ST_TIMEOUT_MMA)) return false;
+                        ptx::tc_fence_after_sync();
+                        return true;
+                    };
+                    auto both = [&](int u, int kb) { issue(tmem_base + u * Cfg::kTileC, u, kb, it + kb); };
+                    ok = wait_drained(0);
+                    for (int kb = 0; kb < lead && ok; ++kb) {
+                        ok = wait_block(it + kb, kb);
+                        if (ok) both(0, kb);
+                    }
+                    ok = ok && wait_drained(1);
+                    for (int kb = 0; kb < lead && ok; ++kb) {
+                        both(1, kb);
+                        commit_all(&empty_bar[(it + kb) % STAGES]);
+                    }
+                    for (int kb = lead; kb < n - lead && ok; ++kb) {
+                        ok = wait_block(it + kb, kb);
+                        if (!ok) break;
+                        both(0, kb);
+                        both(1, kb);
+                        commit_all(&empty_bar[(it + kb) % STAGES]);
+                    }
+                    for (int kb = n - lead; kb < n && ok; ++kb) {
+                        ok = wait_block(it + kb, kb);
+                        if (ok) both(0, kb);
+                    }
+                    if (!ok) break;
+                    commit_all(&tfull_bar[0]);
+                    for (int kb = n - lead; kb < n; ++kb) {
+                        both(1, kb);
+                        commit_all(&empty_bar[(it + kb) % STAGES]);
+                    }
+                    commit_all(&tfull_bar[1]);
                 }
-                if (ok) {
-                    ptx::umma_commit_pair(ptx::map_to_cta(&tfull_bar[acc], 0));
-                    ptx::umma_commit_pair(ptx::map_to_cta(&tfull_bar[acc], 1));
-                }
+                it += g.num_kb;
                 ++lt;
             }
         }
-    } else if (Cfg::kGrad && warp == 6) {
-        // ------------------------------------------------------------ clears the end of ragged blocks (both CTAs)
+    } else if (Cfg::kGrad && warp == 2 + Cfg::kEpiWarps) {
+        // ------------------------------------------------------------ clears the end of ragged blocks (every CTA)
         int it = 0, e = 0;
         uint32_t tail_ph = 0;
         GroupedTile g;
-        for (int t = pair; grouped_tile<MODE>(p, off, first, t, e, g); t += num_pairs) {
+        for (int t = worker; grouped_tile<MODE, VAR>(p, off, first, t, e, g); t += num_workers) {
             it += g.num_kb;
             if (g.num_kb == 0 || g.tail == 64) continue;
             const int s = (it - 1) % STAGES;
             if (!bounded_wait_warp(&tail_bar[s], (tail_ph >> s) & 1, ab, ST_TIMEOUT_SPLITTER, lane)) break;
             tail_ph ^= 1u << s;
             uint8_t* sp = smem + s * Cfg::kStageBytes;
-            const int boxes = (g.ncols >> 1) > 64 ? 4 : 3;
+            const int boxes = Cfg::kPBytes / 8192 + (g.ncols / kPair > 64 ? 2 : 1);
             for (int b = 0; b < boxes; ++b)
                 for (int i = g.tail * 128 + lane * 16; i < 8192; i += 512)
                     *reinterpret_cast<uint4*>(sp + b * 8192 + i) = make_uint4(0, 0, 0, 0);
@@ -349,44 +459,58 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
             if (lane == 0) ptx::mbar_arrive_cluster(&fixed_bar[s], 0);
         }
     } else {
-        // ------------------------------------------------------------ epilogue (both CTAs, own 128 n)
-        const int q = warp & 3;
+        // ------------------------------------------------------------ epilogue (every CTA, its own 128 n): two warps to a quarter of the
+        // lanes, each takes every other 32 columns
+        const int q = warp & 3, turn = (warp - 2) >> 2;
         const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+        uint8_t* out_tile = out_tiles + (turn * 2 + (q >> 1)) * 4096;
         int lt = 0, e = 0;
+        bool ok = true;
         GroupedTile g;
-        for (int t = pair; grouped_tile<MODE>(p, off, first, t, e, g); t += num_pairs) {
-            const int acc = lt & 1;
-            const int n = g.n0 + static_cast<int>(rank) * 128 + q * 32;
-            O* dst = static_cast<O*>(p.c) + (MODE == GR_GRAD ? g.e * p.bs_c : 0) + g.c0 * p.ldc + n;
-            if (g.num_kb) {
-                if (!bounded_wait_warp(&tfull_bar[acc], (lt >> 1) & 1, ab, ST_TIMEOUT_EPILOGUE, lane)) break;
-                ptx::tc_fence_after_sync();
-            }
+        for (int t = worker; ok && grouped_tile<MODE, VAR>(p, off, first, t, e, g); t += num_workers) {
 #pragma unroll 1
-            for (int c = 0; c < g.cols; c += 32) {
-                const uint32_t taddr = lane_base + acc * 256 + c;
-                if constexpr (sizeof(O) == 2) {
-                    if (p.wide_out) {
-                        grouped_put(taddr, g.num_kb == 0, out_tiles + (q * 2 + ((c >> 5) & 1)) * 2048, dst + c * p.ldc, p.ldc, p.N - n, g.cols - c, lane);
-                        continue;
+            for (int u = 0; u < kSub; ++u) {
+                const int acc = kSub == 2 ? u : lt & 1;
+                const uint32_t parity = kSub == 2 ? lt & 1 : (lt >> 1) & 1;
+                const int n = g.n0 + u * 256 + rank * 128 + q * 32;
+                O* dst = static_cast<O*>(p.c) + (MODE == GR_GRAD ? g.e * p.bs_c : 0) + g.c0 * p.ldc + n;
+                if (g.num_kb) {
+                    if (!bounded_wait_warp(&tfull_bar[acc], parity, ab, ST_TIMEOUT_EPILOGUE, lane)) { ok = false; break; }
+                    ptx::tc_fence_after_sync();
+                }
+                const int n64 = n & ~63;   // of the two warps that write together
+                if (n64 < p.N) {
+#pragma unroll 1
+                    for (int c = turn * 32; c < g.cols; c += 64) {
+                        const uint32_t taddr = lane_base + acc * Cfg::kTileC + c;
+                        if constexpr (sizeof(O) == 2) {
+                            if (p.wide_out) {
+                                grouped_put(taddr, g.num_kb == 0, out_tile, dst + (n64 - n) + c * p.ldc, p.ldc, p.N - n64, g.cols - c, lane, q & 1,
+                                            1 + turn * 2 + (q >> 1));
+                                continue;
+                            }
+                        }
+                        uint32_t r[32];
+                        if (g.num_kb) {
+                            ptx::tmem_ld_32x32(taddr, r);
+                            ptx::tmem_ld_wait();
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) r[j] = 0u;
+                        }
+                        if (n + lane < p.N) grouped_store(dst + c * p.ldc + lane, p.ldc, g.cols - c, r);
                     }
                 }
-                uint32_t r[32];
                 if (g.num_kb) {
-                    ptx::tmem_ld_32x32(taddr, r);
-                    ptx::tmem_ld_wait();
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) r[j] = 0u;
+                    ptx::tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if constexpr (kPair == 2) ptx::mbar_arrive_peer(&tempty_bar[acc], 0);
+                        else ptx::mbar_arrive(&tempty_bar[acc]);
+                    }
                 }
-                if (n + lane < p.N) grouped_store(dst + c * p.ldc + lane, p.ldc, g.cols - c, r);
             }
-            if (g.num_kb) {
-                ptx::tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive_peer(&tempty_bar[acc], 0);
-                ++lt;
-            }
+            if (g.num_kb) ++lt;
         }
     }
 
@@ -394,10 +518,10 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
     ptx::tc_fence_before_sync();
     __syncthreads();
     if (*abort_slot) __nanosleep(200000);
-    ptx::cluster_sync();  // neither CTA may release shared memory or TMEM the pair's MMAs still use
+    if constexpr (kPair == 2) ptx::cluster_sync();  // neither CTA may release shared memory or TMEM the pair's MMAs still use
     if (warp == 1) {
         ptx::tc_fence_after_sync();
-        ptx::tmem_dealloc<2>(tmem_base, Cfg::kTmemCols);
+        ptx::tmem_dealloc<kPair>(tmem_base, Cfg::kTmemCols);
     }
 }
 
