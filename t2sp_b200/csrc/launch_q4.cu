@@ -349,18 +349,20 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
 
 
 // Two ways to multiply, by the number of rows that share a pass over the weights.
-//   INT  a few rows: the weights stay unsigned nibbles, whose offset 8 the sum of x over the group takes out, and x is written, group by group of k, as 24-bit integers times a power of two, in three signed bytes, and each byte is a column of
-//        m16n8k32: two operations turn a word of weights into operands, half as many instructions as with 16-bit products, and the sums of
-//        a group are exact. A value of x down to 2^-11 of its group's largest is held exactly (bf16: 2^-14); a smaller one is off by at
-//        most 2^-23 of the largest, about what an fp32 sum over the group rounds away at each step.
+//   INT  a few rows: the weights stay unsigned nibbles, whose offset 8 the sum of x over the group takes out, and a row of x is written
+//        as 32-bit integers times one power of two, in four signed bytes; each byte is a column of m16n8k32. Two operations turn a word of weights into
+//        operands, half as many instructions as with 16-bit products, and the sums of a group are exact. A value of x is off by at most
+//        2^-31 of its row's largest, where an fp32 sum over the row rounds at 2^-24 of a partial sum at every step; values down to 2^-19
+//        of the largest (bf16: 2^-22) are exact.
 //   else x stays in 16 bits, one column of m16n8k16 a row, with the nibbles as 16-bit numbers (Q4Frag).
 template <int NT, bool INT>
 struct GemvShape {
     static constexpr int kCols = 8 * NT;
-    static constexpr int kPerRow = INT ? 3 : 1;                 // columns of a row
+    static constexpr int kPerRow = INT ? 4 : 1;                 // columns of a row
     static constexpr int kRows = kCols / kPerRow;               // rows of a pass
     static constexpr int kBlockBytes = INT ? 64 : 128;          // of a column, for 64 k
-    static constexpr int kSumBytes = INT ? 8 : 0;               // of a column, for a group
+    static constexpr int kFlush = INT ? 4 : 1;                  // strips whose partial sums meet at a time
+    static constexpr int kPartPitch = INT ? kRows : kCols + 1;  // floats of an n of them
 };
 
 // Shared memory of q4_gemv_kernel. A staged column of x holds, for each block of 64 k and each t = 0 .. 3, the bytes that lanes 4 g + t
@@ -368,20 +370,36 @@ struct GemvShape {
 // lanes of a load (two columns, four t) meet every bank once.
 template <int NT, bool INT>
 struct GemvLayout {
-    int pitch, xs, part, ring, bars, rows, units, idx, bytes;   // byte offsets
+    int pitch, xi, part, ring, bars, rows, units, idx, bytes;   // byte offsets
     __host__ __device__ GemvLayout(int kblocks, int groups, int unit_rows, int depth, int R, bool indexed) {
         using S = GemvShape<NT, INT>;
         pitch = INT ? (kblocks | 1) * 64 : kblocks * 128 + 16;
-        xs = (unit_rows * S::kPerRow * pitch + 15) & ~15;
-        part = (xs + groups * S::kCols * S::kSumBytes + 15) & ~15;
-        ring = part + ((2 * kGemvWarps * 16 * (S::kCols + 1) * 4 + 127) & ~127);
+        xi = (unit_rows * S::kPerRow * pitch + 15) & ~15;
+        part = (xi + (INT ? groups * S::kCols * 4 : 0) + 15) & ~15;
+        ring = (part + 2 * S::kFlush * kGemvWarps * 16 * S::kPartPitch * 4 + 127) & ~127;
         bars = ring + kGemvWarps * depth * kGemvSlot;
         rows = bars + kGemvWarps * depth * 16;
-        units = rows + S::kCols * 4 + 16;
+        units = rows + 2 * S::kCols * 4 + 16;
         idx = units + (indexed ? R * 4 : 0);
         bytes = idx + (indexed ? R * 4 : 0);
     }
 };
+
+// What an integer sum of a group starts from, beside -8 times the sum of x's bytes: as the bits of a float this is 1.5 * 2^23, and an integer
+// within 2^22 added to the bits is one added to the number, so a subtraction turns the sum into a float.
+constexpr int kGemvZero = 0x4b400000;
+
+// The largest power of two f1 * f2 that keeps a row whose largest magnitude has the bits `top` within four signed bytes (at most 127 * 16843009
+// in magnitude); true if the row holds a value that is not finite. Two factors: the power itself may leave fp32's range. Subnormal
+// numbers are taken for 2^-126, where nothing of a 16-bit type needs more.
+__device__ __forceinline__ bool gemv_scale(uint32_t top, float& f1, float& f2) {
+    const bool bad = top >= 0x7f800000u;
+    const int up = bad ? 0 : 30 - max(static_cast<int>(top >> 23) - 127, -126), up1 = up >> 1;
+    f1 = __uint_as_float(static_cast<uint32_t>(up1 + 127) << 23);
+    f2 = __uint_as_float(static_cast<uint32_t>(up - up1 + 127) << 23);
+    if (__uint_as_float(top) * f1 * f2 > 2139062143.f) f2 *= 0.5f;
+    return bad;
+}
 
 // Y[r] = X[r / per] x W[index[r]]. Work items are (unit, strip of 16 n), where a unit is up to `unit_rows` rows that name one matrix:
 // a matrix is read once for all of them. Every CTA takes an equal run of consecutive items, stages a unit's rows of x in shared memory once, with
@@ -396,13 +414,13 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
     constexpr int kCols = S::kCols;
     const int kblocks = q4_kblocks(p.K), strips = q4_strips(p.N), groups = q4_groups(p.K, G);
     const GemvLayout<NT, INT> lay(kblocks, groups, unit_rows, depth, p.R, p.index != nullptr);
-    int* xi = reinterpret_cast<int*>(smem_raw + lay.xs);        // INT, [group][column]: -8 times the sum of the bytes of x, and behind all of them
-    float* xf = reinterpret_cast<float*>(xi + groups * kCols);  // what a unit of the integer sums is worth
+    int* xi = reinterpret_cast<int*>(smem_raw + lay.xi);        // INT, [group][column]: see kGemvZero
     float* part = reinterpret_cast<float*>(smem_raw + lay.part);
     int* rows = reinterpret_cast<int*>(smem_raw + lay.rows);
     int* units = reinterpret_cast<int*>(smem_raw + lay.units);
     int* idx = reinterpret_cast<int*>(smem_raw + lay.idx);
-    int* count_slot = rows + kCols;
+    uint32_t* top = reinterpret_cast<uint32_t*>(rows + kCols);  // INT: the largest magnitude of each row, as the bits of a float
+    int* count_slot = rows + 2 * kCols;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int group = warp / gs, wig = warp % gs, num_groups = kGemvWarps / gs;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + lay.bars);   // [group][depth] filled, then [group][depth] free
@@ -414,6 +432,8 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
         }
         ptx::fence_mbar_init();
     }
+    ptx::grid_dep_launch();
+    ptx::grid_dep_wait();
 
     // units: the rows whose number among the rows of their matrix is a multiple of unit_rows start one
     int num_units;
@@ -502,7 +522,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
     const uint8_t* ring = smem_raw + lay.ring + group * depth * slot_bytes;
     uint64_t* full = bars + group * depth;
     uint64_t* freed = full + num_groups * depth;
-    int flip = 0;
+    int flip = 0, held = 0;
     int c_slot = 0;          // next slot to read
     uint32_t c_phase = 0;
 
@@ -531,95 +551,96 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
                 for (int i = lane; i < found; i += 32) rows[i] = lead + i;
             }
             if (lane == 0) *count_slot = found;
+            if (lane < kCols) top[lane] = 0u;
         }
         ptx::bar_sync(15, kGemvWarps * 32);
         const int count = *count_slot;
-        const int pieces = kblocks * 8, padded = (pieces + 15) & ~15;   // of 8 k; a row's lanes start on a group of lanes
+        // x in pieces of 8 k, a warp's 32 pieces of one row at a time; the first ones stay in registers between the two looks at them
+        const int pieces = kblocks * 8, runs = (pieces + 31) / 32, total = count * runs;
         constexpr int kLanes = G / 8;                                   // lanes that hold a group
-        for (int row = 0; row < count; ++row)
-            for (int k0 = warp * 32; k0 < padded; k0 += kGemvWarps * 32) {   // whole warps: the shuffles need every lane
-                const int k8 = k0 + lane;
-                const bool real = k8 < pieces;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (real) {
-                    const long long k = k8 * 8ll;
-                    const uint16_t* src = static_cast<const uint16_t*>(p.x) + (rows[row] / p.per) * p.ldx + k;
-                    if (x_aligned && k + 8 <= p.K) {
-                        v = *reinterpret_cast<const uint4*>(src);
-                    } else {
-                        uint32_t* w = &v.x;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (k + j < p.K) w[j >> 1] |= uint32_t(src[j]) << (16 * (j & 1));
-                    }
-                }
-                const float2 a = pair_f32<T>(v.x), b = pair_f32<T>(v.y), c = pair_f32<T>(v.z), d = pair_f32<T>(v.w);
-                const float f[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-                // k = 16 w + 4 t + j of block k8 / 8: w = (k8 % 8) / 2, t = 2 (k8 % 2) and the next
-                if constexpr (INT) {
-                    float top = 0.f;
-                    bool bad = false;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        top = fmaxf(top, fabsf(f[j]));
-                        bad = bad || !(fabsf(f[j]) < __int_as_float(0x7f800000));
-                    }
-#pragma unroll
-                    for (int m = 1; m < kLanes; m <<= 1) {
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-                        bad = __shfl_xor_sync(0xffffffffu, bad, m) || bad;
-                    }
-                    // The largest power of two that keeps the integers within three signed bytes (127 * 65793): top < 2^(e + 1) has e in
-                    // its exponent bits. Subnormal numbers are taken for 2^-126, where nothing of a 16-bit type needs more.
-                    const int e = max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -126);
-                    int up = bad ? 0 : 22 - e;
-                    const int up1 = up >> 1;   // in two steps: 2^up itself may leave fp32's range
-                    float f1 = __uint_as_float(static_cast<uint32_t>(up1 + 127) << 23), f2 = __uint_as_float(static_cast<uint32_t>(up - up1 + 127) << 23);
-                    if (top * f1 * f2 > 8355711.f) { --up; f2 *= 0.5f; }
-                    // x + 0x808080 as an unsigned number: its bytes less 128 are the signed bytes
-                    uint32_t u[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) u[j] = bad ? 0x808080u : __float2int_rn(f[j] * f1 * f2) + 0x808080;
-                    uint32_t digits[3][2];
-                    int sums[3];
-#pragma unroll
-                    for (int n = 0; n < 3; ++n) {
-                        const uint32_t sel = n | ((4 + n) << 4);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            digits[n][h] = __byte_perm(__byte_perm(u[4 * h], u[4 * h + 1], sel), __byte_perm(u[4 * h + 2], u[4 * h + 3], sel), 0x5410) ^ 0x80808080u;
-                        sums[n] = __dp4a(static_cast<int>(digits[n][0]), 0x01010101, __dp4a(static_cast<int>(digits[n][1]), 0x01010101, 0));
-                    }
-                    // two sums to a word on the way over the lanes: each stays within 2^14
-                    int low = sums[0] + sums[1] * 65536;
-#pragma unroll
-                    for (int m = 1; m < kLanes; m <<= 1) {
-                        low += __shfl_xor_sync(0xffffffffu, low, m);
-                        sums[2] += __shfl_xor_sync(0xffffffffu, sums[2], m);
-                    }
-                    sums[0] = static_cast<int16_t>(low & 0xffff);
-                    sums[1] = (low - sums[0]) >> 16;
-                    const float back = __uint_as_float(static_cast<uint32_t>(127 - (up >> 1)) << 23) * __uint_as_float(static_cast<uint32_t>(127 - (up - (up >> 1))) << 23);
-                    if (real) {
-#pragma unroll
-                        for (int n = 0; n < 3; ++n) {
-                            uint8_t* dst = smem_raw + (row * 3 + n) * lay.pitch + (k8 >> 3) * 64 + (k8 & 1) * 32 + ((k8 >> 1) & 3) * 4;
-                            *reinterpret_cast<uint32_t*>(dst) = digits[n][0];
-                            *reinterpret_cast<uint32_t*>(dst + 16) = digits[n][1];
-                            if (k8 % kLanes == 0) {
-                                xi[(k8 / kLanes) * kCols + row * 3 + n] = -8 * sums[n];
-                                xf[(k8 / kLanes) * kCols + row * 3 + n] = bad ? __int_as_float(0x7fc00000) : back * static_cast<float>(1 << (8 * n));
-                            }
-                        }
-                    }
+        constexpr int kKeep = 4;
+        auto piece = [&](int i) -> uint4 {
+            const int row = i / runs, k8 = (i - row * runs) * 32 + lane;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (i < total && k8 < pieces) {
+                const long long k = k8 * 8ll;
+                const uint16_t* src = static_cast<const uint16_t*>(p.x) + (rows[row] / p.per) * p.ldx + k;
+                if (x_aligned && k + 8 <= p.K) {
+                    v = *reinterpret_cast<const uint4*>(src);
                 } else {
-                    if (real) {   // in the order j = 0, 2, 1, 3 of the weights' pairs
-                        uint8_t* dst = smem_raw + row * lay.pitch + (k8 >> 3) * 128 + (k8 & 1) * 64 + ((k8 >> 1) & 3) * 8;
-                        *reinterpret_cast<uint2*>(dst) = make_uint2(__byte_perm(v.x, v.y, 0x5410), __byte_perm(v.x, v.y, 0x7632));
-                        *reinterpret_cast<uint2*>(dst + 32) = make_uint2(__byte_perm(v.z, v.w, 0x5410), __byte_perm(v.z, v.w, 0x7632));
-                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (k + j < p.K) (&v.x)[j >> 1] |= uint32_t(src[j]) << (16 * (j & 1));
                 }
             }
+            return v;
+        };
+        uint4 kept[kKeep];
+#pragma unroll
+        for (int n = 0; n < kKeep; ++n) kept[n] = piece(warp + n * kGemvWarps);
+        if constexpr (INT) {
+            auto look = [&](int i, const uint4& v) {
+                uint32_t m = max_abs2<T>(max_abs2<T>(max_abs2<T>(max_abs2<T>(0u, v.x), v.y), v.z), v.w);
+                const float2 f = pair_f32<T>(max_abs2<T>(m, __byte_perm(m, m, 0x1032)));
+                const uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(f.x) & 0x7fffffffu);   // a NaN's bits are above infinity's
+                if (lane == 0) atomicMax(&top[i / runs], b);
+            };
+#pragma unroll
+            for (int n = 0; n < kKeep; ++n)
+                if (warp + n * kGemvWarps < total) look(warp + n * kGemvWarps, kept[n]);
+            for (int i = warp + kKeep * kGemvWarps; i < total; i += kGemvWarps) look(i, piece(i));
+            ptx::bar_sync(15, kGemvWarps * 32);
+        }
+        auto place = [&](int i, const uint4& v) {
+            const int row = i / runs, k8 = (i - row * runs) * 32 + lane;
+            const bool real = k8 < pieces;
+            // k = 16 w + 4 t + j of block k8 / 8: w = (k8 % 8) / 2, t = 2 (k8 % 2) and the next
+            if constexpr (INT) {
+                float f1, f2;
+                const bool bad = gemv_scale(top[row], f1, f2);
+                const float2 a = pair_f32<T>(v.x), b = pair_f32<T>(v.y), c = pair_f32<T>(v.z), d = pair_f32<T>(v.w);
+                const float f[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+                // x + 0x80808080 as an unsigned number: its bytes less 128 are the signed bytes
+                uint32_t u[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) u[j] = (bad ? 0u : static_cast<uint32_t>(__float2int_rn(f[j] * f1 * f2))) + 0x80808080u;
+                int sums[4];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const uint32_t sel = n | ((4 + n) << 4);
+                    uint32_t digits[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        digits[h] = __byte_perm(__byte_perm(u[4 * h], u[4 * h + 1], sel), __byte_perm(u[4 * h + 2], u[4 * h + 3], sel), 0x5410) ^ 0x80808080u;
+                    sums[n] = __dp4a(static_cast<int>(digits[0]), 0x01010101, __dp4a(static_cast<int>(digits[1]), 0x01010101, 0));
+                    if (real) {
+                        uint8_t* dst = smem_raw + (row * 4 + n) * lay.pitch + (k8 >> 3) * 64 + (k8 & 1) * 32 + ((k8 >> 1) & 3) * 4;
+                        *reinterpret_cast<uint32_t*>(dst) = digits[0];
+                        *reinterpret_cast<uint32_t*>(dst + 16) = digits[1];
+                    }
+                }
+                // two sums to a word on the way over the group's lanes: each stays within 2^14
+                int lo = sums[0] + sums[1] * 65536, hi = sums[2] + sums[3] * 65536;
+#pragma unroll
+                for (int m = 1; m < kLanes; m <<= 1) {
+                    lo += __shfl_xor_sync(0xffffffffu, lo, m);
+                    hi += __shfl_xor_sync(0xffffffffu, hi, m);
+                }
+                if (real && k8 % kLanes == 0) {
+                    const int s0 = static_cast<int16_t>(lo & 0xffff), s2 = static_cast<int16_t>(hi & 0xffff);
+                    *reinterpret_cast<int4*>(xi + (k8 / kLanes) * kCols + row * 4) =
+                        make_int4(kGemvZero - 8 * s0, kGemvZero - 8 * ((lo - s0) >> 16), kGemvZero - 8 * s2, kGemvZero - 8 * ((hi - s2) >> 16));
+                }
+            } else if (real) {   // in the order j = 0, 2, 1, 3 of the weights' pairs
+                uint8_t* dst = smem_raw + row * lay.pitch + (k8 >> 3) * 128 + (k8 & 1) * 64 + ((k8 >> 1) & 3) * 8;
+                *reinterpret_cast<uint2*>(dst) = make_uint2(__byte_perm(v.x, v.y, 0x5410), __byte_perm(v.x, v.y, 0x7632));
+                *reinterpret_cast<uint2*>(dst + 32) = make_uint2(__byte_perm(v.z, v.w, 0x5410), __byte_perm(v.z, v.w, 0x7632));
+            }
+        };
+#pragma unroll
+        for (int n = 0; n < kKeep; ++n)
+            if (warp + n * kGemvWarps < total) place(warp + n * kGemvWarps, kept[n]);
+        for (int i = warp + kKeep * kGemvWarps; i < total; i += kGemvWarps) place(i, piece(i));
         ptx::bar_sync(15, kGemvWarps * 32);
 
         // lanes of columns without a row read column 0 of x: what they compute is in columns that are not stored
@@ -678,11 +699,10 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             if constexpr (INT) {
-                                const float2 m = *reinterpret_cast<const float2*>(xf + at0 + in_slot * kCols + n * 8);
-                                acc[n][0] += f.x * (m.x * ci[n][0]);
-                                acc[n][1] += f.x * (m.y * ci[n][1]);
-                                acc[n][2] += f.y * (m.x * ci[n][2]);
-                                acc[n][3] += f.y * (m.y * ci[n][3]);
+                                acc[n][0] += f.x * (__int_as_float(ci[n][0]) - __int_as_float(kGemvZero));
+                                acc[n][1] += f.x * (__int_as_float(ci[n][1]) - __int_as_float(kGemvZero));
+                                acc[n][2] += f.y * (__int_as_float(ci[n][2]) - __int_as_float(kGemvZero));
+                                acc[n][3] += f.y * (__int_as_float(ci[n][3]) - __int_as_float(kGemvZero));
                             } else {
                                 acc[n][0] += f.x * c[n][0];
                                 acc[n][1] += f.x * c[n][1];
@@ -711,29 +731,45 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
                 if (lane == 0) ptx::mbar_arrive(&freed[c_slot]);
                 if (++c_slot == depth) { c_slot = 0; c_phase ^= 1u; }
             }
-            float* mine = part + (flip * kGemvWarps + warp) * 16 * (kCols + 1);
+            float* mine = part + ((flip * S::kFlush + held) * kGemvWarps + warp) * 16 * S::kPartPitch;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n) {
+                if constexpr (INT) {
+                    // bytes 0, 1 of a row in the lanes with even t, bytes 2, 3 in the next lanes
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    mine[(g + (j >> 1) * 8) * (kCols + 1) + n * 8 + 2 * t + (j & 1)] = acc[n][j];
-            ptx::bar_sync(1 + group, gs * 32);
-            // two buffers in turn: this one is written again only after the barrier of the next strip
-            for (int i = wig * 32 + lane; i < 16 * count; i += gs * 32) {
-                const int n = i & 15, col = i >> 4;
-                const float* from = part + (flip * kGemvWarps + group * gs) * 16 * (kCols + 1) + n * (kCols + 1) + col * S::kPerRow;
-                float v = 0.f;
-                for (int w = 0; w < gs; ++w, from += 16 * (kCols + 1)) {
-                    if constexpr (INT) v += (from[0] + from[1]) + from[2];   // the smallest byte's sum first
-                    else v += from[0];
+                    for (int h = 0; h < 2; ++h) {
+                        const float v = acc[n][2 * h] + 256.f * acc[n][2 * h + 1];
+                        const float v2 = __shfl_xor_sync(0xffffffffu, v, 1);
+                        if (t % 2 == 0) mine[(g + 8 * h) * S::kPartPitch + n * 2 + (t >> 1)] = v + 65536.f * v2;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mine[(g + (j >> 1) * 8) * S::kPartPitch + n * 8 + 2 * t + (j & 1)] = acc[n][j];
                 }
-                if (strip * 16 + n < p.N) {
-                    const long long at = rows[col] * p.ldy + strip * 16 + n;
+            }
+            if (++held < S::kFlush && strip + num_groups < s_end) continue;
+            ptx::bar_sync(1 + group, gs * 32);
+            // two buffers in turn: this one is written again only after the barrier of the next flush
+            for (int i = wig * 32 + lane; i < held * 16 * count; i += gs * 32) {
+                const int n = i & 15, col = (i >> 4) % count, f = (i >> 4) / count;
+                const float* from = part + ((flip * S::kFlush + f) * kGemvWarps + group * gs) * 16 * S::kPartPitch + n * S::kPartPitch + col;
+                float v = 0.f;
+#pragma unroll 4
+                for (int w = 0; w < gs; ++w) v += from[w * 16 * S::kPartPitch];
+                if constexpr (INT) {
+                    float f1, f2;
+                    const bool bad = gemv_scale(top[col], f1, f2);
+                    v = bad ? __int_as_float(0x7fc00000) : v * (1.f / f1) * (1.f / f2);   // powers of two
+                }
+                const int n_at = (strip - (held - 1 - f) * num_groups) * 16 + n;
+                if (n_at < p.N) {
+                    const long long at = rows[col] * p.ldy + n_at;
                     if (p.out_f32) static_cast<float*>(p.y)[at] = v;
                     else static_cast<T*>(p.y)[at] = rounded<T>(v);
                 }
             }
             flip ^= 1;
+            held = 0;
         }
     }
 }
@@ -775,8 +811,7 @@ cudaError_t gemv_launch(const Q4Params& p, cudaStream_t stream) {
         const long long cost = (per_cta * n + 15) / 16 * (2 * ((kblocks + n * kGemvBlocks - 1) / (n * kGemvBlocks)) + 1);
         if (n == 16 || cost < best) { best = cost; gs = n; }
     }
-    kern<<<grid, kGemvThreads, plan.bytes, stream>>>(p, gs, plan.unit_rows, plan.depth);
-    return cudaGetLastError();
+    return launch_behind(kern, grid, kGemvThreads, plan.bytes, stream, p, gs, plan.unit_rows, plan.depth);
 }
 
 template <class T, int NT, bool INT>
@@ -790,8 +825,8 @@ cudaError_t gemv_typed(const Q4Params& p, cudaStream_t stream) {
     const bool indexed = p.index != nullptr;
     // rows that may be expected to share a matrix: with an index the mean over the matrices
     const int rows = indexed && p.E > 0 ? (p.R + p.E - 1) / p.E : p.R;
-    if (rows <= 2) return gemv_group<T, 1, true>(p, stream);
-    if (rows <= 5 && gemv_plan<2, true>(p.K, p.group, p.R, indexed).unit_rows >= rows) return gemv_group<T, 2, true>(p, stream);
+    if (rows <= 2 && gemv_plan<1, true>(p.K, p.group, p.R, indexed).unit_rows >= rows) return gemv_group<T, 1, true>(p, stream);
+    if (rows <= 4 && gemv_plan<2, true>(p.K, p.group, p.R, indexed).unit_rows >= rows) return gemv_group<T, 2, true>(p, stream);
     const bool two = rows > 8 && gemv_plan<2, false>(p.K, p.group, p.R, indexed).unit_rows > 8;
     return two ? gemv_group<T, 2, false>(p, stream) : gemv_group<T, 1, false>(p, stream);
 }
@@ -828,7 +863,7 @@ cudaError_t q4_unpack_launch(const Q4Params& p, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
-bool q4_gemv_fits(int K, int group, int R, bool indexed) { return gemv_plan<1, true>(K, group, 1, indexed).unit_rows > 0 && gemv_plan<1, false>(K, group, R, indexed).unit_rows > 0; }
+bool q4_gemv_fits(int K, int group, int R, bool indexed) { return gemv_plan<1, false>(K, group, R, indexed).unit_rows > 0; }
 
 cudaError_t q4_gemv_launch(const Q4Params& p, cudaStream_t stream) {
     return p.bf16 ? gemv_typed<__nv_bfloat16>(p, stream) : gemv_typed<__half>(p, stream);

@@ -22,4 +22,21 @@ cudaError_t allow_smem(Kern kern, int bytes, std::atomic<bool>* configured) {
     return cudaSuccess;
 }
 
+// Launch with programmatic stream serialization: it is set up while the kernel before it ends. The kernel calls
+// ptx::grid_dep_wait() before it touches memory.
+template <class... Args>
+cudaError_t launch_behind(void (*kern)(Args...), unsigned grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
 }  // namespace t2sp

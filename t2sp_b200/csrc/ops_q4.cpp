@@ -175,7 +175,7 @@ extern "C" int t2sp_b200_q4_gemv(halide_buffer_t* X, halide_buffer_t* Q, halide_
     if (!index && p.E != 1) return constraint("Q.extent.3", p.E, "one matrix where no index is given", 1);
     if (index && index->dim[0].extent != p.R) return constraint("index.extent.0", index->dim[0].extent, "Y.extent.1", p.R);
     if (index && p.R > 1024) return constraint("Y.extent.1", p.R, "at most 1024 rows where an index is given", 1024);
-    if (!q4_gemv_fits(p.K, group, p.R, index != nullptr)) return constraint("X.extent.0", p.K, "at most about", 32768);   // a row of x is staged whole in shared memory
+    if (!q4_gemv_fits(p.K, group, p.R, index != nullptr)) return constraint("X.extent.0", p.K, "at most about", 65536);   // a row of x is staged whole in shared memory
     if (T == 0 || p.R % T) return constraint("Y.extent.1", p.R, "a multiple of X.extent.1", T);
     for (int i = 0; i < n_args; ++i)
         if (int e = check_min0(args[i])) return e;

@@ -109,7 +109,7 @@ def test_pack_infinities_and_nan(lib):
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 @pytest.mark.parametrize("R,K,N,group", [(1, 64, 16, 64), (1, 1, 1, 32), (1, 4096, 520, 64), (2, 100, 40, 32), (7, 1001, 777, 32), (8, 512, 48, 128),
                                          (9, 130, 33, 128), (17, 192, 64, 64), (33, 256, 80, 32), (70, 64, 17, 64), (3, 8200, 24, 128), (9, 30000, 20, 64),
-                                         (1, 32000, 16, 128), (1100, 64, 16, 64)])
+                                         (1, 65000, 16, 128), (1, 16000, 20, 32), (1100, 64, 16, 64)])
 def test_gemv_one_matrix(lib, R, K, N, group, dtype):
     import torch
     dt = getattr(torch, dtype)
@@ -285,7 +285,7 @@ def test_experts_of_a_layer_together(lib):
 @pytest.mark.parametrize("R", [1, 4, 8])
 def test_gemv_ranges_of_x(lib, R, dtype):
     """Rows of x over the whole range of their type: outliers, numbers near the largest and the smallest, zeros, subnormal numbers.
-    A value may be held to 2^-23 of the largest one in its group of k: that is added to the tolerance."""
+    A value may be held to 2^-31 of the largest one in its row: that is added to the tolerance."""
     import torch
     dt = getattr(torch, dtype)
     fi = torch.finfo(dt)
@@ -307,9 +307,9 @@ def test_gemv_ranges_of_x(lib, R, dtype):
             Q, S = packed(w, group)
             assert t2sp_b200.q4_gemv(buf(only), buf(Q), buf(S), None, buf(y), Q4Desc(group, 0)) == 0
         v, u = only.double(), quantised64(w, group)[0]
-        top = v.abs().view(R, K // group, group).amax(2)
+        top = v.abs().amax(1, keepdim=True)
         tol = ((group // 16 + 16) + (K // group + 16)) * 2.0 ** -23 * (v.abs() @ u.abs())
-        tol = tol + 2.0 ** -23 * (top @ u.abs().view(K // group, group, N).sum(1)) + 2.0 ** -140
+        tol = tol + 2.0 ** -31 * top * u.abs().sum(0) + 2.0 ** -140
         assert ((y.double() - v @ u).abs() <= tol).all(), part
 
 
