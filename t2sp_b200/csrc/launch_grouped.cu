@@ -40,6 +40,36 @@ cudaError_t launch_var(int out, const GroupedParams& p, const GroupedMaps& maps,
     return launch_typed<MODE, VAR, __half>(p, maps, workers, stream);
 }
 
+template <int MODE, class O>
+cudaError_t split_typed(const GroupedParams& p, const GroupedMaps& maps, int workers, int splits, cudaStream_t stream) {
+    auto kern = grouped_split_kernel<MODE, O>;
+    static std::atomic<bool> configured[kMaxDev];
+    if (cudaError_t e = allow_smem(kern, SplitCfg::kSmemBytes, configured)) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(workers * splits);
+    cfg.blockDim = dim3(SplitCfg::kThreads);
+    cfg.dynamicSmemBytes = SplitCfg::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, p, maps, splits);
+}
+
+template <int MODE>
+cudaError_t launch_split(int out, const GroupedParams& p, const GroupedMaps& maps, long long tiles, int splits, cudaStream_t stream) {
+    const long long slots = core_sm_count() / splits;
+    const int workers = static_cast<int>(tiles < slots ? (tiles > 0 ? tiles : 1) : slots);
+    if (out == GR_OUT_F32) return split_typed<MODE, float>(p, maps, workers, splits, stream);
+    if (out == GR_OUT_BF16) return split_typed<MODE, __nv_bfloat16>(p, maps, workers, splits, stream);
+    return split_typed<MODE, __half>(p, maps, workers, splits, stream);
+}
+
 // Tiles of a call: how the rows fall into the groups is known on the device only. `most`: an upper bound (a tile of each group
 // more than the rows alone would need); else as if the rows were spread evenly.
 long long count_tiles(int mode, const GroupedParams& p, int tn, int tc, bool most) {
@@ -64,9 +94,14 @@ cudaError_t launch_mode(int out, const GroupedParams& p, const GroupedMaps& maps
     const int kb = MODE == GR_GRAD ? p.rows / (p.E * 64) : (p.K + 63) / 64;
     if (kb >= (MODE == GR_GRAD ? 12 : 32) && 200 * rounds512 <= 108 * rounds256)
         return launch_var<MODE, GR_TILE_512>(out, p, maps, count_tiles(MODE, p, 512, 256, true), stream);
-    if constexpr (MODE != GR_GRAD)
+    if constexpr (MODE != GR_GRAD) {
+        const long long t128 = count_tiles(MODE, p, 128, 128, false);
+        for (int splits = 8; splits >= 2; splits /= 2)
+            if (t128 * splits <= core_sm_count() - (splits == 8 ? 20 : 4) && kb >= 2 * splits)   // clusters do not fill every GPC
+                return launch_split<MODE>(out, p, maps, count_tiles(MODE, p, 128, 128, true), splits, stream);
         if (2 * count_tiles(MODE, p, 256, 256, false) <= pairs)
             return launch_var<MODE, GR_TILE_128>(out, p, maps, count_tiles(MODE, p, 128, 128, true), stream);
+    }
     return launch_var<MODE, GR_TILE_256>(out, p, maps, count_tiles(MODE, p, 256, 256, true), stream);
 }
 

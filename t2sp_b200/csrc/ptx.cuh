@@ -341,6 +341,11 @@ __device__ __forceinline__ uint32_t map_to_cta(const void* p, uint32_t cta_rank)
     return r;
 }
 
+// Store to shared memory of a CTA of the cluster (address from map_to_cta); visible to it after a cluster barrier.
+__device__ __forceinline__ void st_cluster(uint32_t cluster_addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+
 // ---------------------------------------------------------------- tcgen05: TMEM -> registers
 // 32 lanes x 32 consecutive 32-bit columns; thread t of the warp gets lane (base_lane + t).
 __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32]) {

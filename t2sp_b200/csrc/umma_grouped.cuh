@@ -525,4 +525,175 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
     }
 }
 
+// ---------------------------------------------------------------- few tiles: the contraction split over a cluster
+// Forward products of a few rows, or with a few columns, have fewer 128 x 128 tiles than the GPU has SMs, and one SM brings weights at 60 to 80 GB/s
+// only. Here a cluster of `splits` CTAs shares a tile: each adds up its run of k-blocks, hands the fp32 sums of 32 n x 32 columns to the CTA that owns
+// them through distributed shared memory, and the owners add the parts in the order of the ranks and write the results. (8 groups of
+// 2 rows, 1024 x 1024, 64 tiles: two CTAs a tile.)
+struct SplitCfg {
+    static constexpr int kStages = 4;
+    static constexpr int kStageBytes = 2 * 128 * 128;
+    static constexpr int kUnitBytes = 32 * 32 * 4;           // sums of 32 n x 32 columns
+    static constexpr int kPartBytes = 16 * kUnitBytes;       // an owner's units times the ranks: 16 units in a tile
+    static constexpr int kThreads = (2 + 8) * 32;
+    static constexpr int kTmemCols = 128;
+    static constexpr int kTableBytes = 2 * (kMaxGroups + 4) * 4;
+    static constexpr int kSmemBytes = kStages * kStageBytes + kPartBytes + kTableBytes + (2 * kStages + 1) * 8 + 24 + 1024;
+    static_assert(kSmemBytes <= 232448, "shared memory budget exceeded");
+};
+
+template <int MODE, class O>
+__global__ void __launch_bounds__(SplitCfg::kThreads, 1)
+grouped_split_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ GroupedMaps maps, int splits) {
+    constexpr int STAGES = SplitCfg::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float* parts = reinterpret_cast<float*>(smem + STAGES * SplitCfg::kStageBytes);   // [unit of this owner][rank][column][n]
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * SplitCfg::kStageBytes + SplitCfg::kPartBytes);
+    uint64_t* empty_bar = full_bar + STAGES;
+    uint64_t* tfull_bar = empty_bar + STAGES;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull_bar + 1);
+    uint32_t* abort_slot = tmem_slot + 1;
+    int* off = reinterpret_cast<int*>(tmem_slot + 4);
+    int* first = off + kMaxGroups + 4;
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int rank = static_cast<int>(ptx::cluster_ctarank());
+    const AbortCtx ab{abort_slot, p.status, p.wait_cycles > 0 ? p.wait_cycles : kWaitTimeoutCycles};
+    const int worker = blockIdx.x / splits, num_workers = gridDim.x / splits;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            ptx::mbar_init(&full_bar[s], 1);
+            ptx::mbar_init(&empty_bar[s], 1);
+        }
+        ptx::mbar_init(tfull_bar, 1);
+        *abort_slot = 0u;
+        ptx::fence_mbar_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc<1>(tmem_slot, SplitCfg::kTmemCols);
+        ptx::tmem_relinquish<1>();
+    }
+    ptx::grid_dep_launch();
+    ptx::grid_dep_wait();
+    const bool valid = grouped_tables<MODE, GR_TILE_128>(p, off, first);
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::cluster_sync();   // every CTA of the cluster runs before its shared memory is written
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    if (!valid) {
+        if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(p.status, ST_BAD_OFFSETS);
+        if (warp == 1) ptx::tmem_dealloc<1>(tmem_base, SplitCfg::kTmemCols);
+        return;
+    }
+
+    int e = 0, it = 0;
+    uint32_t phase = 0;   // of the accumulator's barrier: it completes once for every tile with k-blocks
+    GroupedTile g;
+    for (int t = worker; grouped_tile<MODE, GR_TILE_128>(p, off, first, t, e, g); t += num_workers) {
+        const int kb0 = rank * g.num_kb / splits, nkb = (rank + 1) * g.num_kb / splits - kb0;   // this CTA's run, possibly empty
+        if (warp == 0) {
+            // -------------------------------------------------------- TMA producer
+            if (lane == 0) {
+                for (int i = 0; i < nkb; ++i) {
+                    const int s = (it + i) % STAGES, kb = kb0 + i;
+                    if (!bounded_wait(&empty_bar[s], (((it + i) / STAGES) & 1) ^ 1, ab, ST_TIMEOUT_PRODUCER)) break;
+                    uint8_t* sp = smem + s * SplitCfg::kStageBytes;
+                    uint8_t* sq = sp + 128 * 128;
+                    ptx::mbar_expect_tx(&full_bar[s], 128 * 128 + g.ncols * 128);
+                    if constexpr (MODE == GR_FWD_MN) {
+                        ptx::tma_load_3d(sp, &maps.p, &full_bar[s], g.n0, kb * 64, g.e);
+                        ptx::tma_load_3d(sp + 8192, &maps.p, &full_bar[s], g.n0 + 64, kb * 64, g.e);
+                    } else {
+                        ptx::tma_load_3d(sp, &maps.p, &full_bar[s], kb * 64, g.n0, g.e);
+                    }
+                    int j = 0;
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+                        if (g.ncols & (128 >> b)) {
+                            ptx::tma_load_2d(sq + j * 128, &maps.q[b], &full_bar[s], kb * 64, g.c0 + j);
+                            j += 128 >> b;
+                        }
+                }
+            }
+        } else if (warp == 1) {
+            // -------------------------------------------------------- MMA issuer
+            if (lane == 0) {
+                const uint32_t idesc = make_instr_desc(1, p.bf16 ? 1 : 0, MODE == GR_FWD_MN, false, 128, g.ncols);
+                constexpr uint32_t kStepP = MODE == GR_FWD_MN ? (16 * 128) >> 4 : 32 >> 4, kStepQ = 32 >> 4;
+                bool ok = true;
+                for (int i = 0; i < nkb && ok; ++i) {
+                    const int s = (it + i) % STAGES;
+                    ok = bounded_wait(&full_bar[s], ((it + i) / STAGES) & 1, ab, ST_TIMEOUT_MMA);
+                    if (!ok) break;
+                    ptx::tc_fence_after_sync();
+                    const uint32_t sp = ptx::smem_u32(smem + s * SplitCfg::kStageBytes);
+                    const uint64_t dp = ptx::make_smem_desc(sp, MODE == GR_FWD_MN ? 8192 : 16, 1024);
+                    const uint64_t dq = ptx::make_smem_desc(sp + 128 * 128, 16, 1024);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        ptx::umma<ptx::KIND_F16, 1>(tmem_base, dp + j * kStepP, dq + j * kStepQ, idesc, (i | j) ? 1u : 0u);
+                    ptx::umma_commit(&empty_bar[s]);
+                }
+                if (ok && nkb) ptx::umma_commit(tfull_bar);
+            }
+        } else {
+            // -------------------------------------------------------- hands 32 n x 32 columns at a time to their owners
+            const int q = warp & 3, turn = (warp - 2) >> 2;
+            bool have = nkb > 0;
+            if (have) {
+                have = bounded_wait_warp(tfull_bar, phase, ab, ST_TIMEOUT_EPILOGUE, lane);
+                ptx::tc_fence_after_sync();
+            }
+            for (int c = turn * 32; c < g.cols; c += 64) {
+                uint32_t r[32];
+                if (have) {
+                    ptx::tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + c, r);
+                    ptx::tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) r[j] = 0u;
+                }
+                const int unit = (c >> 5) * 4 + q;
+                const uint32_t at = ptx::map_to_cta(parts + (unit / splits * splits + rank) * 1024 + lane, unit % splits);
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (c + j < g.cols) ptx::st_cluster(at + j * 128, r[j]);
+            }
+            ptx::tc_fence_before_sync();
+        }
+        it += nkb;
+        if (nkb) phase ^= 1u;
+        __syncwarp();
+        ptx::cluster_sync();   // all parts have arrived
+        ptx::tc_fence_after_sync();
+        if (warp >= 2) {
+            const int units = 4 * ((g.cols + 31) >> 5);
+            for (int i = warp - 2; i < (units - rank + splits - 1) / splits * 32; i += 8) {
+                const int own = i >> 5, unit = own * splits + rank, j = i & 31;
+                const int col = (unit >> 2) * 32 + j, n = g.n0 + (unit & 3) * 32 + lane;
+                if (unit >= units || col >= g.cols) continue;
+                const float* part = parts + (own * splits * 32 + j) * 32 + lane;
+                float v = part[0];
+                for (int k = 1; k < splits; ++k) v += part[k * 1024];
+                if (n < p.N) {
+                    O* dst = static_cast<O*>(p.c) + (g.c0 + col) * p.ldc + n;
+                    if constexpr (sizeof(O) == 4) *dst = v;
+                    else if constexpr (std::is_same<O, __half>::value) *dst = __float2half_rn(v);
+                    else *dst = __float2bfloat16_rn(v);
+                }
+            }
+        }
+        __syncwarp();
+        ptx::cluster_sync();   // the parts have been read: the next tile may overwrite them
+    }
+
+    __syncthreads();
+    if (*abort_slot) __nanosleep(200000);
+    if (warp == 1) ptx::tmem_dealloc<1>(tmem_base, SplitCfg::kTmemCols);
+}
+
 }  // namespace t2sp

@@ -72,6 +72,10 @@ SHAPES = [
     ([1] * 300, 64, 128, 0, 0),
     ([20, 200], 2056, 24, 0, 0),
     ([0, 1700, 0, 0, 900], 256, 776, 0, 16),
+    ([129, 71] * 8, 1024, 100, 0, 3),      # uneven groups: more tiles than an even spread would give
+    ([3], 4104, 136, 1, 1),
+    ([2, 1], 320, 1000, 0, 0),
+    ([2100, 300], 2112, 1032, 0, 0),
 ]
 
 
