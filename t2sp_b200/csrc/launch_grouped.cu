@@ -1,6 +1,7 @@
 // Grouped products: instantiations and launchers (umma_grouped.cuh), and the copy that makes operands fit for TMA.
 #include "umma_grouped.cuh"
 #include "launch_util.cuh"
+#include "row16.cuh"
 #include "umma_launch.h"
 
 namespace t2sp {
@@ -40,15 +41,15 @@ cudaError_t launch_var(int out, const GroupedParams& p, const GroupedMaps& maps,
     return launch_typed<MODE, VAR, __half>(p, maps, workers, stream);
 }
 
-template <int MODE, class O>
+template <int MODE, int VAR, class O>
 cudaError_t split_typed(const GroupedParams& p, const GroupedMaps& maps, int workers, int splits, cudaStream_t stream) {
-    auto kern = grouped_split_kernel<MODE, O>;
+    auto kern = grouped_split_kernel<MODE, VAR, O>;
     static std::atomic<bool> configured[kMaxDev];
-    if (cudaError_t e = allow_smem(kern, SplitCfg::kSmemBytes, configured)) return e;
+    if (cudaError_t e = allow_smem(kern, SplitCfg<VAR>::kSmemBytes, configured)) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(workers * splits);
-    cfg.blockDim = dim3(SplitCfg::kThreads);
-    cfg.dynamicSmemBytes = SplitCfg::kSmemBytes;
+    cfg.blockDim = dim3(SplitCfg<VAR>::kThreads);
+    cfg.dynamicSmemBytes = SplitCfg<VAR>::kSmemBytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -61,13 +62,13 @@ cudaError_t split_typed(const GroupedParams& p, const GroupedMaps& maps, int wor
     return cudaLaunchKernelEx(&cfg, kern, p, maps, splits);
 }
 
-template <int MODE>
+template <int MODE, int VAR>
 cudaError_t launch_split(int out, const GroupedParams& p, const GroupedMaps& maps, long long tiles, int splits, cudaStream_t stream) {
     const long long slots = core_sm_count() / splits;
     const int workers = static_cast<int>(tiles < slots ? (tiles > 0 ? tiles : 1) : slots);
-    if (out == GR_OUT_F32) return split_typed<MODE, float>(p, maps, workers, splits, stream);
-    if (out == GR_OUT_BF16) return split_typed<MODE, __nv_bfloat16>(p, maps, workers, splits, stream);
-    return split_typed<MODE, __half>(p, maps, workers, splits, stream);
+    if (out == GR_OUT_F32) return split_typed<MODE, VAR, float>(p, maps, workers, splits, stream);
+    if (out == GR_OUT_BF16) return split_typed<MODE, VAR, __nv_bfloat16>(p, maps, workers, splits, stream);
+    return split_typed<MODE, VAR, __half>(p, maps, workers, splits, stream);
 }
 
 // Tiles of a call: how the rows fall into the groups is known on the device only. `most`: an upper bound (a tile of each group
@@ -96,30 +97,27 @@ cudaError_t launch_mode(int out, const GroupedParams& p, const GroupedMaps& maps
         return launch_var<MODE, GR_TILE_512>(out, p, maps, count_tiles(MODE, p, 512, 256, true), stream);
     if constexpr (MODE != GR_GRAD) {
         const long long t128 = count_tiles(MODE, p, 128, 128, false);
+        const bool narrow = p.rows <= 32ll * p.E;   // about a tile of 32 columns to a group
         for (int splits = 8; splits >= 2; splits /= 2)
             if (t128 * splits <= core_sm_count() - (splits == 8 ? 20 : 4) && kb >= 2 * splits)   // clusters do not fill every GPC
-                return launch_split<MODE>(out, p, maps, count_tiles(MODE, p, 128, 128, true), splits, stream);
+                return narrow ? launch_split<MODE, GR_TILE_32>(out, p, maps, count_tiles(MODE, p, 128, 32, true), splits, stream)
+                              : launch_split<MODE, GR_TILE_128>(out, p, maps, count_tiles(MODE, p, 128, 128, true), splits, stream);
         if (2 * count_tiles(MODE, p, 256, 256, false) <= pairs)
             return launch_var<MODE, GR_TILE_128>(out, p, maps, count_tiles(MODE, p, 128, 128, true), stream);
     }
     return launch_var<MODE, GR_TILE_256>(out, p, maps, count_tiles(MODE, p, 256, 256, true), stream);
 }
 
-__global__ void repack16_kernel(const uint16_t* __restrict__ src, long long ld_src, long long bs_src, uint16_t* __restrict__ dst,
-                                long long ld_dst, int inner, int rows, long long pieces) {
-    const long long idx = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
-    if (idx >= pieces) return;
-    const int per_row = static_cast<int>(ld_dst >> 3);
-    const int i = static_cast<int>(idx % per_row) * 8;
-    const long long row = idx / per_row;   // over all matrices
+__global__ void __launch_bounds__(256) repack16_kernel(const uint16_t* __restrict__ src, const uint16_t* end, long long ld_src, long long bs_src,
+                                                       uint16_t* __restrict__ dst, long long ld_dst, int inner, int rows, long long all_rows) {
+    // a warp takes 32 pieces of a row at a time
+    const int per_row = static_cast<int>(ld_dst >> 3), runs = (per_row + 31) / 32;
+    const long long idx = (blockIdx.x * 256ll + threadIdx.x) >> 5;
+    const long long row = idx / runs;   // over all matrices
+    const int i = (static_cast<int>(idx - row * runs) * 32 + (threadIdx.x & 31)) * 8;
+    if (row >= all_rows || i >= ld_dst) return;
     const uint16_t* s = src + (row / rows) * bs_src + (row % rows) * ld_src + i;
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint32_t lo = i + 2 * j < inner ? s[2 * j] : 0, hi = i + 2 * j + 1 < inner ? s[2 * j + 1] : 0;
-        w[j] = lo | (hi << 16);
-    }
-    *reinterpret_cast<uint4*>(dst + row * ld_dst + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(dst + row * ld_dst + i) = row16_load(s, inner - i, src, end);
 }
 
 }  // namespace
@@ -132,9 +130,11 @@ cudaError_t grouped_launch(int mode, int out, const GroupedParams& p, const Grou
 
 cudaError_t repack16_launch(const void* src, long long ld_src, long long bs_src, void* dst, long long ld_dst, int inner, int rows,
                             int matrices, cudaStream_t stream) {
-    const long long pieces = (ld_dst >> 3) * rows * matrices;
-    repack16_kernel<<<static_cast<unsigned>((pieces + 255) / 256), 256, 0, stream>>>(
-        static_cast<const uint16_t*>(src), ld_src, bs_src, static_cast<uint16_t*>(dst), ld_dst, inner, rows, pieces);
+    const long long all_rows = static_cast<long long>(rows) * matrices, runs = ((ld_dst >> 3) + 31) / 32;
+    const uint16_t* s = static_cast<const uint16_t*>(src);
+    const uint16_t* end = s + (matrices - 1) * bs_src + (rows - 1) * ld_src + inner;
+    repack16_kernel<<<static_cast<unsigned>((all_rows * runs + 7) / 8), 256, 0, stream>>>(s, end, ld_src, bs_src, static_cast<uint16_t*>(dst),
+                                                                                        ld_dst, inner, rows, all_rows);
     return cudaGetLastError();
 }
 

@@ -7,6 +7,7 @@
 #include "launch_util.cuh"
 #include "ptx.cuh"
 #include "q4.h"
+#include "row16.cuh"
 #include "umma_launch.h"
 
 namespace t2sp {
@@ -76,34 +77,11 @@ struct Q4Tile {
     static constexpr int kBytes = (TRANS ? kTile : kTile / 2) * kPitch;
 };
 
-// Eight elements of a row, zeros from the row's end on.
-__device__ __forceinline__ uint4 row_piece(const uint16_t* src, int left, bool aligned) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (aligned && left >= 8) {
-        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(src));
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < left) (&v.x)[j >> 1] |= static_cast<uint32_t>(src[j]) << (16 * (j & 1));
-    }
-    return v;
-}
-__device__ __forceinline__ void row_piece_out(uint16_t* dst, uint4 v, int left, bool aligned) {
-    if (aligned && left >= 8) {
-        *reinterpret_cast<uint4*>(dst) = v;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < left) dst[j] = static_cast<uint16_t>((&v.x)[j >> 1] >> (16 * (j & 1)));
-    }
-}
-
 // Rows of W between global memory and the tile. Outside the matrix the tile holds zeros. Each thread moves eight pieces of eight elements:
 // two at a time, of rows k and k + 1 (TRANS: n and n + 1).
 template <bool TRANS, bool STORE>
 __device__ __forceinline__ void tile_rows(const Q4Params& p, uint16_t* w, uint8_t* tile, int n0, int k0) {
     const int inner = TRANS ? p.K : p.N, outer = TRANS ? p.N : p.K, i0 = TRANS ? k0 : n0, o0 = TRANS ? n0 : k0;
-    const bool aligned = (reinterpret_cast<uintptr_t>(w) & 15) == 0 && p.ldw % 8 == 0;
     constexpr int kSteps = kTile / 2 * 16 / 256;
     const int pair = threadIdx.x >> 4, c = threadIdx.x & 15;      // pair of rows, piece of the row
     const int left = inner - i0 - c * 8;
@@ -115,7 +93,7 @@ __device__ __forceinline__ void tile_rows(const Q4Params& p, uint16_t* w, uint8_
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                v[s][h] = row_piece(at + s * next + h * p.ldw, o0 + 2 * pair + 32 * s + h < outer ? left : 0, aligned);
+                v[s][h] = row16_load(at + s * next + h * p.ldw, o0 + 2 * pair + 32 * s + h < outer ? left : 0, static_cast<const uint16_t*>(p.w), p.w_end);
     }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
@@ -142,7 +120,7 @@ __device__ __forceinline__ void tile_rows(const Q4Params& p, uint16_t* w, uint8_
         if constexpr (STORE) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                row_piece_out(at + s * next + h * p.ldw, v[s][h], o0 + 2 * pair + 32 * s + h < outer ? left : 0, aligned);
+                row16_store(at + s * next + h * p.ldw, v[s][h], o0 + 2 * pair + 32 * s + h < outer ? left : 0);
         }
     }
 }
@@ -518,7 +496,6 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
     }
 
     // ---------------------------------------------------------------- computing warps
-    const bool x_aligned = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldx % 8 == 0;
     const uint8_t* ring = smem_raw + lay.ring + group * depth * slot_bytes;
     uint64_t* full = bars + group * depth;
     uint64_t* freed = full + num_groups * depth;
@@ -565,13 +542,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
             if (i < total && k8 < pieces) {
                 const long long k = k8 * 8ll;
                 const uint16_t* src = static_cast<const uint16_t*>(p.x) + (rows[row] / p.per) * p.ldx + k;
-                if (x_aligned && k + 8 <= p.K) {
-                    v = *reinterpret_cast<const uint4*>(src);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (k + j < p.K) (&v.x)[j >> 1] |= uint32_t(src[j]) << (16 * (j & 1));
-                }
+                v = row16_load(src, static_cast<int>(min(8ll, p.K - k)), static_cast<const uint16_t*>(p.x), p.x_end);
             }
             return v;
         };

@@ -111,6 +111,7 @@ extern "C" int t2sp_b200_q4_pack(halide_buffer_t* W, halide_buffer_t* Q, halide_
     for (int i = 1; i < 3; ++i, ++vw.n)
         if (int e = rt_output_view(args[i].b, args[i].name, &vw.v[vw.n])) return e;
     p.w = vw.v[0].ptr;
+    p.w_end = static_cast<const uint16_t*>(p.w) + buf_elems_span(W);
     p.ldw = W->dim[1].stride; p.bs_w = W->dim[2].stride;
     p.trans_b = tb; p.group = group; p.bf16 = buf_type_word(W) == kBF16;
     p.q = static_cast<uint8_t*>(vw.v[1].ptr);
@@ -206,6 +207,7 @@ extern "C" int t2sp_b200_q4_gemv(halide_buffer_t* X, halide_buffer_t* Q, halide_
         if (int e = preload_output(Y, &vw.v[3])) return e;   // rows without a matrix keep their values
     }
     p.x = vw.v[0].ptr;
+    p.x_end = static_cast<const uint16_t*>(p.x) + buf_elems_span(X);
     p.ldx = X->dim[1].stride;
     p.q = static_cast<uint8_t*>(vw.v[1].ptr);
     p.s = static_cast<uint16_t*>(vw.v[2].ptr);

@@ -22,6 +22,7 @@ __host__ __device__ __forceinline__ int q4_groups(int K, int group) { return (q4
 struct Q4Params {
     const void* w;        // pack: the 16-bit matrices; unpack: where they go (wout)
     void* wout;
+    const uint16_t* w_end; // behind the last element of w
     long long ldw, bs_w;  // elements between rows (k rows of n, or n rows of k with trans_b) and between matrices
     int trans_b;
     uint8_t* q;
@@ -30,6 +31,7 @@ struct Q4Params {
     int bf16;
     // products
     const void* x;        // T x K
+    const uint16_t* x_end;
     long long ldx;
     const int* index;     // R matrix numbers or null
     void* y;              // R x N

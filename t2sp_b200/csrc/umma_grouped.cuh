@@ -28,10 +28,10 @@ template <int MODE, int VAR>
 struct GroupedCfg {
     static constexpr bool kGrad = MODE == GR_GRAD;
     static constexpr bool kPMn = MODE != GR_FWD_K;           // the MMA's A operand (n) is MN-major
-    static constexpr int kPair = VAR == GR_TILE_128 ? 1 : 2; // CTAs of a tile
+    static constexpr int kPair = VAR == GR_TILE_128 || VAR == GR_TILE_32 ? 1 : 2;  // CTAs of a tile
     static constexpr int kSub = VAR == GR_TILE_512 ? 2 : 1;  // sub-tiles of a CTA
     static constexpr int kTileN = 128 * kPair * kSub;
-    static constexpr int kTileC = 128 * kPair;
+    static constexpr int kTileC = VAR == GR_TILE_32 ? 32 : 128 * kPair;
     // columns come in steps that both CTAs' parts can take: 16 rows of a K-major operand, 64 (a swizzle atom) of an MN-major one
     static constexpr int kColStep = (kGrad ? 64 : 16) * kPair;
     static constexpr int kAccs = 2;                           // accumulators of kTileC columns: two tiles in turn, or the two sub-tiles
@@ -529,12 +529,15 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
 // Forward products of a few rows, or with a few columns, have fewer 128 x 128 tiles than the GPU has SMs, and one SM brings weights at 60 to 80 GB/s
 // only. Here a cluster of `splits` CTAs shares a tile: each adds up its run of k-blocks, hands the fp32 sums of 32 n x 32 columns to the CTA that owns
 // them through distributed shared memory, and the owners add the parts in the order of the ranks and write the results. (8 groups of
-// 2 rows, 1024 x 1024, 64 tiles: two CTAs a tile.)
+// 2 rows, 1024 x 1024, 64 tiles: two CTAs a tile.) Tiles of 32 columns for groups of a few rows leave room for twice the blocks in flight.
+template <int VAR>
 struct SplitCfg {
-    static constexpr int kStages = 4;
-    static constexpr int kStageBytes = 2 * 128 * 128;
+    static constexpr int kTileC = VAR == GR_TILE_32 ? 32 : 128;
+    static constexpr int kStages = VAR == GR_TILE_32 ? 8 : 4;
+    static constexpr int kQBytes = kTileC * 128;
+    static constexpr int kStageBytes = 128 * 128 + kQBytes;
     static constexpr int kUnitBytes = 32 * 32 * 4;           // sums of 32 n x 32 columns
-    static constexpr int kPartBytes = 16 * kUnitBytes;       // an owner's units times the ranks: 16 units in a tile
+    static constexpr int kPartBytes = (VAR == GR_TILE_32 ? 8 : 16) * kUnitBytes;   // an owner's units times the ranks: 4 or 16 units in a tile, 8 ranks
     static constexpr int kThreads = (2 + 8) * 32;
     static constexpr int kTmemCols = 128;
     static constexpr int kTableBytes = 2 * (kMaxGroups + 4) * 4;
@@ -542,14 +545,15 @@ struct SplitCfg {
     static_assert(kSmemBytes <= 232448, "shared memory budget exceeded");
 };
 
-template <int MODE, class O>
-__global__ void __launch_bounds__(SplitCfg::kThreads, 1)
+template <int MODE, int VAR, class O>
+__global__ void __launch_bounds__(SplitCfg<VAR>::kThreads, 1)
 grouped_split_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ GroupedMaps maps, int splits) {
-    constexpr int STAGES = SplitCfg::kStages;
+    using SplitC = SplitCfg<VAR>;
+    constexpr int STAGES = SplitC::kStages;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float* parts = reinterpret_cast<float*>(smem + STAGES * SplitCfg::kStageBytes);   // [unit of this owner][rank][column][n]
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * SplitCfg::kStageBytes + SplitCfg::kPartBytes);
+    float* parts = reinterpret_cast<float*>(smem + STAGES * SplitC::kStageBytes);   // [unit of this owner][rank][column][n]
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * SplitC::kStageBytes + SplitC::kPartBytes);
     uint64_t* empty_bar = full_bar + STAGES;
     uint64_t* tfull_bar = empty_bar + STAGES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull_bar + 1);
@@ -573,12 +577,12 @@ grouped_split_kernel(const __grid_constant__ GroupedParams p, const __grid_const
         ptx::fence_mbar_init();
     }
     if (warp == 1) {
-        ptx::tmem_alloc<1>(tmem_slot, SplitCfg::kTmemCols);
+        ptx::tmem_alloc<1>(tmem_slot, SplitC::kTmemCols);
         ptx::tmem_relinquish<1>();
     }
     ptx::grid_dep_launch();
     ptx::grid_dep_wait();
-    const bool valid = grouped_tables<MODE, GR_TILE_128>(p, off, first);
+    const bool valid = grouped_tables<MODE, VAR>(p, off, first);
     ptx::tc_fence_before_sync();
     __syncthreads();
     ptx::cluster_sync();   // every CTA of the cluster runs before its shared memory is written
@@ -586,14 +590,14 @@ grouped_split_kernel(const __grid_constant__ GroupedParams p, const __grid_const
     const uint32_t tmem_base = *tmem_slot;
     if (!valid) {
         if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(p.status, ST_BAD_OFFSETS);
-        if (warp == 1) ptx::tmem_dealloc<1>(tmem_base, SplitCfg::kTmemCols);
+        if (warp == 1) ptx::tmem_dealloc<1>(tmem_base, SplitC::kTmemCols);
         return;
     }
 
     int e = 0, it = 0;
     uint32_t phase = 0;   // of the accumulator's barrier: it completes once for every tile with k-blocks
     GroupedTile g;
-    for (int t = worker; grouped_tile<MODE, GR_TILE_128>(p, off, first, t, e, g); t += num_workers) {
+    for (int t = worker; grouped_tile<MODE, VAR>(p, off, first, t, e, g); t += num_workers) {
         const int kb0 = rank * g.num_kb / splits, nkb = (rank + 1) * g.num_kb / splits - kb0;   // this CTA's run, possibly empty
         if (warp == 0) {
             // -------------------------------------------------------- TMA producer
@@ -601,7 +605,7 @@ grouped_split_kernel(const __grid_constant__ GroupedParams p, const __grid_const
                 for (int i = 0; i < nkb; ++i) {
                     const int s = (it + i) % STAGES, kb = kb0 + i;
                     if (!bounded_wait(&empty_bar[s], (((it + i) / STAGES) & 1) ^ 1, ab, ST_TIMEOUT_PRODUCER)) break;
-                    uint8_t* sp = smem + s * SplitCfg::kStageBytes;
+                    uint8_t* sp = smem + s * SplitC::kStageBytes;
                     uint8_t* sq = sp + 128 * 128;
                     ptx::mbar_expect_tx(&full_bar[s], 128 * 128 + g.ncols * 128);
                     if constexpr (MODE == GR_FWD_MN) {
@@ -630,7 +634,7 @@ grouped_split_kernel(const __grid_constant__ GroupedParams p, const __grid_const
                     ok = bounded_wait(&full_bar[s], ((it + i) / STAGES) & 1, ab, ST_TIMEOUT_MMA);
                     if (!ok) break;
                     ptx::tc_fence_after_sync();
-                    const uint32_t sp = ptx::smem_u32(smem + s * SplitCfg::kStageBytes);
+                    const uint32_t sp = ptx::smem_u32(smem + s * SplitC::kStageBytes);
                     const uint64_t dp = ptx::make_smem_desc(sp, MODE == GR_FWD_MN ? 8192 : 16, 1024);
                     const uint64_t dq = ptx::make_smem_desc(sp + 128 * 128, 16, 1024);
 #pragma unroll
@@ -687,13 +691,15 @@ grouped_split_kernel(const __grid_constant__ GroupedParams p, const __grid_const
                 }
             }
         }
-        __syncwarp();
-        ptx::cluster_sync();   // the parts have been read: the next tile may overwrite them
+        if (t + num_workers < first[p.E]) {   // the parts have been read: the next tile may overwrite them
+            __syncwarp();
+            ptx::cluster_sync();
+        }
     }
 
     __syncthreads();
     if (*abort_slot) __nanosleep(200000);
-    if (warp == 1) ptx::tmem_dealloc<1>(tmem_base, SplitCfg::kTmemCols);
+    if (warp == 1) ptx::tmem_dealloc<1>(tmem_base, SplitC::kTmemCols);
 }
 
 }  // namespace t2sp
