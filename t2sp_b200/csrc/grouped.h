@@ -24,7 +24,6 @@ struct GroupedParams {
     long long ldc, bs_c;   // row pitch of C or G, stride between the matrices of G
     int rows, E, K, N;
     int bf16;              // element type of the inputs: 1 bf16, 0 f16
-    int wide_out;          // 16-bit results: rows of C and G start on 16 bytes and N is a multiple of 8
     long long wait_cycles; // limit of every mbarrier wait in SM cycles, 0: kWaitTimeoutCycles
     unsigned* status;
 };
@@ -36,8 +35,15 @@ struct GroupedMaps {
 
 cudaError_t grouped_launch(int mode, int out, const GroupedParams& p, const GroupedMaps& maps, cudaStream_t stream);
 
-// dst[m][r][i] (row pitch ld_dst, dense matrices) = src[m * bs_src + r * ld_src + i], 16-bit elements; ld_dst is a multiple of 8.
-cudaError_t repack16_launch(const void* src, long long ld_src, long long bs_src, void* dst, long long ld_dst, int inner, int rows,
-                            int matrices, cudaStream_t stream);
+// dst[m][r][i] (row pitch ld_dst, dense matrices) = src[m * bs_src + r * ld_src + i], 16-bit elements; ld_dst is a multiple of 8. Up to
+// two operands in one launch.
+struct Repack {
+    const uint16_t* src;
+    uint16_t* dst;
+    long long ld_src, bs_src, ld_dst;
+    int inner, rows, matrices;
+    unsigned blocks;       // set by the launcher
+};
+cudaError_t repack16_launch(Repack* jobs, int count, cudaStream_t stream);
 
 }  // namespace t2sp

@@ -108,16 +108,18 @@ cudaError_t launch_mode(int out, const GroupedParams& p, const GroupedMaps& maps
     return launch_var<MODE, GR_TILE_256>(out, p, maps, count_tiles(MODE, p, 256, 256, true), stream);
 }
 
-__global__ void __launch_bounds__(256) repack16_kernel(const uint16_t* __restrict__ src, const uint16_t* end, long long ld_src, long long bs_src,
-                                                       uint16_t* __restrict__ dst, long long ld_dst, int inner, int rows, long long all_rows) {
+__global__ void __launch_bounds__(256) repack16_kernel(const Repack a, const Repack b) {
+    const bool second = blockIdx.x >= a.blocks;
+    const Repack& j = second ? b : a;
     // a warp takes 32 pieces of a row at a time
-    const int per_row = static_cast<int>(ld_dst >> 3), runs = (per_row + 31) / 32;
-    const long long idx = (blockIdx.x * 256ll + threadIdx.x) >> 5;
+    const int per_row = static_cast<int>(j.ld_dst >> 3), runs = (per_row + 31) / 32;
+    const long long idx = ((blockIdx.x - (second ? a.blocks : 0)) * 256ll + threadIdx.x) >> 5;
     const long long row = idx / runs;   // over all matrices
     const int i = (static_cast<int>(idx - row * runs) * 32 + (threadIdx.x & 31)) * 8;
-    if (row >= all_rows || i >= ld_dst) return;
-    const uint16_t* s = src + (row / rows) * bs_src + (row % rows) * ld_src + i;
-    *reinterpret_cast<uint4*>(dst + row * ld_dst + i) = row16_load(s, inner - i, src, end);
+    if (row >= static_cast<long long>(j.rows) * j.matrices || i >= j.ld_dst) return;
+    const uint16_t* s = j.src + (row / j.rows) * j.bs_src + (row % j.rows) * j.ld_src + i;
+    const uint16_t* end = j.src + (j.matrices - 1) * j.bs_src + (j.rows - 1) * j.ld_src + j.inner;
+    *reinterpret_cast<uint4*>(j.dst + row * j.ld_dst + i) = row16_load(s, j.inner - i, j.src, end);
 }
 
 }  // namespace
@@ -128,13 +130,14 @@ cudaError_t grouped_launch(int mode, int out, const GroupedParams& p, const Grou
     return launch_mode<GR_GRAD>(out, p, maps, stream);
 }
 
-cudaError_t repack16_launch(const void* src, long long ld_src, long long bs_src, void* dst, long long ld_dst, int inner, int rows,
-                            int matrices, cudaStream_t stream) {
-    const long long all_rows = static_cast<long long>(rows) * matrices, runs = ((ld_dst >> 3) + 31) / 32;
-    const uint16_t* s = static_cast<const uint16_t*>(src);
-    const uint16_t* end = s + (matrices - 1) * bs_src + (rows - 1) * ld_src + inner;
-    repack16_kernel<<<static_cast<unsigned>((all_rows * runs + 7) / 8), 256, 0, stream>>>(s, end, ld_src, bs_src, static_cast<uint16_t*>(dst),
-                                                                                        ld_dst, inner, rows, all_rows);
+cudaError_t repack16_launch(Repack* jobs, int count, cudaStream_t stream) {
+    unsigned blocks = 0;
+    for (int n = 0; n < count; ++n) {
+        const long long runs = ((jobs[n].ld_dst >> 3) + 31) / 32;
+        jobs[n].blocks = static_cast<unsigned>((static_cast<long long>(jobs[n].rows) * jobs[n].matrices * runs + 7) / 8);
+        blocks += jobs[n].blocks;
+    }
+    repack16_kernel<<<blocks, 256, 0, stream>>>(jobs[0], jobs[count - 1]);
     return cudaGetLastError();
 }
 

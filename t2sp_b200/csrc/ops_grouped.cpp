@@ -25,21 +25,27 @@ struct Operand {
     }
 };
 
-// Copies an operand that TMA cannot read in place into scratch memory with padded rows.
-int fit_operand(Views& vw, Operand& o) {
-    if (o.inner == 0 || o.rows == 0 || o.matrices == 0 || o.fits()) return 0;
-    const int64_t ld = (int64_t(o.inner) + 7) / 8 * 8;
-    void* q = rt_alloc(size_t(ld) * o.rows * o.matrices * 2);
-    if (!q) return halide_error_code_device_malloc_failed;
-    vw.v[vw.n].ptr = q; vw.v[vw.n].borrowed = false; vw.n++;
-    if (repack16_launch(o.ptr, o.ld, o.bs, q, ld, o.inner, o.rows, o.matrices, rt_stream()) != cudaSuccess) {
+// Copies operands that TMA cannot read in place into scratch memory with padded rows.
+int fit_operands(Views& vw, Operand& a, Operand& b) {
+    Repack jobs[2];
+    int count = 0;
+    for (Operand* o : {&a, &b}) {
+        if (o->fits()) continue;
+        const int64_t ld = (int64_t(o->inner) + 7) / 8 * 8;
+        void* q = rt_alloc(size_t(ld) * o->rows * o->matrices * 2);
+        if (!q) return halide_error_code_device_malloc_failed;
+        vw.v[vw.n].ptr = q; vw.v[vw.n].borrowed = false; vw.n++;
+        jobs[count++] = {reinterpret_cast<const uint16_t*>(o->ptr), static_cast<uint16_t*>(q), o->ld, o->bs, ld, o->inner, o->rows, o->matrices, 0};
+        o->ptr = static_cast<char*>(q);
+        o->ld = ld;
+        o->bs = ld * o->rows;
+    }
+    if (count == 0) return 0;
+    if (repack16_launch(jobs, count, rt_stream()) != cudaSuccess) {
         cudaGetLastError();
         return halide_error_code_device_run_failed;
     }
     rt_count_launch(1);
-    o.ptr = static_cast<char*>(q);
-    o.ld = ld;
-    o.bs = ld * o.rows;
     return 0;
 }
 
@@ -62,13 +68,11 @@ int run_grouped(const char* who, int mode, uint32_t type, uint32_t out, GroupedP
     p.status = rt_status_word();
     p.wait_cycles = rt_env().wait_cycles;
     p.bf16 = type == kBF16;
-    p.wide_out = out != kF32 && !(reinterpret_cast<uintptr_t>(p.c) & 15) && p.ldc % 8 == 0 && p.bs_c % 8 == 0 && p.N % 8 == 0;
     if (sync_after) cudaEventRecord(rt_event(0), s);
     GroupedMaps maps;
     memset(&maps, 0, sizeof(maps));
     if (p.K > 0 && p.rows > 0) {   // else nothing is read
-        if (int e = fit_operand(vw, p_op)) return e;
-        if (int e = fit_operand(vw, q_op)) return e;
+        if (int e = fit_operands(vw, p_op, q_op)) return e;
         bool ok = encode(&maps.p, type, p_op, 3, 64, mode == GR_FWD_K ? 128 : 64) &&
                   encode(&maps.q[0], type, q_op, 2, 64, mode == GR_GRAD ? 64 : 128);
         if (mode != GR_GRAD)

@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "grouped.h"
+#include "row16.cuh"
 #include "umma_core.cuh"
 
 namespace t2sp {
@@ -191,22 +192,15 @@ __device__ __forceinline__ void grouped_put(uint32_t taddr, bool zero, uint8_t* 
     for (int i = 0; i < 4; ++i) {
         const int col = 16 * half + 4 * i + (lane >> 3);
         const uint4 v = *reinterpret_cast<const uint4*>(tile + col * 128 + ((piece ^ (col & 7)) << 4));
-        if (col < cols && piece * 8 < n_left) *reinterpret_cast<uint4*>(dst + col * ld + piece * 8) = v;
+        if (col < cols && piece * 8 < n_left) row16_store(reinterpret_cast<uint16_t*>(dst + col * ld + piece * 8), v, n_left - piece * 8);
     }
 }
 
-// Writes 32 columns of the accumulator: lane = n, one output row (or k) for each column. Each store instruction writes 32
-// consecutive n. For fp32 results, and for places that take no 16-byte stores.
-template <class O>
-__device__ __forceinline__ void grouped_store(O* dst, long long ld, int cols, const uint32_t (&r)[32]) {
+// Writes 32 columns of fp32 results: lane = n, one output row (or k) for each column. Each store instruction writes 32 consecutive n.
+__device__ __forceinline__ void grouped_store(float* dst, long long ld, int cols, const uint32_t (&r)[32]) {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-        if (j < cols) {
-            const float v = __uint_as_float(r[j]);
-            if constexpr (sizeof(O) == 4) dst[j * ld] = v;
-            else if constexpr (std::is_same<O, __half>::value) dst[j * ld] = __float2half_rn(v);
-            else dst[j * ld] = __float2bfloat16_rn(v);
-        }
+        if (j < cols) dst[j * ld] = __uint_as_float(r[j]);
 }
 
 template <int MODE, int VAR, class O>
@@ -484,21 +478,19 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
                     for (int c = turn * 32; c < g.cols; c += 64) {
                         const uint32_t taddr = lane_base + acc * Cfg::kTileC + c;
                         if constexpr (sizeof(O) == 2) {
-                            if (p.wide_out) {
-                                grouped_put(taddr, g.num_kb == 0, out_tile, dst + (n64 - n) + c * p.ldc, p.ldc, p.N - n64, g.cols - c, lane, q & 1,
-                                            1 + turn * 2 + (q >> 1));
-                                continue;
-                            }
-                        }
-                        uint32_t r[32];
-                        if (g.num_kb) {
-                            ptx::tmem_ld_32x32(taddr, r);
-                            ptx::tmem_ld_wait();
+                            grouped_put(taddr, g.num_kb == 0, out_tile, dst + (n64 - n) + c * p.ldc, p.ldc, p.N - n64, g.cols - c, lane, q & 1,
+                                        1 + turn * 2 + (q >> 1));
                         } else {
+                            uint32_t r[32];
+                            if (g.num_kb) {
+                                ptx::tmem_ld_32x32(taddr, r);
+                                ptx::tmem_ld_wait();
+                            } else {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) r[j] = 0u;
+                                for (int j = 0; j < 32; ++j) r[j] = 0u;
+                            }
+                            if (n + lane < p.N) grouped_store(dst + c * p.ldc + lane, p.ldc, g.cols - c, r);
                         }
-                        if (n + lane < p.N) grouped_store(dst + c * p.ldc + lane, p.ldc, g.cols - c, r);
                     }
                 }
                 if (g.num_kb) {
