@@ -36,7 +36,8 @@ template <int MODE, int VAR>
 cudaError_t launch_var(int out, const GroupedParams& p, const GroupedMaps& maps, long long tiles, cudaStream_t stream) {
     const long long slots = core_sm_count() / GroupedCfg<MODE, VAR>::kPair;
     const int workers = static_cast<int>(tiles < slots ? (tiles > 0 ? tiles : 1) : slots);
-    if (out == GR_OUT_F32) return launch_typed<MODE, VAR, float>(p, maps, workers, stream);
+    if constexpr (VAR != GR_TILE_512)
+        if (out == GR_OUT_F32) return launch_typed<MODE, VAR, float>(p, maps, workers, stream);
     if (out == GR_OUT_BF16) return launch_typed<MODE, VAR, __nv_bfloat16>(p, maps, workers, stream);
     return launch_typed<MODE, VAR, __half>(p, maps, workers, stream);
 }
@@ -93,13 +94,14 @@ cudaError_t launch_mode(int out, const GroupedParams& p, const GroupedMaps& maps
     const long long rounds256 = (count_tiles(MODE, p, 256, 256, false) + pairs - 1) / pairs;
     const long long rounds512 = (count_tiles(MODE, p, 512, 256, false) + pairs - 1) / pairs;
     const int kb = MODE == GR_GRAD ? p.rows / (p.E * 64) : (p.K + 63) / 64;
-    if (kb >= (MODE == GR_GRAD ? 12 : 32) && 200 * rounds512 <= 108 * rounds256)
+    if (out != GR_OUT_F32 && kb >= (MODE == GR_GRAD ? 12 : 32) && 200 * rounds512 <= 108 * rounds256)
         return launch_var<MODE, GR_TILE_512>(out, p, maps, count_tiles(MODE, p, 512, 256, true), stream);
     if constexpr (MODE != GR_GRAD) {
         const long long t128 = count_tiles(MODE, p, 128, 128, false);
         const bool narrow = p.rows <= 32ll * p.E;   // about a tile of 32 columns to a group
         for (int splits = 8; splits >= 2; splits /= 2)
-            if (t128 * splits <= core_sm_count() - (splits == 8 ? 20 : 4) && kb >= 2 * splits)   // clusters do not fill every GPC
+            if (t128 * splits <= core_sm_count() - (splits == 8 ? 20 : 4) && kb >= 2 * splits &&   // clusters do not fill every GPC
+                (out != GR_OUT_F32 || kb <= 8 * splits))                                             // kRun of the other kernel
                 return narrow ? launch_split<MODE, GR_TILE_32>(out, p, maps, count_tiles(MODE, p, 128, 32, true), splits, stream)
                               : launch_split<MODE, GR_TILE_128>(out, p, maps, count_tiles(MODE, p, 128, 128, true), splits, stream);
         if (2 * count_tiles(MODE, p, 256, 256, false) <= pairs)

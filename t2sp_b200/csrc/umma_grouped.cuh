@@ -197,10 +197,10 @@ __device__ __forceinline__ void grouped_put(uint32_t taddr, bool zero, uint8_t* 
 }
 
 // Writes 32 columns of fp32 results: lane = n, one output row (or k) for each column. Each store instruction writes 32 consecutive n.
-__device__ __forceinline__ void grouped_store(float* dst, long long ld, int cols, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void grouped_store(float* dst, long long ld, int cols, const float (&r)[32]) {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-        if (j < cols) dst[j * ld] = __uint_as_float(r[j]);
+        if (j < cols) dst[j * ld] = r[j];
 }
 
 template <int MODE, int VAR, class O>
@@ -208,6 +208,11 @@ __global__ void __launch_bounds__(GroupedCfg<MODE, VAR>::kThreads, 1)
 grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ GroupedMaps maps) {
     using Cfg = GroupedCfg<MODE, VAR>;
     constexpr int STAGES = Cfg::kStages, kPair = Cfg::kPair, kSub = Cfg::kSub;
+    // k-blocks that are added up in tensor memory before the epilogue takes them. The tensor core cuts its sums off rather than rounding them, about
+    // 4e-9 of the result a step of 16 k: nothing to a 16-bit result, but 8e-5 of an fp32 gradient over 65536 rows. For fp32 results
+    // the epilogue adds runs of 32 such steps in registers, rounding to nearest (5e-7 at every length).
+    constexpr int kRun = sizeof(O) == 4 ? 8 : 1 << 30;
+    static_assert(sizeof(O) == 2 || kSub == 1, "runs need an accumulator to go on with");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* out_tiles = smem + STAGES * Cfg::kStageBytes;
@@ -379,16 +384,18 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
                 if (g.num_kb == 0) continue;   // nothing to add up: the epilogue writes zeros
                 idesc = make_instr_desc(1, p.bf16 ? 1 : 0, Cfg::kPMn, Cfg::kGrad, 128 * kPair, g.ncols);
                 if constexpr (kSub == 1) {
-                    const int acc = lt & 1;
-                    ok = bounded_wait(&tempty_bar[acc], ((lt >> 1) & 1) ^ 1, ab, ST_TIMEOUT_MMA);
-                    ptx::tc_fence_after_sync();
-                    for (int kb = 0; kb < g.num_kb && ok; ++kb) {
-                        ok = wait_block(it + kb, kb);
-                        if (!ok) break;
-                        issue(tmem_base + acc * Cfg::kTileC, 0, kb, it + kb);
-                        commit_all(&empty_bar[(it + kb) % STAGES]);
+                    for (int kb0 = 0; kb0 < g.num_kb && ok; kb0 += kRun, ++lt) {
+                        const int acc = lt & 1, kb1 = min(g.num_kb, kb0 + kRun);
+                        ok = bounded_wait(&tempty_bar[acc], ((lt >> 1) & 1) ^ 1, ab, ST_TIMEOUT_MMA);
+                        ptx::tc_fence_after_sync();
+                        for (int kb = kb0; kb < kb1 && ok; ++kb) {
+                            ok = wait_block(it + kb, kb);
+                            if (!ok) break;
+                            issue(tmem_base + acc * Cfg::kTileC, 0, kb - kb0, it + kb);
+                            commit_all(&empty_bar[(it + kb) % STAGES]);
+                        }
+                        if (ok) commit_all(&tfull_bar[acc]);
                     }
-                    if (ok) commit_all(&tfull_bar[acc]);
                 } else {
                     // Both accumulators belong to this tile. Sub-tile 0 runs `lead` k-blocks ahead of sub-tile 1 at both ends of the tile, so that
                     // its MMAs begin while accumulator 1 is still drained, and its own drain runs under sub-tile 1's last MMAs.
@@ -427,9 +434,9 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
                         commit_all(&empty_bar[(it + kb) % STAGES]);
                     }
                     commit_all(&tfull_bar[1]);
+                    ++lt;
                 }
                 it += g.num_kb;
-                ++lt;
             }
         }
     } else if (Cfg::kGrad && warp == 2 + Cfg::kEpiWarps) {
@@ -462,38 +469,26 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
         bool ok = true;
         GroupedTile g;
         for (int t = worker; ok && grouped_tile<MODE, VAR>(p, off, first, t, e, g); t += num_workers) {
-#pragma unroll 1
-            for (int u = 0; u < kSub; ++u) {
-                const int acc = kSub == 2 ? u : lt & 1;
-                const uint32_t parity = kSub == 2 ? lt & 1 : (lt >> 1) & 1;
-                const int n = g.n0 + u * 256 + rank * 128 + q * 32;
-                O* dst = static_cast<O*>(p.c) + (MODE == GR_GRAD ? g.e * p.bs_c : 0) + g.c0 * p.ldc + n;
-                if (g.num_kb) {
-                    if (!bounded_wait_warp(&tfull_bar[acc], parity, ab, ST_TIMEOUT_EPILOGUE, lane)) { ok = false; break; }
-                    ptx::tc_fence_after_sync();
-                }
-                const int n64 = n & ~63;   // of the two warps that write together
-                if (n64 < p.N) {
-#pragma unroll 1
-                    for (int c = turn * 32; c < g.cols; c += 64) {
-                        const uint32_t taddr = lane_base + acc * Cfg::kTileC + c;
-                        if constexpr (sizeof(O) == 2) {
-                            grouped_put(taddr, g.num_kb == 0, out_tile, dst + (n64 - n) + c * p.ldc, p.ldc, p.N - n64, g.cols - c, lane, q & 1,
-                                        1 + turn * 2 + (q >> 1));
-                        } else {
-                            uint32_t r[32];
-                            if (g.num_kb) {
-                                ptx::tmem_ld_32x32(taddr, r);
-                                ptx::tmem_ld_wait();
-                            } else {
+            if constexpr (sizeof(O) == 4) {
+                constexpr int kPieces = Cfg::kTileC / 64;   // of 32 columns for each warp
+                float sums[kPieces][32];
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) r[j] = 0u;
-                            }
-                            if (n + lane < p.N) grouped_store(dst + c * p.ldc + lane, p.ldc, g.cols - c, r);
-                        }
+                for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) sums[i][j] = 0.f;
+                for (int kb = 0; kb < g.num_kb && ok; kb += kRun, ++lt) {
+                    const int acc = lt & 1;
+                    ok = bounded_wait_warp(&tfull_bar[acc], (lt >> 1) & 1, ab, ST_TIMEOUT_EPILOGUE, lane);
+                    if (!ok) break;
+                    ptx::tc_fence_after_sync();
+#pragma unroll
+                    for (int i = 0; i < kPieces; ++i) {
+                        uint32_t r[32];
+                        ptx::tmem_ld_32x32(lane_base + acc * Cfg::kTileC + turn * 32 + i * 64, r);
+                        ptx::tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sums[i][j] += __uint_as_float(r[j]);
                     }
-                }
-                if (g.num_kb) {
                     ptx::tc_fence_before_sync();
                     __syncwarp();
                     if (lane == 0) {
@@ -501,8 +496,45 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
                         else ptx::mbar_arrive(&tempty_bar[acc]);
                     }
                 }
+                const int n = g.n0 + rank * 128 + q * 32 + lane;
+                float* dst = static_cast<float*>(p.c) + (MODE == GR_GRAD ? g.e * p.bs_c : 0) + g.c0 * p.ldc + n;
+                if (ok && n < p.N)
+#pragma unroll
+                    for (int i = 0; i < kPieces; ++i) {
+                        const int c = turn * 32 + i * 64;
+                        grouped_store(dst + c * p.ldc, p.ldc, g.cols - c, sums[i]);
+                    }
+            } else {
+#pragma unroll 1
+                for (int u = 0; u < kSub; ++u) {
+                    const int acc = kSub == 2 ? u : lt & 1;
+                    const uint32_t parity = kSub == 2 ? lt & 1 : (lt >> 1) & 1;
+                    const int n = g.n0 + u * 256 + rank * 128 + q * 32;
+                    O* dst = static_cast<O*>(p.c) + (MODE == GR_GRAD ? g.e * p.bs_c : 0) + g.c0 * p.ldc + n;
+                    if (g.num_kb) {
+                        if (!bounded_wait_warp(&tfull_bar[acc], parity, ab, ST_TIMEOUT_EPILOGUE, lane)) { ok = false; break; }
+                        ptx::tc_fence_after_sync();
+                    }
+                    const int n64 = n & ~63;   // of the two warps that write together
+                    if (n64 < p.N) {
+#pragma unroll 1
+                        for (int c = turn * 32; c < g.cols; c += 64) {
+                            const uint32_t taddr = lane_base + acc * Cfg::kTileC + c;
+                            grouped_put(taddr, g.num_kb == 0, out_tile, dst + (n64 - n) + c * p.ldc, p.ldc, p.N - n64, g.cols - c, lane, q & 1,
+                                        1 + turn * 2 + (q >> 1));
+                        }
+                    }
+                    if (g.num_kb) {
+                        ptx::tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if constexpr (kPair == 2) ptx::mbar_arrive_peer(&tempty_bar[acc], 0);
+                            else ptx::mbar_arrive(&tempty_bar[acc]);
+                        }
+                    }
+                }
+                if (g.num_kb) ++lt;
             }
-            if (g.num_kb) ++lt;
         }
     }
 

@@ -338,3 +338,46 @@ def test_repeatable(lib):
             assert t2sp_b200.grouped_gemm_grad(buf(a), buf(d), buf(off), buf(g)) == 0
         outs.append((c, g))
     assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+def test_long_fp32_gradient(lib):
+    """An fp32 gradient over many rows is added up in runs of 512. With values of random sign (deviation s for a product) a run's
+    partial sums have about 12 s on the mean; 32 steps that cut off 2^-24 of them on the mean give 2.3e-5 s a run, over 79 runs in
+    quadrature 2e-4 s, of a result of 200 s: 1e-6 relative in the 2-norm, 5e-6 with room. One sum over all rows would be 5e-5 off."""
+    import torch
+    a, _, d, off = make(1, 256, 256, [40000], torch.bfloat16)
+    g = torch.empty(1, 256, 256, dtype=torch.float32, device="cuda")
+    with on_stream():
+        assert t2sp_b200.grouped_gemm_grad(buf(a), buf(d), buf(off), buf(g)) == 0
+    ref = a.double().T @ d.double()
+    assert float((g[0].double() - ref).norm() / ref.norm()) <= 5e-6
+
+
+def test_two_threads_on_their_own_streams(lib):
+    """Two host threads call at once, each on its own stream, one of them with operands that need scratch memory."""
+    import threading
+
+    import torch
+    made = [make(3, 64 + 5 * i, 128, [100, 0, 57], torch.bfloat16, seed=i) for i in range(2)]
+    outs = [torch.zeros(157, 128, dtype=torch.bfloat16, device="cuda") for _ in made]
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(i):
+        try:
+            a, b, _, off = made[i]
+            stream = torch.cuda.Stream()
+            with on_stream(stream, asynchronous=True) as L:
+                for _ in range(50):
+                    assert t2sp_b200.grouped_gemm(buf(a), buf(b), buf(off), buf(outs[i])) == 0
+                assert L.t2sp_b200_sync() == 0
+        except BaseException as e:   # reported by the main thread
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for (a, b, _, off), c in zip(made, outs):
+        check_forward(a, b, off, c, False, c)
