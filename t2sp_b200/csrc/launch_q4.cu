@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
         // x in pieces of 8 k, a warp's 32 pieces of one row at a time; the first ones stay in registers between the two looks at them
         const int pieces = kblocks * 8, runs = (pieces + 31) / 32, total = count * runs;
         constexpr int kLanes = G / 8;                                   // lanes that hold a group
-        constexpr int kKeep = 4;
+        constexpr int kKeep = INT ? 4 : 8;
         auto piece = [&](int i) -> uint4 {
             const int row = i / runs, k8 = (i - row * runs) * 32 + lane;
             uint4 v = make_uint4(0, 0, 0, 0);
@@ -549,6 +549,17 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
         uint4 kept[kKeep];
 #pragma unroll
         for (int n = 0; n < kKeep; ++n) kept[n] = piece(warp + n * kGemvWarps);
+        // the others, as many at a time: the loads of a batch are on their way together
+        auto rest = [&](auto f) {
+            for (int i = warp + kKeep * kGemvWarps; i < total; i += kKeep * kGemvWarps) {
+                uint4 v[kKeep];
+#pragma unroll
+                for (int n = 0; n < kKeep; ++n) v[n] = piece(i + n * kGemvWarps);
+#pragma unroll
+                for (int n = 0; n < kKeep; ++n)
+                    if (i + n * kGemvWarps < total) f(i + n * kGemvWarps, v[n]);
+            }
+        };
         if constexpr (INT) {
             auto look = [&](int i, const uint4& v) {
                 uint32_t m = max_abs2<T>(max_abs2<T>(max_abs2<T>(max_abs2<T>(0u, v.x), v.y), v.z), v.w);
@@ -559,7 +570,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
 #pragma unroll
             for (int n = 0; n < kKeep; ++n)
                 if (warp + n * kGemvWarps < total) look(warp + n * kGemvWarps, kept[n]);
-            for (int i = warp + kKeep * kGemvWarps; i < total; i += kGemvWarps) look(i, piece(i));
+            rest(look);
             ptx::bar_sync(15, kGemvWarps * 32);
         }
         auto place = [&](int i, const uint4& v) {
@@ -611,7 +622,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
 #pragma unroll
         for (int n = 0; n < kKeep; ++n)
             if (warp + n * kGemvWarps < total) place(warp + n * kGemvWarps, kept[n]);
-        for (int i = warp + kKeep * kGemvWarps; i < total; i += kGemvWarps) place(i, piece(i));
+        rest(place);
         ptx::bar_sync(15, kGemvWarps * 32);
 
         // lanes of columns without a row read column 0 of x: what they compute is in columns that are not stored
@@ -770,7 +781,8 @@ cudaError_t gemv_launch(const Q4Params& p, cudaStream_t stream) {
     const GemvPlan plan = gemv_plan<NT, INT>(p.K, G, p.R, p.index != nullptr);
     if (plan.unit_rows <= 0) return cudaErrorInvalidValue;   // the entry point has checked q4_gemv_fits
     const int sms = core_sm_count(), kblocks = q4_kblocks(p.K);
-    const long long units = p.index ? (p.R < p.E ? p.R : p.E) : (p.R + plan.unit_rows - 1) / plan.unit_rows;   // about
+    const long long matrices = p.index && p.E > 0 ? (p.R < p.E ? p.R : p.E) : 1, share = (p.R + matrices - 1) / matrices;
+    const long long units = matrices * ((share + plan.unit_rows - 1) / plan.unit_rows);   // as if the rows were spread evenly
     const long long items = units * q4_strips(p.N);
     const int grid = static_cast<int>(items < 1 ? 1 : (items < sms ? items : sms));
     // Warps to a strip: the number that needs the fewest slot times, where the groups of a CTA share its strips and a strip's end costs about
