@@ -11,8 +11,9 @@ namespace t2sp {
 constexpr int kMaxGroups = 1024;  // the kernels keep the groups' tables in shared memory
 
 enum : int { GR_FWD_MN = 0, GR_FWD_K = 1, GR_GRAD = 2 };  // B with n innermost, B with k innermost, gradient of B
-// 128 x 128 by one CTA, 256 x 256 and 512 x 256 by a pair, 128 x 32 by one (of a cluster that shares the contraction)
-enum : int { GR_TILE_128 = 0, GR_TILE_256 = 1, GR_TILE_512 = 2, GR_TILE_32 = 3 };
+// 128 x 128 by one CTA, 256 x 256 and 512 x 256 by a pair, 128 x 32 by one (of a cluster that shares the contraction), 128 x 128 with
+// a B that warps bring
+enum : int { GR_TILE_128 = 0, GR_TILE_256 = 1, GR_TILE_512 = 2, GR_TILE_32 = 3, GR_TILE_WARPS = 4 };
 enum : int { GR_OUT_F32 = 0, GR_OUT_BF16 = 1, GR_OUT_F16 = 2 };
 
 // Forward: C[t][n] = sum_k A[t][k] * B[e][k][n] for offsets[e] <= t < offsets[e+1]; rows outside every group are not
@@ -24,6 +25,9 @@ struct GroupedParams {
     long long ldc, bs_c;   // row pitch of C or G, stride between the matrices of G
     int rows, E, K, N;
     int bf16;              // element type of the inputs: 1 bf16, 0 f16
+    // an operand B that TMA cannot read in place, read by warps instead (null: through the map)
+    const uint16_t *b_src, *b_end;
+    long long b_ld, b_bs;
     long long wait_cycles; // limit of every mbarrier wait in SM cycles, 0: kWaitTimeoutCycles
     unsigned* status;
 };
@@ -34,6 +38,9 @@ struct GroupedMaps {
 };
 
 cudaError_t grouped_launch(int mode, int out, const GroupedParams& p, const GroupedMaps& maps, cudaStream_t stream);
+
+// Whether a B that TMA cannot read in place is better read by warps (through b_src) than copied first.
+bool grouped_warps_worthwhile(int mode, int out, const GroupedParams& p);
 
 // dst[m][r][i] (row pitch ld_dst, dense matrices) = src[m * bs_src + r * ld_src + i], 16-bit elements; ld_dst is a multiple of 8. Up to
 // two operands in one launch.

@@ -36,7 +36,7 @@ template <int MODE, int VAR>
 cudaError_t launch_var(int out, const GroupedParams& p, const GroupedMaps& maps, long long tiles, cudaStream_t stream) {
     const long long slots = core_sm_count() / GroupedCfg<MODE, VAR>::kPair;
     const int workers = static_cast<int>(tiles < slots ? (tiles > 0 ? tiles : 1) : slots);
-    if constexpr (VAR != GR_TILE_512)
+    if constexpr (VAR != GR_TILE_512 && VAR != GR_TILE_WARPS)
         if (out == GR_OUT_F32) return launch_typed<MODE, VAR, float>(p, maps, workers, stream);
     if (out == GR_OUT_BF16) return launch_typed<MODE, VAR, __nv_bfloat16>(p, maps, workers, stream);
     return launch_typed<MODE, VAR, __half>(p, maps, workers, stream);
@@ -90,6 +90,8 @@ long long count_tiles(int mode, const GroupedParams& p, int tn, int tc, bool mos
 // (8 groups of 2 rows, 1024 x 1024: 8.8 us against 10.0); the gradient's outputs are too large for that to pay (12.0 against 13.9).
 template <int MODE>
 cudaError_t launch_mode(int out, const GroupedParams& p, const GroupedMaps& maps, cudaStream_t stream) {
+    if constexpr (MODE != GR_GRAD)
+        if (p.b_src) return launch_var<MODE, GR_TILE_WARPS>(out, p, maps, count_tiles(MODE, p, 128, 128, true), stream);
     const long long pairs = core_sm_count() / 2;
     const long long rounds256 = (count_tiles(MODE, p, 256, 256, false) + pairs - 1) / pairs;
     const long long rounds512 = (count_tiles(MODE, p, 512, 256, false) + pairs - 1) / pairs;
@@ -130,6 +132,16 @@ cudaError_t grouped_launch(int mode, int out, const GroupedParams& p, const Grou
     if (mode == GR_FWD_MN) return launch_mode<GR_FWD_MN>(out, p, maps, stream);
     if (mode == GR_FWD_K) return launch_mode<GR_FWD_K>(out, p, maps, stream);
     return launch_mode<GR_GRAD>(out, p, maps, stream);
+}
+
+// Where each group has one tile of columns, B is read once and the copy costs more than the products: 18 groups of 57 rows, 3520 x 2767: 153 us
+// by warps against 226 with the copy; 27 groups of 2 rows, 5759 x 1408: 173 against 285; 128 rows a group 209 against 230. With more rows
+// the warps read B again for every tile (250 rows, 1001 x 2001: 54 against 44), and with few tiles they cannot keep the memory busy while the
+// copy lets a cluster share a tile (2 tiles, K = 5378: 60 against 15).
+bool grouped_warps_worthwhile(int mode, int out, const GroupedParams& p) {
+    if (mode == GR_GRAD || out == GR_OUT_F32 || p.rows == 0 || p.E == 0) return false;
+    const long long groups = p.rows < p.E ? p.rows : p.E;
+    return p.rows <= 128 * groups && 3 * count_tiles(mode, p, 128, 128, false) >= 2 * core_sm_count();
 }
 
 cudaError_t repack16_launch(Repack* jobs, int count, cudaStream_t stream) {

@@ -26,11 +26,11 @@ struct Operand {
 };
 
 // Copies operands that TMA cannot read in place into scratch memory with padded rows.
-int fit_operands(Views& vw, Operand& a, Operand& b) {
+int fit_operands(Views& vw, Operand* a, Operand* b) {
     Repack jobs[2];
     int count = 0;
-    for (Operand* o : {&a, &b}) {
-        if (o->fits()) continue;
+    for (Operand* o : {a, b}) {
+        if (!o || o->fits()) continue;
         const int64_t ld = (int64_t(o->inner) + 7) / 8 * 8;
         void* q = rt_alloc(size_t(ld) * o->rows * o->matrices * 2);
         if (!q) return halide_error_code_device_malloc_failed;
@@ -63,7 +63,9 @@ bool encode(CUtensorMap* map, uint32_t type, const Operand& o, int rank, uint32_
 // `q_op` the rows (A).
 int run_grouped(const char* who, int mode, uint32_t type, uint32_t out, GroupedParams& p, Operand p_op, Operand q_op, Views& vw,
                 bool sync_after) {
-    if (int e = check_capture(who, false, !p_op.fits() || !q_op.fits())) return e;
+    const int out_kind = out == kF32 ? GR_OUT_F32 : (out == kBF16 ? GR_OUT_BF16 : GR_OUT_F16);
+    const bool in_place = !p_op.fits() && grouped_warps_worthwhile(mode, out_kind, p);
+    if (int e = check_capture(who, false, (!p_op.fits() && !in_place) || !q_op.fits())) return e;
     cudaStream_t s = rt_stream();
     p.status = rt_status_word();
     p.wait_cycles = rt_env().wait_cycles;
@@ -72,14 +74,20 @@ int run_grouped(const char* who, int mode, uint32_t type, uint32_t out, GroupedP
     GroupedMaps maps;
     memset(&maps, 0, sizeof(maps));
     if (p.K > 0 && p.rows > 0) {   // else nothing is read
-        if (int e = fit_operands(vw, p_op, q_op)) return e;
-        bool ok = encode(&maps.p, type, p_op, 3, 64, mode == GR_FWD_K ? 128 : 64) &&
+        if (in_place) {
+            p.b_src = reinterpret_cast<const uint16_t*>(p_op.ptr);
+            p.b_end = p.b_src + (p_op.matrices - 1) * p_op.bs + (p_op.rows - 1) * p_op.ld + p_op.inner;
+            p.b_ld = p_op.ld;
+            p.b_bs = p_op.bs;
+        }
+        if (int e = fit_operands(vw, in_place ? nullptr : &p_op, &q_op)) return e;
+        bool ok = (in_place || encode(&maps.p, type, p_op, 3, 64, mode == GR_FWD_K ? 128 : 64)) &&
                   encode(&maps.q[0], type, q_op, 2, 64, mode == GR_GRAD ? 64 : 128);
         if (mode != GR_GRAD)
             for (int b = 1; b < 4; ++b) ok = ok && encode(&maps.q[b], type, q_op, 2, 64, 128 >> b);
         if (!ok) return tma_unsupported(mode == GR_GRAD ? "A or D" : "A or B");
     }
-    const cudaError_t e = grouped_launch(mode, out == kF32 ? GR_OUT_F32 : (out == kBF16 ? GR_OUT_BF16 : GR_OUT_F16), p, maps, s);
+    const cudaError_t e = grouped_launch(mode, out_kind, p, maps, s);
     if (e != cudaSuccess) {
         fprintf(stderr, "t2sp_b200: %s: kernel launch failed: %s\n", who, cudaGetErrorString(e));
         return halide_error_code_device_run_failed;

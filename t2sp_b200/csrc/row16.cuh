@@ -11,6 +11,19 @@ __device__ __forceinline__ uint4 load16_stream(const void* p) {
     return v;
 }
 
+// The eight elements from element m on (0 .. 7) of two aligned pieces.
+__device__ __forceinline__ uint4 row16_cut(const uint4& a, const uint4& b, int m) {
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = m & 4 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = m & 2 ? w[i + 1] : w[i];
+    const int bits = (m & 1) * 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // Elements src[0 .. 7], zeros from src[left] on. A piece that does not start on 16 bytes is cut out of the two aligned pieces around it, where
 // these lie within [begin, end), the operand's memory (eight 2-byte loads a thread kept a copy at a fifth of the memory's rate).
 __device__ __forceinline__ uint4 row16_load(const uint16_t* src, int left, const uint16_t* begin, const uint16_t* end) {
@@ -20,17 +33,7 @@ __device__ __forceinline__ uint4 row16_load(const uint16_t* src, int left, const
     uint4 v = make_uint4(0, 0, 0, 0);
     if (left >= 8 && base >= begin && base + 16 <= end) {
         const uint4 a = load16_stream(base), b = load16_stream(base + 8);
-        uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        if (m & 4)
-#pragma unroll
-            for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-        if (m & 2)
-#pragma unroll
-            for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-        if (m & 1)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
-        return make_uint4(w[0], w[1], w[2], w[3]);
+        return row16_cut(a, b, m);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j)

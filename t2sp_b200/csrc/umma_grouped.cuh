@@ -29,7 +29,8 @@ template <int MODE, int VAR>
 struct GroupedCfg {
     static constexpr bool kGrad = MODE == GR_GRAD;
     static constexpr bool kPMn = MODE != GR_FWD_K;           // the MMA's A operand (n) is MN-major
-    static constexpr int kPair = VAR == GR_TILE_128 || VAR == GR_TILE_32 ? 1 : 2;  // CTAs of a tile
+    static constexpr bool kWarps = VAR == GR_TILE_WARPS;
+    static constexpr int kPair = VAR == GR_TILE_128 || VAR == GR_TILE_32 || kWarps ? 1 : 2;  // CTAs of a tile
     static constexpr int kSub = VAR == GR_TILE_512 ? 2 : 1;  // sub-tiles of a CTA
     static constexpr int kTileN = 128 * kPair * kSub;
     static constexpr int kTileC = VAR == GR_TILE_32 ? 32 : 128 * kPair;
@@ -42,7 +43,8 @@ struct GroupedCfg {
     static constexpr int kQBytes = 128 * 128;                 // up to 128 columns x 64 k of one CTA
     static constexpr int kStageBytes = kPBytes + kQBytes;
     static constexpr int kEpiWarps = 8;                       // two for each quarter of the tensor memory's lanes
-    static constexpr int kThreads = (2 + kEpiWarps + (kGrad ? 1 : 0)) * 32;
+    static constexpr int kLoadWarps = kWarps ? 2 * kStages : 0;   // two for each stage
+    static constexpr int kThreads = (2 + kEpiWarps + (kGrad ? 1 : 0) + kLoadWarps) * 32;
     static constexpr int kTmemCols = kAccs * kTileC;
     static constexpr int kNumBars = 4 * kStages + 4;
     static constexpr int kOutBytes = kEpiWarps * 2048;        // a 64 x 32 tile of 16-bit results for two epilogue warps
@@ -219,6 +221,83 @@ __device__ __forceinline__ void grouped_store(float* dst, long long ld, int cols
         if (j < cols) dst[j * ld] = r[j];
 }
 
+// The blocks of a B whose rows do not start on 16 bytes, brought by two warps for each stage of the ring (a stage stays with its warps: a wait on
+// the parity of its barrier must not miss a phase). A block is 1024 pieces of eight elements, cut out of the aligned pieces around them and written
+// where TMA's 128-byte swizzle would put them (piece ^ row % 8); a lane has the loads of eight pieces on their way together.
+// (Copying B into padded memory first moves it three times, once as writes that take nearly twice as long as reads; see
+// grouped_warps_worthwhile for what was measured.)
+template <int MODE, int VAR>
+__device__ __forceinline__ void grouped_load(const GroupedParams& p, const int* off, const int* first, uint8_t* smem, uint64_t* full_bar,
+                                             uint64_t* empty_bar, int worker, int num_workers, const AbortCtx& ab) {
+    using Cfg = GroupedCfg<MODE, VAR>;
+    constexpr bool kMn = MODE == GR_FWD_MN;
+    constexpr int kBatch = 8;
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - (2 + Cfg::kEpiWarps), mine = warp >> 1, id = (warp & 1) * 32 + lane;
+    // n innermost: 64 k x 16 pieces of 8 n; k innermost: 128 n x 8 pieces of 8 k. This lane's piece of a row, its first row and the step to the next
+    constexpr int kPieces = kMn ? 16 : 8, kStep = 64 / kPieces;
+    const int c = id % kPieces, r0 = id / kPieces;
+    int it = 0, e = 0;
+    GroupedTile g;
+    for (int t = worker; grouped_tile<MODE, VAR>(p, off, first, t, e, g); t += num_workers) {
+        const uint16_t* b = p.b_src + g.e * p.b_bs;
+        for (int kb = 0; kb < g.num_kb; ++kb, ++it) {
+            const int s = it % Cfg::kStages;
+            if (s != mine) continue;
+            uint8_t* slot = smem + s * Cfg::kStageBytes;
+            constexpr int kRows = kMn ? 64 : 128, kCols = kMn ? 128 : 64;
+            const int row0 = kMn ? kb * 64 : g.n0, col0 = kMn ? g.n0 : kb * 64;
+            const int rows = min(kRows, (kMn ? p.K : p.N) - row0), cols = min(kCols, (kMn ? p.N : p.K) - col0);   // that exist
+            const uint16_t* block = b + row0 * p.b_ld + col0;
+            // Pieces outside the matrix are loaded as if they were its last row's or the row's first one. What they hold does not matter
+            // beyond N, whose results are not stored; beyond K it is cleared.
+            const uint16_t* src = block + (c * 8 < cols ? c * 8 : 0);
+            // the aligned pieces around the first and the last piece lie inside the operand's memory (not at its very ends)
+            const bool inside = block - 7 >= p.b_src && block + (rows - 1) * p.b_ld + ((cols - 1) & ~7) + 16 <= p.b_end;
+#pragma unroll 1
+            for (int i = 0; i < kRows / kStep; i += kBatch) {
+                uint4 v[kBatch];
+                if (inside) {
+                    uint4 lo[kBatch], hi[kBatch];
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const uint16_t* at = src + min(r0 + (i + j) * kStep, rows - 1) * p.b_ld;
+                        const uint16_t* base = reinterpret_cast<const uint16_t*>(reinterpret_cast<uintptr_t>(at) & ~uintptr_t(15));
+                        lo[j] = load16_stream(base);
+                        hi[j] = load16_stream(base + 8);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const uint16_t* at = src + min(r0 + (i + j) * kStep, rows - 1) * p.b_ld;
+                        v[j] = row16_cut(lo[j], hi[j], static_cast<int>(reinterpret_cast<uintptr_t>(at) & 15) >> 1);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j)
+                        v[j] = row16_load(src + min(r0 + (i + j) * kStep, rows - 1) * p.b_ld, min(8, cols - (c * 8 < cols ? c * 8 : 0)), p.b_src, p.b_end);
+                }
+                if (kb * 64 + 64 > p.K) {
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const int left = kMn ? (r0 + (i + j) * kStep < rows ? 8 : 0) : cols - c * 8;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (2 * k + 1 >= left) (&v[j].x)[k] = 2 * k < left ? (&v[j].x)[k] & 0xffffu : 0u;
+                    }
+                }
+                if (i == 0 && !bounded_wait_warp(&empty_bar[s], ((it / Cfg::kStages) & 1) ^ 1, ab, ST_TIMEOUT_SPLITTER, lane)) return;
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) {
+                    const int r = r0 + (i + j) * kStep;
+                    *reinterpret_cast<uint4*>(slot + (kMn ? (c >> 3) * 8192 : 0) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[j];
+                }
+            }
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&full_bar[s]);
+        }
+    }
+}
+
 template <int MODE, int VAR, class O>
 __global__ void __launch_bounds__(GroupedCfg<MODE, VAR>::kThreads, 1)
 grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ GroupedMaps maps) {
@@ -251,7 +330,7 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
-            ptx::mbar_init(&full_bar[s], 1);
+            ptx::mbar_init(&full_bar[s], Cfg::kWarps ? 3 : 1);
             ptx::mbar_init(&empty_bar[s], 1);
             ptx::mbar_init(&tail_bar[s], 1);
             ptx::mbar_init(&fixed_bar[s], kPair);
@@ -302,7 +381,7 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer (every CTA)
         if (lane == 0) {
-            if (p.K > 0 && p.rows > 0) {   // else the maps describe nothing and no tile has a k-block
+            if (!Cfg::kWarps && p.K > 0 && p.rows > 0) {   // else a map may describe nothing
                 ptx::prefetch_tensormap(&maps.p);
                 ptx::prefetch_tensormap(&maps.q[0]);
             }
@@ -343,9 +422,9 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
                         load2(sq, &maps.q[0], bar, owner, c0, row);
                         if (qboxes == 2) load2(sq + 8192, &maps.q[0], bar, owner, c0 + 64, row);
                     } else {
-                        if (rank == 0) ptx::mbar_expect_tx(&full_bar[s], kPair * (Cfg::kPBytes + part * 128));
+                        if (rank == 0) ptx::mbar_expect_tx(&full_bar[s], kPair * ((Cfg::kWarps ? 0 : Cfg::kPBytes) + part * 128));
 #pragma unroll
-                        for (int u = 0; u < kSub; ++u) {
+                        for (int u = 0; u < (Cfg::kWarps ? 0 : kSub); ++u) {
                             if constexpr (MODE == GR_FWD_MN) {
                                 load3(sp + u * Cfg::kSubBytes, &maps.p, bar, owner, n0 + u * 256, kb * 64, g.e);
                                 load3(sp + u * Cfg::kSubBytes + 8192, &maps.p, bar, owner, n0 + u * 256 + 64, kb * 64, g.e);
@@ -475,6 +554,9 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive_cluster(&fixed_bar[s], 0);
         }
+    } else if (Cfg::kWarps && warp >= 2 + Cfg::kEpiWarps) {
+        // ------------------------------------------------------------ warps that bring a B which TMA cannot read in place
+        if constexpr (Cfg::kWarps) grouped_load<MODE, VAR>(p, off, first, smem, full_bar, empty_bar, worker, num_workers, ab);
     } else {
         // ------------------------------------------------------------ epilogue (every CTA, its own 128 n): two warps to a quarter of the
         // lanes, each takes every other 32 columns

@@ -76,6 +76,9 @@ SHAPES = [
     ([3], 4104, 136, 1, 1),
     ([2, 1], 320, 1000, 0, 0),
     ([2100, 300], 2112, 1032, 0, 0),
+    ([64, 5, 0, 300], 1379, 1188, 0, 2),   # rows that do not start on 16 bytes, many blocks and tiles
+    ([20] * 12, 1222, 1417, 0, 0),
+    ([7], 5378, 187, 0, 1),
 ]
 
 
