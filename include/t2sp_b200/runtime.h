@@ -204,9 +204,12 @@ int t2sp_b200_mttkrp(halide_buffer_t *a, halide_buffer_t *b, halide_buffer_t *c,
  * compute nothing and report halide_error_code_access_out_of_bounds (for asynchronous calls at t2sp_b200_sync).
  *   grouped_gemm_grad: the gradient of B, G(n,k,e) = sum over the rows t of group e of A(k,t) * D(n,t);
  * D: 2-D (N, M), G: 3-D (N, K, E), zeros for an empty group. For a B with trans_b, exchange A and D.
- * Strides: innermost 1, outer ones positive, outputs without overlap. Operands whose base and outer strides are multiples
- * of 16 bytes are read in place; others are first copied into scratch memory, which a captured stream refuses
- * (halide_error_code_constraint_violated). */
+ * Strides: innermost 1, outer ones positive, outputs without overlap; extents up to 2^30; device addresses are multiples of the
+ * element's size. Operands whose base and outer strides are multiples of 16 bytes are read in place, and so is any B of the
+ * forward product with a 16-bit result where the groups have 128 rows at most on average and the tiles fill the GPU; other operands
+ * are first copied into scratch memory, which a captured stream refuses (halide_error_code_constraint_violated). Aligned
+ * strides are up to three times as fast.
+ * An operand without elements needs an address too: a buffer with neither host nor device address makes the call a bounds query. */
 typedef struct t2sp_grouped_desc {
     int32_t trans_b;
 } t2sp_grouped_desc;
@@ -226,7 +229,12 @@ int t2sp_b200_grouped_gemm_grad(halide_buffer_t *A, halide_buffer_t *D, halide_b
  * gives their shapes; both 16-byte aligned). X: 2-D (K, T), Y: 2-D (N, R) with R a multiple of T, of X's type or fp32;
  * X and S have one type. index: 1-D (R) int32, or NULL with E = 1. A row with a negative index is left as it was; an index
  * of E or more leaves the row as it was and reports halide_error_code_access_out_of_bounds (for asynchronous calls
- * at t2sp_b200_sync). For many rows, q4_unpack and grouped_gemm are faster. */
+ * at t2sp_b200_sync). Up to 1024 rows with an index. A row of X is staged in shared memory, which ends K at about 65536
+ * (halide_error_code_constraint_violated beyond).
+ * Up to four rows to a matrix are multiplied as integers of 31 bits times a power of two of the row: a value of X counts to
+ * 2^-31 of its row's largest (values down to 2^-19 of it in f16, 2^-22 in bf16, count exactly), and a row that holds a NaN or an
+ * infinity gives NaN. More rows are multiplied in X's type. The results of a row do not depend on the other rows' values, but their last bits
+ * do on how many there are. For many rows, q4_unpack and grouped_gemm are faster. */
 typedef struct t2sp_q4_desc {
     int32_t group;   /* 32, 64 or 128; 0 = 64 */
     int32_t trans_b; /* W has k innermost (q4_gemv ignores it) */

@@ -200,6 +200,21 @@ int check_strides(const Arg& a) {
     return 0;
 }
 
+// The kernels of the entries with ragged shapes count in 32 bits and add a tile's length to an extent.
+int check_extent_limit(const Arg& a) {
+    for (int d = 0; d < a.b->dimensions; ++d)
+        if (a.b->dim[d].extent > (1 << 30))
+            return halide_error_buffer_extents_too_large(nullptr, a.name, a.b->dim[d].extent, int64_t(1) << 30);
+    return 0;
+}
+
+// A device address is a multiple of the element's size (the kernels that take any 16-bit alignment need at least that).
+int check_device_address(const Arg& a) {
+    const int bytes = (a.b->type.bits + 7) / 8, off = static_cast<int>(a.b->device % uint64_t(bytes));
+    if (!buf_on_our_device(a.b) || off == 0) return 0;
+    return constraint((std::string(a.name) + ".device").c_str(), off, "a multiple of the element's size", bytes);
+}
+
 // A call whose stream is being captured into a graph can neither wait for its kernels nor take scratch memory that
 // the graph would go on using after the call has handed it back.
 int check_capture(const char* who, bool waits, bool scratch) {

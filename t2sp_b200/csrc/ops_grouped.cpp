@@ -134,6 +134,8 @@ extern "C" int t2sp_b200_grouped_gemm(halide_buffer_t* A, halide_buffer_t* B, ha
     if (int e = check_type_dims(args[3], out_f32 ? kF32 : in_t)) return e;
     for (auto& a : args)
         if (int e = check_extents_nonneg(a)) return e;
+    for (auto& a : args)
+        if (int e = check_extent_limit(a)) return e;
     const int K = A->dim[0].extent, M = A->dim[1].extent, N = B->dim[tb ? 1 : 0].extent, E = B->dim[2].extent;
     if (B->dim[tb ? 0 : 1].extent != K)
         return constraint(tb ? "B.extent.0" : "B.extent.1", B->dim[tb ? 0 : 1].extent, "A.extent.0", K);
@@ -149,6 +151,8 @@ extern "C" int t2sp_b200_grouped_gemm(halide_buffer_t* A, halide_buffer_t* B, ha
         if (int e = check_strides(a)) return e;
     for (auto& a : args)
         if (int e = check_sizes(a)) return e;
+    for (auto& a : args)
+        if (int e = check_device_address(a)) return e;
     for (auto& a : args)
         if (int e = check_host(a)) return e;
     if (M == 0 || N == 0 || E == 0) return 0;
@@ -203,6 +207,8 @@ extern "C" int t2sp_b200_grouped_gemm_grad(halide_buffer_t* A, halide_buffer_t* 
     if (int e = check_type_dims(args[3], out_f32 ? kF32 : in_t)) return e;
     for (auto& a : args)
         if (int e = check_extents_nonneg(a)) return e;
+    for (auto& a : args)
+        if (int e = check_extent_limit(a)) return e;
     const int K = A->dim[0].extent, M = A->dim[1].extent, N = D->dim[0].extent;
     if (D->dim[1].extent != M) return constraint("D.extent.1", D->dim[1].extent, "A.extent.1", M);
     if (int e = check_offsets(args[2])) return e;
@@ -218,6 +224,8 @@ extern "C" int t2sp_b200_grouped_gemm_grad(halide_buffer_t* A, halide_buffer_t* 
         if (int e = check_strides(a)) return e;
     for (auto& a : args)
         if (int e = check_sizes(a)) return e;
+    for (auto& a : args)
+        if (int e = check_device_address(a)) return e;
     for (auto& a : args)
         if (int e = check_host(a)) return e;
     if (K == 0 || N == 0 || E == 0) return 0;

@@ -52,6 +52,30 @@ void packed_extents(int N, int K, int E, int group, int* q, int* s) {
     s[0] = 16; s[1] = q4_groups(K, group); s[2] = q4_strips(N); s[3] = E;
 }
 
+// Bounds queries of q4_pack and q4_unpack: the packed shapes from W, or the largest W that the packed shapes hold.
+int query_w_q_s(Arg* args, int w, int q, int s, int tb, int group) {
+    halide_buffer_t *W = args[w].b, *Q = args[q].b, *S = args[s].b;
+    if (buf_is_bounds_query(W)) {
+        if (buf_is_bounds_query(Q)) return halide_error_host_is_null(nullptr, args[w].role().c_str());
+        if (int e = check_type_dims(args[q], kU8)) return e;
+        const uint32_t t = buf_is_bounds_query(S) ? kBF16 : buf_type_word(S);
+        const int N = Q->dim[2].extent * 16, K = Q->dim[1].extent * 64;
+        const int we[3] = {tb ? K : N, tb ? N : K, Q->dim[3].extent};
+        fill_query(W, t, 3, we);
+    } else {
+        const uint32_t t = buf_type_word(W);
+        if (t != kBF16 && t != kF16) return halide_error_bad_type(nullptr, args[w].role().c_str(), t, kBF16);
+        if (int e = check_type_dims(args[w], t)) return e;
+        if (int e = check_extents_nonneg(args[w])) return e;
+    }
+    int qe[4], se[4];
+    packed_extents(W->dim[tb ? 1 : 0].extent, W->dim[tb ? 0 : 1].extent, W->dim[2].extent, group, qe, se);
+    const uint32_t t = buf_type_word(W);
+    if (buf_is_bounds_query(Q)) fill_query(Q, kU8, 4, qe);
+    if (buf_is_bounds_query(S)) fill_query(S, t, 4, se);
+    return 0;
+}
+
 // W with Q and S: the checks that q4_pack and q4_unpack share.
 int check_w_q_s(Arg* args, int w, int q, int s, int tb, int group) {
     const uint32_t t = buf_type_word(args[w].b);
@@ -61,11 +85,13 @@ int check_w_q_s(Arg* args, int w, int q, int s, int tb, int group) {
     if (int e = check_type_dims(args[s], t)) return e;
     for (int i = 0; i < 3; ++i)
         if (int e = check_extents_nonneg(args[i])) return e;
+    if (int e = check_extent_limit(args[w])) return e;
     if (int e = check_min0(args[w])) return e;
     if (int e = check_stride0(args[w])) return e;
     if (int e = check_strides(args[w])) return e;
     for (int i = 0; i < 3; ++i)
         if (int e = check_sizes(args[i])) return e;
+    if (int e = check_device_address(args[w])) return e;
     const halide_buffer_t* W = args[w].b;
     int qe[4], se[4];
     packed_extents(W->dim[tb ? 1 : 0].extent, W->dim[tb ? 0 : 1].extent, W->dim[2].extent, group, qe, se);
@@ -85,18 +111,7 @@ extern "C" int t2sp_b200_q4_pack(halide_buffer_t* W, halide_buffer_t* Q, halide_
     int group = 0;
     if (int e = resolve_group(desc, &group)) return e;
     const int tb = desc && desc->trans_b ? 1 : 0;
-    if (buf_is_bounds_query(W)) return halide_error_host_is_null(nullptr, args[0].role().c_str());
-    if (buf_is_bounds_query(Q) || buf_is_bounds_query(S)) {
-        const uint32_t t = buf_type_word(W);
-        if (t != kBF16 && t != kF16) return halide_error_bad_type(nullptr, args[0].role().c_str(), t, kBF16);
-        if (int e = check_type_dims(args[0], t)) return e;
-        if (int e = check_extents_nonneg(args[0])) return e;
-        int qe[4], se[4];
-        packed_extents(W->dim[tb ? 1 : 0].extent, W->dim[tb ? 0 : 1].extent, W->dim[2].extent, group, qe, se);
-        if (buf_is_bounds_query(Q)) fill_query(Q, kU8, 4, qe);
-        if (buf_is_bounds_query(S)) fill_query(S, t, 4, se);
-        return 0;
-    }
+    if (buf_is_bounds_query(W) || buf_is_bounds_query(Q) || buf_is_bounds_query(S)) return query_w_q_s(args, 0, 1, 2, tb, group);
     if (int e = check_w_q_s(args, 0, 1, 2, tb, group)) return e;
     Q4Params p = {};
     p.N = W->dim[tb ? 1 : 0].extent; p.K = W->dim[tb ? 0 : 1].extent; p.E = W->dim[2].extent;
@@ -128,6 +143,7 @@ extern "C" int t2sp_b200_q4_unpack(halide_buffer_t* Q, halide_buffer_t* S, halid
     int group = 0;
     if (int e = resolve_group(desc, &group)) return e;
     const int tb = desc && desc->trans_b ? 1 : 0;
+    if (buf_is_bounds_query(Q) || buf_is_bounds_query(S) || buf_is_bounds_query(W)) return query_w_q_s(args, 2, 0, 1, tb, group);
     if (int e = check_w_q_s(args, 2, 0, 1, tb, group)) return e;
     Q4Params p = {};
     p.N = W->dim[tb ? 1 : 0].extent; p.K = W->dim[tb ? 0 : 1].extent; p.E = W->dim[2].extent;
@@ -158,6 +174,26 @@ extern "C" int t2sp_b200_q4_gemv(halide_buffer_t* X, halide_buffer_t* Q, halide_
     const int n_args = index ? 5 : 4;
     int group = 0;
     if (int e = resolve_group(desc, &group)) return e;
+    const bool query_index = index && buf_is_bounds_query(index);
+    if (buf_is_bounds_query(X) || buf_is_bounds_query(Q) || buf_is_bounds_query(S) || buf_is_bounds_query(Y) || query_index) {
+        // where X or Y does not say K or N, the most that the packed matrices hold
+        int K = 0, N = 0, T = 0, R = 0, E = 1;
+        uint32_t t = kBF16;
+        if (!buf_is_bounds_query(Q) && Q->dimensions == 4) { K = Q->dim[1].extent * 64; N = Q->dim[2].extent * 16; E = Q->dim[3].extent; }
+        if (!buf_is_bounds_query(S)) t = buf_type_word(S);
+        if (!buf_is_bounds_query(X) && X->dimensions == 2) { t = buf_type_word(X); K = X->dim[0].extent; T = R = X->dim[1].extent; }
+        if (index && !query_index && index->dimensions == 1) R = index->dim[0].extent;
+        if (!buf_is_bounds_query(Y) && Y->dimensions == 2) { N = Y->dim[0].extent; R = Y->dim[1].extent; }
+        if (!T) T = R;
+        int qe[4], se[4];
+        packed_extents(N, K, E, group, qe, se);
+        if (buf_is_bounds_query(X)) { int x[2] = {K, T}; fill_query(X, t, 2, x); }
+        if (buf_is_bounds_query(Q)) fill_query(Q, kU8, 4, qe);
+        if (buf_is_bounds_query(S)) fill_query(S, t, 4, se);
+        if (query_index) { int x[1] = {R}; fill_query(index, kI32, 1, x); }
+        if (buf_is_bounds_query(Y)) { int x[2] = {N, R}; fill_query(Y, t, 2, x); }
+        return 0;
+    }
     const uint32_t t = buf_type_word(X);
     if (t != kBF16 && t != kF16) return halide_error_bad_type(nullptr, args[0].role().c_str(), t, kBF16);
     const bool out_f32 = buf_type_word(Y) == kF32;
@@ -169,6 +205,8 @@ extern "C" int t2sp_b200_q4_gemv(halide_buffer_t* X, halide_buffer_t* Q, halide_
         if (int e = check_type_dims(args[4], kI32)) return e;
     for (int i = 0; i < n_args; ++i)
         if (int e = check_extents_nonneg(args[i])) return e;
+    for (int i = 0; i < n_args; ++i)
+        if (int e = check_extent_limit(args[i])) return e;
     Q4Params p = {};
     p.K = X->dim[0].extent; p.N = Y->dim[0].extent; p.E = Q->dim[3].extent; p.R = Y->dim[1].extent;
     const int T = X->dim[1].extent;
@@ -186,6 +224,8 @@ extern "C" int t2sp_b200_q4_gemv(halide_buffer_t* X, halide_buffer_t* Q, halide_
         if (int e = check_strides(args[i])) return e;
     for (int i = 0; i < n_args; ++i)
         if (int e = check_sizes(args[i])) return e;
+    for (int i = 0; i < n_args; ++i)
+        if (int e = check_device_address(args[i])) return e;
     int qe[4], se[4];
     packed_extents(p.N, p.K, p.E, group, qe, se);
     if (int e = check_packed(args[1], qe, 16)) return e;

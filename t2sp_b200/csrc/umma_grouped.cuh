@@ -62,13 +62,13 @@ struct GroupedTile {
     int row0, tail;     // gradient: first row of the group; rows in its last block (64: not ragged)
 };
 
-// n / d and n % d for 0 <= n, 0 < d, n / d < 2^21, through a reciprocal (the compiler's division takes several times as long, and every role
-// goes through a handful for each tile): the product is off the quotient by less than one.
+// n / d and n % d for 0 <= n, 0 < d, through a reciprocal (the compiler's division takes several times as long, and every role
+// goes through a handful for each tile): up to quotients of 2^21 the product is off by less than one, beyond by a few.
 __device__ __forceinline__ int quick_div(int n, int d, int& rest) {
     int q = static_cast<int>(__fdividef(static_cast<float>(n), static_cast<float>(d)));
     rest = n - q * d;
-    if (rest < 0) { --q; rest += d; }
-    else if (rest >= d) { ++q; rest -= d; }
+    while (rest < 0) { --q; rest += d; }
+    while (rest >= d) { ++q; rest -= d; }
     return q;
 }
 // tile_coords of umma_core.cuh: groups of G row-blocks sweep all column-blocks, rows fastest inside a group.
@@ -149,8 +149,8 @@ __device__ __forceinline__ bool grouped_tables(const GroupedParams& p, int* off,
     }
     if (MODE == GR_GRAD) {
         // The gradient's tiles take as long as their group has rows, and every worker takes every num_workers-th tile: the largest groups
-        // come first, so that what is left to even out at the end is small (5 groups of 2560 uneven rows, 1328 x 3072: 79 -> 69 us
-        // with both gradients). Many groups are taken as they come: ordering them would cost more than it evens out.
+        // come first, so that what is left to even out at the end is small (5 groups of 2560 uneven rows: 79 -> 69 us with
+        // both gradients). Many groups are taken as they come: ordering them would cost more than it evens out.
         const bool sorted = p.E <= 128;
         for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
             const int rows = off[e + 1] - off[e];

@@ -170,3 +170,48 @@ def test_no_device_launches_nothing(lib, name):
             "q4_pack": lambda: t2sp_b200.q4_pack(h16(2, 100, 40), a["Q"], a["S"], a["desc"]),
             "q4_unpack": lambda: t2sp_b200.q4_unpack(a["Q"], a["S"], h16(2, 100, 40), a["desc"])}[name]() == -36
     assert lib.t2sp_b200_kernel_launches() == before
+
+
+def test_extent_limits(lib):
+    # 32-bit counts: extents end at 2^30 (the packed shapes of such a matrix would not fit 32 bits either)
+    big, top = (1 << 30) + 1, (1 << 31) - 1
+    for n in (big, top):
+        assert grouped(A=strided((16, n), (1, 16)), C=strided((24, n), (1, 24))) == -6
+        assert grad(A=strided((n, 8), (1, n)), G=strided((24, n, 3), (1, 24, 24))) == -6
+        assert gemv(X=strided((n, 3), (1, n))) == -6
+        a = q4_args()
+        assert t2sp_b200.q4_pack(strided((40, n, 2), (1, 40, 40)), a["Q"], a["S"], a["desc"]) == -6
+
+
+def test_device_addresses(lib):
+    def at(extents, dtype, address):
+        b = Buffer(extents, dtype)
+        assert t2sp_b200.wrap_device(b, address) == 0
+        return b
+    assert grouped(A=at((16, 8), "bf16", 4097)) == -8
+    assert grouped(C=at((24, 8), "f32", 4098)) == -8
+    assert grouped(offsets=at((4,), "i32", 4098)) == -8
+    assert grad(G=at((24, 16, 3), "f32", 4098)) == -8
+    assert gemv(X=at((100, 3), "bf16", 4097)) == -8
+    assert gemv(Y=at((40, 6), "f32", 4098)) == -8
+    assert gemv(index=at((6,), "i32", 4097)) == -8
+    a = q4_args()
+    assert t2sp_b200.q4_pack(at((40, 100, 2), "bf16", 4097), a["Q"], a["S"], a["desc"]) == -8
+    assert t2sp_b200.q4_unpack(a["Q"], a["S"], at((40, 100, 2), "bf16", 4097), a["desc"]) == -8
+
+
+def test_q4_bounds_queries_of_products_and_reading(lib):
+    a = q4_args()
+    q = Buffer.query(2)
+    assert gemv(Y=Buffer.query(2)) == 0 and gemv(Y=q) == 0 and [e for _, e, _ in q.shape()] == [48, 6]
+    q = Buffer.query(2)
+    assert gemv(X=q) == 0 and [e for _, e, _ in q.shape()] == [128, 6] and q.raw.type.bits == 16
+    q, s, i = Buffer.query(4), Buffer.query(4), Buffer.query(1)
+    assert gemv(Q=q) == 0 and [e for _, e, _ in q.shape()] == [512, 2, 3, 1]
+    assert gemv(S=s) == 0 and [e for _, e, _ in s.shape()] == [16, 4, 3, 2]
+    assert gemv(index=i) == 0 and [e for _, e, _ in i.shape()] == [6]
+    for trans in (0, 1):
+        w = Buffer.query(3)
+        assert t2sp_b200.q4_unpack(a["Q"], a["S"], w, Q4Desc(32, trans)) == 0
+        assert [e for _, e, _ in w.shape()] == ([128, 48, 2] if trans else [48, 128, 2]) and w.raw.type.bits == 16
+    assert t2sp_b200.q4_pack(Buffer.query(3), Buffer.query(4), Buffer.query(4)) == -34
