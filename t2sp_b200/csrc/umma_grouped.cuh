@@ -48,13 +48,13 @@ struct GroupedCfg {
     static constexpr int kTmemCols = kAccs * kTileC;
     static constexpr int kNumBars = 4 * kStages + 4;
     static constexpr int kOutBytes = kEpiWarps * 2048;        // a 64 x 32 tile of 16-bit results for two epilogue warps
-    static constexpr int kTableBytes = 2 * (kMaxGroups + 4) * 4;  // offsets, first tile of each group
-    static constexpr int kSmemBytes = kStages * kStageBytes + kOutBytes + kTableBytes + kNumBars * 8 + 16 + 1024;
+    static constexpr int kTableBytes = 2 * (kMaxGroups + 4) * 4 + 16;  // offsets, first tile of each group
+    static constexpr int kSmemBytes = kStages * kStageBytes + kOutBytes + kTableBytes + 2048 + kNumBars * 8 + 16 + 1024;
     static_assert(kSmemBytes <= 232448, "shared memory budget exceeded");
 };
 
 // One tile of the output and its contraction.
-struct GroupedTile {
+struct __align__(16) GroupedTile {
     int e, n0, c0;      // group, first n, first column (row t of the group in the forward, k in the gradient)
     int cols;           // columns that exist
     int ncols;          // columns the MMA computes
@@ -79,17 +79,41 @@ __device__ __forceinline__ void quick_coords(int t, int tiles_m, int tiles_n, in
     mb += g * G;
 }
 
+// Blocks of `tile` that are dealt out first; a last block of at most half a tile is left for the end of the call, so that no CTA has full ones only.
+__device__ __forceinline__ int main_blocks(int extent, int tile) {
+    const int full = extent / tile, rest = extent - full * tile;
+    return full + (rest > tile / 2 ? 1 : 0);
+}
+
+// The t-th tile of the call; false when there are no more. Every worker takes every num_workers-th tile.
+//   forward   the groups in turn, each with its main blocks of n; then the narrow last blocks of all groups
+//             (24 groups of 64 rows, 1416 x 776: 22 us when they were dealt out among the others, 13.3 with 1416 x 768)
+//   gradient  long groups (grouped_tables) with all their tiles; then the main blocks of the others, their narrow blocks of n, those of k
 template <int MODE, int VAR>
-__device__ __forceinline__ bool grouped_tile(const GroupedParams& p, const int* off, const int* first, int t, int& e, GroupedTile& g) {
+__device__ bool grouped_tile(const GroupedParams& p, const int* off, const int* first, int t, GroupedTile& g) {
     using Cfg = GroupedCfg<MODE, VAR>;
     constexpr int kRaster = 2048 / Cfg::kTileN;   // n-blocks that are swept together: 2048 n
-    const int nblk = (p.N + Cfg::kTileN - 1) / Cfg::kTileN;
+    const int nblk = (p.N + Cfg::kTileN - 1) / Cfg::kTileN, nmain = main_blocks(p.N, Cfg::kTileN);
     if constexpr (MODE == GR_GRAD) {
-        const int kblk = (p.K + Cfg::kTileC - 1) / Cfg::kTileC, per = nblk * kblk;
+        const int kblk = (p.K + Cfg::kTileC - 1) / Cfg::kTileC, kmain = main_blocks(p.K, Cfg::kTileC), per = nblk * kblk;
         if (t >= per * p.E) return false;
-        int mb, kb, rest;
-        g.e = first[quick_div(t, per, rest)];   // the groups in the order of their rows, most first
-        quick_coords(rest, nblk, kblk, kRaster, mb, kb);
+        const int heavy = first[p.E], light = p.E - heavy;
+        int mb, kb, rest, place;   // place in the order of the groups
+        if (t < heavy * per) {
+            place = quick_div(t, per, rest);
+            quick_coords(rest, nblk, kblk, kRaster, mb, kb);
+        } else if ((t -= heavy * per) < light * nmain * kmain) {
+            place = heavy + quick_div(t, nmain * kmain, rest);
+            quick_coords(rest, nmain, kmain, kRaster, mb, kb);
+        } else if ((t -= light * nmain * kmain) < light * (nblk - nmain) * kmain) {
+            place = heavy + quick_div(t, kmain, kb);
+            mb = nmain;
+        } else {
+            t -= light * (nblk - nmain) * kmain;
+            place = heavy + quick_div(t, nblk, mb);
+            kb = kmain;
+        }
+        g.e = first[place];
         g.n0 = mb * Cfg::kTileN;
         g.c0 = kb * Cfg::kTileC;
         g.cols = min(Cfg::kTileC, p.K - g.c0);
@@ -98,13 +122,19 @@ __device__ __forceinline__ bool grouped_tile(const GroupedParams& p, const int* 
         g.num_kb = (rows + 63) >> 6;
         g.tail = rows - (g.num_kb - 1) * 64;
     } else {
-        if (t >= first[p.E]) return false;
-        while (t >= first[e + 1]) ++e;   // tiles are visited in increasing order
+        const int last = first[p.E] * nmain;   // the first of the narrow tiles
+        if (t >= first[p.E] * nblk) return false;
+        int mb, tb, e = 0;
+        const bool narrow = t >= last;
+        if (narrow) t -= last;
+        const int each = narrow ? 1 : nmain;
+        for (int step = 1 << (31 - __clz(p.E)); step > 0; step >>= 1)   // the last group whose tiles do not begin behind t
+            if (e + step < p.E && first[e + step] * each <= t) e += step;
         g.e = e;
         const int lo = off[e], rows = off[e + 1] - lo;
         const int tiles = (rows + Cfg::kTileC - 1) / Cfg::kTileC;
-        int mb, tb;
-        quick_coords(t - first[e], nblk, tiles, kRaster, mb, tb);
+        if (narrow) { mb = nmain; tb = t - first[e]; }
+        else quick_coords(t - first[e] * nmain, nmain, tiles, kRaster, mb, tb);
         int rest;
         const int per = quick_div(rows + tiles * Cfg::kColStep - 1, tiles * Cfg::kColStep, rest) * Cfg::kColStep;   // near-equal tiles
         g.n0 = mb * Cfg::kTileN;
@@ -118,8 +148,39 @@ __device__ __forceinline__ bool grouped_tile(const GroupedParams& p, const int* 
     return true;
 }
 
-// Offsets into shared memory, checked, and the number of the first tile of every group (forward) or the order of the groups
-// (gradient). Returns false when the
+// The first kListed tiles of a worker, prepared by as many threads at the start: every role goes through the same tiles, and working one out
+// takes 0.2 us (gradient with 24 groups, 576 tiles: XX -> YY us).
+constexpr int kListed = 64;
+constexpr int kListBytes = kListed * static_cast<int>(sizeof(GroupedTile));
+template <int MODE, int VAR>
+__device__ __forceinline__ void grouped_list(const GroupedParams& p, const int* off, const int* first, GroupedTile* list, int worker, int num_workers) {
+    if (threadIdx.x < kListed) {
+        GroupedTile g;
+        g.e = -1;
+        const long long t = worker + static_cast<long long>(threadIdx.x) * num_workers;
+        if (t > 0x7fffffff || !grouped_tile<MODE, VAR>(p, off, first, static_cast<int>(t), g)) g.e = -1;
+        list[threadIdx.x] = g;
+    }
+}
+// What a role needs to go through a worker's tiles: for (i = 0; tiles.get(i, g); ++i).
+template <int MODE, int VAR>
+struct GroupedTiles {
+    const GroupedParams& p;
+    const int *off, *first;
+    const GroupedTile* list;
+    int worker, num_workers;
+    __device__ __forceinline__ bool get(int i, GroupedTile& g) const {
+        if (i < kListed) {
+            g = list[i];
+            return g.e >= 0;
+        }
+        const long long t = worker + static_cast<long long>(i) * num_workers;
+        return t <= 0x7fffffff && grouped_tile<MODE, VAR>(p, off, first, static_cast<int>(t), g);
+    }
+};
+
+// Offsets into shared memory, checked, and the number of tiles of rows before every group (forward) or the order of the groups
+// and how many are long (gradient). Returns false when the
 // offsets decrease or leave the rows; every thread of the CTA gets the verdict.
 template <int MODE, int VAR>
 __device__ __forceinline__ bool grouped_tables(const GroupedParams& p, int* off, int* first) {
@@ -131,11 +192,11 @@ __device__ __forceinline__ bool grouped_tables(const GroupedParams& p, int* off,
     if (__syncthreads_or(bad)) return false;
     if (MODE != GR_GRAD) {
         if (threadIdx.x < 32) {
-            const int lane = threadIdx.x, nblk = (p.N + Cfg::kTileN - 1) / Cfg::kTileN;
+            const int lane = threadIdx.x;
             int base = 0;
             for (int e0 = 0; e0 < p.E; e0 += 32) {
                 const int e = e0 + lane;
-                int v = e < p.E ? (off[e + 1] - off[e] + Cfg::kTileC - 1) / Cfg::kTileC * nblk : 0;
+                int v = e < p.E ? (off[e + 1] - off[e] + Cfg::kTileC - 1) / Cfg::kTileC : 0;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
                     const int u = __shfl_up_sync(0xffffffffu, v, d);
@@ -152,8 +213,11 @@ __device__ __forceinline__ bool grouped_tables(const GroupedParams& p, int* off,
         // come first, so that what is left to even out at the end is small (5 groups of 2560 uneven rows: 79 -> 69 us with
         // both gradients). Many groups are taken as they come: ordering them would cost more than it evens out.
         const bool sorted = p.E <= 128;
+        const int mean = (off[p.E] - off[0]) / max(1, p.E);
+        int longer = 0;
         for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
             const int rows = off[e + 1] - off[e];
+            longer += sorted && rows > 2 * mean + 64;
             int place = sorted ? 0 : e;
             for (int i = 0; i < (sorted ? p.E : 0); ++i) {
                 const int other = off[i + 1] - off[i];
@@ -161,6 +225,10 @@ __device__ __forceinline__ bool grouped_tables(const GroupedParams& p, int* off,
             }
             first[place] = e;
         }
+        longer = __reduce_add_sync(0xffffffffu, longer);
+        if (threadIdx.x == 0) first[p.E] = 0;
+        __syncthreads();
+        if (sorted && (threadIdx.x & 31) == 0 && longer) atomicAdd(&first[p.E], longer);
     }
     return true;   // the caller synchronises the CTA before the tables are used
 }
@@ -227,8 +295,8 @@ __device__ __forceinline__ void grouped_store(float* dst, long long ld, int cols
 // (Copying B into padded memory first moves it three times, once as writes that take nearly twice as long as reads; see
 // grouped_warps_worthwhile for what was measured.)
 template <int MODE, int VAR>
-__device__ __forceinline__ void grouped_load(const GroupedParams& p, const int* off, const int* first, uint8_t* smem, uint64_t* full_bar,
-                                             uint64_t* empty_bar, int worker, int num_workers, const AbortCtx& ab) {
+__device__ __forceinline__ void grouped_load(const GroupedParams& p, const GroupedTiles<MODE, VAR>& tiles, uint8_t* smem, uint64_t* full_bar,
+                                             uint64_t* empty_bar, const AbortCtx& ab) {
     using Cfg = GroupedCfg<MODE, VAR>;
     constexpr bool kMn = MODE == GR_FWD_MN;
     constexpr int kBatch = 8;
@@ -236,9 +304,9 @@ __device__ __forceinline__ void grouped_load(const GroupedParams& p, const int* 
     // n innermost: 64 k x 16 pieces of 8 n; k innermost: 128 n x 8 pieces of 8 k. This lane's piece of a row, its first row and the step to the next
     constexpr int kPieces = kMn ? 16 : 8, kStep = 64 / kPieces;
     const int c = id % kPieces, r0 = id / kPieces;
-    int it = 0, e = 0;
+    int it = 0;
     GroupedTile g;
-    for (int t = worker; grouped_tile<MODE, VAR>(p, off, first, t, e, g); t += num_workers) {
+    for (int i_tile = 0; tiles.get(i_tile, g); ++i_tile) {
         const uint16_t* b = p.b_src + g.e * p.b_bs;
         for (int kb = 0; kb < g.num_kb; ++kb, ++it) {
             const int s = it % Cfg::kStages;
@@ -321,6 +389,7 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
     uint32_t* abort_slot = tmem_slot + 1;
     int* off = reinterpret_cast<int*>(tmem_slot + 4);
     int* first = off + kMaxGroups + 4;
+    GroupedTile* list = reinterpret_cast<GroupedTile*>((reinterpret_cast<uintptr_t>(first + kMaxGroups + 4) + 15) & ~uintptr_t(15));
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -349,6 +418,8 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
     ptx::grid_dep_launch();
     ptx::grid_dep_wait();
     const bool valid = grouped_tables<MODE, VAR>(p, off, first);
+    __syncthreads();
+    if (valid) grouped_list<MODE, VAR>(p, off, first, list, worker, num_workers);
     ptx::tc_fence_before_sync();
     __syncthreads();
     if constexpr (kPair == 2) ptx::cluster_sync();
@@ -359,6 +430,8 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
         if (warp == 1) ptx::tmem_dealloc<kPair>(tmem_base, Cfg::kTmemCols);
         return;
     }
+
+    const GroupedTiles<MODE, VAR> tiles = {p, off, first, list, worker, num_workers};
 
     // the forms for one CTA and for a pair
     auto load2 = [&](void* dst, const void* map, uint64_t* bar, int owner, int c0, int c1) {
@@ -385,10 +458,10 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
                 ptx::prefetch_tensormap(&maps.p);
                 ptx::prefetch_tensormap(&maps.q[0]);
             }
-            int it = 0, e = 0;
+            int it = 0;
             bool ok = true;
             GroupedTile g;
-            for (int t = worker; ok && grouped_tile<MODE, VAR>(p, off, first, t, e, g); t += num_workers) {
+            for (int i_tile = 0; ok && tiles.get(i_tile, g); ++i_tile) {
                 const int part = g.ncols / kPair;   // columns of this CTA
                 const int n0 = g.n0 + rank * 128;
                 const int c0 = g.c0 + rank * part;
@@ -448,7 +521,7 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer (leader CTA only)
         if (lane == 0 && rank == 0) {
-            int it = 0, lt = 0, e = 0;
+            int it = 0, lt = 0;
             uint32_t fixed_ph = 0;
             bool ok = true;
             GroupedTile g;
@@ -467,15 +540,16 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
                 ptx::tc_fence_after_sync();
                 return true;
             };
-            auto issue = [&](uint32_t d_tmem, int u, int kb, int i) {
+            auto steps_of = [&](int kb) -> int { return Cfg::kGrad && kb == g.num_kb - 1 ? (g.tail + 15) >> 4 : 4; };   // of 16 k
+            auto issue = [&](uint32_t d_tmem, int u, int kb, int i, int steps) {
                 const uint32_t sp = ptx::smem_u32(smem + (i % STAGES) * Cfg::kStageBytes);
                 const uint64_t dp = ptx::make_smem_desc(sp + u * Cfg::kSubBytes, Cfg::kPMn ? 8192 : 16, 1024);
                 const uint64_t dq = ptx::make_smem_desc(sp + Cfg::kPBytes, Cfg::kGrad ? 8192 : 16, 1024);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    ptx::umma<ptx::KIND_F16, kPair>(d_tmem, dp + j * kStepP, dq + j * kStepQ, idesc, (kb | j) ? 1u : 0u);
+                    if (j < steps) ptx::umma<ptx::KIND_F16, kPair>(d_tmem, dp + j * kStepP, dq + j * kStepQ, idesc, (kb | j) ? 1u : 0u);
             };
-            for (int t = worker; ok && grouped_tile<MODE, VAR>(p, off, first, t, e, g); t += num_workers) {
+            for (int i_tile = 0; ok && tiles.get(i_tile, g); ++i_tile) {
                 if (g.num_kb == 0) continue;   // nothing to add up: the epilogue writes zeros
                 idesc = make_instr_desc(1, p.bf16 ? 1 : 0, Cfg::kPMn, Cfg::kGrad, 128 * kPair, g.ncols);
                 if constexpr (kSub == 1) {
@@ -486,7 +560,7 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
                         for (int kb = kb0; kb < kb1 && ok; ++kb) {
                             ok = wait_block(it + kb, kb);
                             if (!ok) break;
-                            issue(tmem_base + acc * Cfg::kTileC, 0, kb - kb0, it + kb);
+                            issue(tmem_base + acc * Cfg::kTileC, 0, kb - kb0, it + kb, steps_of(kb));
                             commit_all(&empty_bar[(it + kb) % STAGES]);
                         }
                         if (ok) commit_all(&tfull_bar[acc]);
@@ -500,7 +574,7 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
                         ptx::tc_fence_after_sync();
                         return true;
                     };
-                    auto both = [&](int u, int kb) { issue(tmem_base + u * Cfg::kTileC, u, kb, it + kb); };
+                    auto both = [&](int u, int kb) { issue(tmem_base + u * Cfg::kTileC, u, kb, it + kb, steps_of(kb)); };
                     ok = wait_drained(0);
                     for (int kb = 0; kb < lead && ok; ++kb) {
                         ok = wait_block(it + kb, kb);
@@ -536,10 +610,10 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
         }
     } else if (Cfg::kGrad && warp == 2 + Cfg::kEpiWarps) {
         // ------------------------------------------------------------ clears the end of ragged blocks (every CTA)
-        int it = 0, e = 0;
+        int it = 0;
         uint32_t tail_ph = 0;
         GroupedTile g;
-        for (int t = worker; grouped_tile<MODE, VAR>(p, off, first, t, e, g); t += num_workers) {
+        for (int i_tile = 0; tiles.get(i_tile, g); ++i_tile) {
             it += g.num_kb;
             if (g.num_kb == 0 || g.tail == 64) continue;
             const int s = (it - 1) % STAGES;
@@ -547,8 +621,9 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
             tail_ph ^= 1u << s;
             uint8_t* sp = smem + s * Cfg::kStageBytes;
             const int boxes = Cfg::kPBytes / 8192 + (g.ncols / kPair > 64 ? 2 : 1);
+            const int end = ((g.tail + 15) & ~15) * 128;   // of the last step of 16 rows that is multiplied
             for (int b = 0; b < boxes; ++b)
-                for (int i = g.tail * 128 + lane * 16; i < 8192; i += 512)
+                for (int i = g.tail * 128 + lane * 16; i < end; i += 512)
                     *reinterpret_cast<uint4*>(sp + b * 8192 + i) = make_uint4(0, 0, 0, 0);
             ptx::fence_proxy_async_smem();
             __syncwarp();
@@ -556,17 +631,17 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
         }
     } else if (Cfg::kWarps && warp >= 2 + Cfg::kEpiWarps) {
         // ------------------------------------------------------------ warps that bring a B which TMA cannot read in place
-        if constexpr (Cfg::kWarps) grouped_load<MODE, VAR>(p, off, first, smem, full_bar, empty_bar, worker, num_workers, ab);
+        if constexpr (Cfg::kWarps) grouped_load<MODE, VAR>(p, tiles, smem, full_bar, empty_bar, ab);
     } else {
         // ------------------------------------------------------------ epilogue (every CTA, its own 128 n): two warps to a quarter of the
         // lanes, each takes every other 32 columns
         const int q = warp & 3, turn = (warp - 2) >> 2;
         const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
         uint8_t* out_tile = out_tiles + (turn * 2 + (q >> 1)) * 4096;
-        int lt = 0, e = 0;
+        int lt = 0;
         bool ok = true;
         GroupedTile g;
-        for (int t = worker; ok && grouped_tile<MODE, VAR>(p, off, first, t, e, g); t += num_workers) {
+        for (int i_tile = 0; ok && tiles.get(i_tile, g); ++i_tile) {
             if constexpr (sizeof(O) == 4) {
                 constexpr int kPieces = Cfg::kTileC / 64;   // of 32 columns for each warp
                 float sums[kPieces][32];
@@ -662,8 +737,8 @@ struct SplitCfg {
     static constexpr int kPartBytes = (VAR == GR_TILE_32 ? 8 : 16) * kUnitBytes;   // an owner's units times the ranks: 4 or 16 units in a tile, 8 ranks
     static constexpr int kThreads = (2 + 8) * 32;
     static constexpr int kTmemCols = 128;
-    static constexpr int kTableBytes = 2 * (kMaxGroups + 4) * 4;
-    static constexpr int kSmemBytes = kStages * kStageBytes + kPartBytes + kTableBytes + (2 * kStages + 1) * 8 + 24 + 1024;
+    static constexpr int kTableBytes = 2 * (kMaxGroups + 4) * 4 + 16;
+    static constexpr int kSmemBytes = kStages * kStageBytes + kPartBytes + kTableBytes + 2048 + (2 * kStages + 1) * 8 + 24 + 1024;
     static_assert(kSmemBytes <= 232448, "shared memory budget exceeded");
 };
 
@@ -682,6 +757,7 @@ grouped_split_kernel(const __grid_constant__ GroupedParams p, const __grid_const
     uint32_t* abort_slot = tmem_slot + 1;
     int* off = reinterpret_cast<int*>(tmem_slot + 4);
     int* first = off + kMaxGroups + 4;
+    GroupedTile* list = reinterpret_cast<GroupedTile*>((reinterpret_cast<uintptr_t>(first + kMaxGroups + 4) + 15) & ~uintptr_t(15));
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -705,6 +781,8 @@ grouped_split_kernel(const __grid_constant__ GroupedParams p, const __grid_const
     ptx::grid_dep_launch();
     ptx::grid_dep_wait();
     const bool valid = grouped_tables<MODE, VAR>(p, off, first);
+    __syncthreads();
+    if (valid) grouped_list<MODE, VAR>(p, off, first, list, worker, num_workers);
     ptx::tc_fence_before_sync();
     __syncthreads();
     ptx::cluster_sync();   // every CTA of the cluster runs before its shared memory is written
@@ -716,10 +794,12 @@ grouped_split_kernel(const __grid_constant__ GroupedParams p, const __grid_const
         return;
     }
 
-    int e = 0, it = 0;
+    int it = 0;
+    const GroupedTiles<MODE, VAR> tiles = {p, off, first, list, worker, num_workers};
+    const long long total = static_cast<long long>(first[p.E]) * ((p.N + 127) / 128);
     uint32_t phase = 0;   // of the accumulator's barrier: it completes once for every tile with k-blocks
     GroupedTile g;
-    for (int t = worker; grouped_tile<MODE, VAR>(p, off, first, t, e, g); t += num_workers) {
+    for (int i_tile = 0; tiles.get(i_tile, g); ++i_tile) {
         const int kb0 = rank * g.num_kb / splits, nkb = (rank + 1) * g.num_kb / splits - kb0;   // this CTA's run, possibly empty
         if (warp == 0) {
             // -------------------------------------------------------- TMA producer
@@ -813,7 +893,7 @@ grouped_split_kernel(const __grid_constant__ GroupedParams p, const __grid_const
                 }
             }
         }
-        if (t + num_workers < first[p.E]) {   // the parts have been read: the next tile may overwrite them
+        if (worker + (i_tile + 1ll) * num_workers < total) {   // the parts have been read: the next tile may overwrite them
             __syncwarp();
             ptx::cluster_sync();
         }
