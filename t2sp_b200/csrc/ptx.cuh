@@ -341,6 +341,13 @@ __device__ __forceinline__ uint32_t map_to_cta(const void* p, uint32_t cta_rank)
     return r;
 }
 
+// True in one lane of the converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(ok));
+    return ok != 0;
+}
+
 // Store to shared memory of a CTA of the cluster (address from map_to_cta); visible to it after a cluster barrier.
 __device__ __forceinline__ void st_cluster(uint32_t cluster_addr, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
