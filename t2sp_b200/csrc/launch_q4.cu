@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
 
     if (warp >= kGemvWarps) {
         // ------------------------------------------------------------ copying warps: each takes every `share`-th slot of one group
-        if (lane != 0) return;
+        if (!ptx::elect_one()) return;
         // a slot stays with one of them (`share` divides `depth`): a wait on the parity of its barrier must not miss a phase
         const int gr = (warp - kGemvWarps) % num_groups, mine = (warp - kGemvWarps) / num_groups;
         int share = kGemvCopiers / num_groups;
