@@ -11,9 +11,9 @@ namespace t2sp {
 constexpr int kMaxGroups = 1024;  // the kernels keep the groups' tables in shared memory
 
 enum : int { GR_FWD_MN = 0, GR_FWD_K = 1, GR_GRAD = 2 };  // B with n innermost, B with k innermost, gradient of B
-// 128 x 128 by one CTA, 256 x 256 and 512 x 256 by a pair, 128 x 32 by one (of a cluster that shares the contraction), 128 x 128 with
+// 128 x 128 by one CTA, 256 x 256 by a pair, 128 x 32 by one (of a cluster that shares the contraction), 128 x 128 with
 // a B that warps bring
-enum : int { GR_TILE_128 = 0, GR_TILE_256 = 1, GR_TILE_512 = 2, GR_TILE_32 = 3, GR_TILE_WARPS = 4 };
+enum : int { GR_TILE_128 = 0, GR_TILE_256 = 1, GR_TILE_32 = 2, GR_TILE_WARPS = 3 };
 enum : int { GR_OUT_F32 = 0, GR_OUT_BF16 = 1, GR_OUT_F16 = 2 };
 
 // Forward: C[t][n] = sum_k A[t][k] * B[e][k][n] for offsets[e] <= t < offsets[e+1]; rows outside every group are not

@@ -36,7 +36,7 @@ template <int MODE, int VAR>
 cudaError_t launch_var(int out, const GroupedParams& p, const GroupedMaps& maps, long long tiles, cudaStream_t stream) {
     const long long slots = core_sm_count() / GroupedCfg<MODE, VAR>::kPair;
     const int workers = static_cast<int>(tiles < slots ? (tiles > 0 ? tiles : 1) : slots);
-    if constexpr (VAR != GR_TILE_512 && VAR != GR_TILE_WARPS)
+    if constexpr (VAR != GR_TILE_WARPS)
         if (out == GR_OUT_F32) return launch_typed<MODE, VAR, float>(p, maps, workers, stream);
     if (out == GR_OUT_BF16) return launch_typed<MODE, VAR, __nv_bfloat16>(p, maps, workers, stream);
     return launch_typed<MODE, VAR, __half>(p, maps, workers, stream);
@@ -83,30 +83,28 @@ long long count_tiles(int mode, const GroupedParams& p, int tn, int tc, bool mos
     return nblk * groups * ((mean + tc - 1) / tc);
 }
 
-// Which tiles: those that need the least time for whole rounds over the SMs. A 512 x 256 tile brings 48 KB a k-block into each SM for twice the products
-// of a 256 x 256 one's 32 KB, which is what bounds long contractions (16384 rows in 8 groups, K = 4096, N = 8192: 766 us against
-// 860), but has no second accumulator to drain under the next tile's products (64 groups of 128 rows, K = 1024, N = 2048: 64 us
-// against 57; gradient with 512 rows a group, 2048 x 2048: 69 against 67). 128 x 128 tiles of single CTAs where the larger ones would leave half the SMs idle
-// (8 groups of 2 rows, 1024 x 1024: 8.8 us against 10.0); the gradient's outputs are too large for that to pay (12.0 against 13.9).
+// Which tiles. 256 x 256 by a pair brings an SM 32 KB a k-block, and its two accumulators let one tile drain under the next one's products.
+// (512 x 256, 48 KB for twice the products but one accumulator, was taken out: 16384 rows in 8 groups, K = 4096, N = 8192: 776 us against 766; gradient
+// with 1024 rows a group, 2048 x 2048: 143 against 120.) 128 x 128 by single CTAs where all of them run at once (1000 rows,
+// 512 x 512: 6.0 us against 8.6; 256 rows, 4096 x 4096: 14.5 against 24.4; the gradient's outputs are too large for that to pay).
+// Of these, clusters share a tile's contraction where that saves more than handing over the sums costs. Measured for 8 tiles, in us with k-blocks: one CTA
+// 4.1 + 0.138 kb; of 2, 4 and 8 CTAs with 32 columns 5.9 + 0.069 kb, 5.5 + 0.034 kb and 5.5 + 0.018 kb, with 128 columns
+// 11.2 + 0.09 kb, 9.3 + 0.046 kb and 8.3 + 0.026 kb.
 template <int MODE>
 cudaError_t launch_mode(int out, const GroupedParams& p, const GroupedMaps& maps, cudaStream_t stream) {
-    if constexpr (MODE != GR_GRAD)
-        if (p.b_src) return launch_var<MODE, GR_TILE_WARPS>(out, p, maps, count_tiles(MODE, p, 128, 128, true), stream);
-    const long long pairs = core_sm_count() / 2;
-    const long long rounds256 = (count_tiles(MODE, p, 256, 256, false) + pairs - 1) / pairs;
-    const long long rounds512 = (count_tiles(MODE, p, 512, 256, false) + pairs - 1) / pairs;
-    const int kb = MODE == GR_GRAD ? p.rows / (p.E * 64) : (p.K + 63) / 64;
-    if (out != GR_OUT_F32 && kb >= (MODE == GR_GRAD ? 12 : 32) && 200 * rounds512 <= 108 * rounds256)
-        return launch_var<MODE, GR_TILE_512>(out, p, maps, count_tiles(MODE, p, 512, 256, true), stream);
     if constexpr (MODE != GR_GRAD) {
+        if (p.b_src) return launch_var<MODE, GR_TILE_WARPS>(out, p, maps, count_tiles(MODE, p, 128, 128, true), stream);
         const long long t128 = count_tiles(MODE, p, 128, 128, false);
+        const int kb = (p.K + 63) / 64;
         const bool narrow = p.rows <= 32ll * p.E;   // about a tile of 32 columns to a group
-        for (int splits = 8; splits >= 2; splits /= 2)
-            if (t128 * splits <= core_sm_count() - (splits == 8 ? 20 : 4) && kb >= 2 * splits &&   // clusters do not fill every GPC
-                (out != GR_OUT_F32 || kb <= 8 * splits))                                             // kRun of the other kernel
+        for (int splits = 8; splits >= 2; splits /= 2) {
+            const int least = narrow ? (splits == 8 ? 12 : splits == 4 ? 16 : 28) : (splits == 8 ? 32 : splits == 4 ? 48 : 128);
+            if (t128 * splits <= core_sm_count() - (splits == 8 ? 20 : 4) && kb >= least &&   // clusters do not fill every GPC
+                (out != GR_OUT_F32 || kb <= 8 * splits))                                       // kRun of the other kernel
                 return narrow ? launch_split<MODE, GR_TILE_32>(out, p, maps, count_tiles(MODE, p, 128, 32, true), splits, stream)
                               : launch_split<MODE, GR_TILE_128>(out, p, maps, count_tiles(MODE, p, 128, 128, true), splits, stream);
-        if (2 * count_tiles(MODE, p, 256, 256, false) <= pairs)
+        }
+        if (t128 <= core_sm_count())
             return launch_var<MODE, GR_TILE_128>(out, p, maps, count_tiles(MODE, p, 128, 128, true), stream);
     }
     return launch_var<MODE, GR_TILE_256>(out, p, maps, count_tiles(MODE, p, 256, 256, true), stream);

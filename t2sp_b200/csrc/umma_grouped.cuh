@@ -3,8 +3,8 @@
 // that a group's ragged end costs an MMA of fewer columns (any multiple of 16, of a pair 32) instead of rows computed in vain, and a
 // weight tile that meets a handful of rows is still fetched at full width.
 //
-//   forward   D[n][t] = sum_k B[e][k][n] A[t][k]       tiles of up to 512 n x up to 256 rows of one group
-//   gradient  D[n][k] = sum_t D[t][n] A[t][k]          tiles of up to 512 n x up to 256 k of one group's matrix; the contraction
+//   forward   D[n][t] = sum_k B[e][k][n] A[t][k]       tiles of up to 256 n x up to 256 rows of one group
+//   gradient  D[n][k] = sum_t D[t][n] A[t][k]          tiles of up to 256 n x up to 256 k of one group's matrix; the contraction
 //                                                      runs over the group's rows, whose last block is ragged
 //
 // The group boundaries are read here, on the device: every CTA loads the offsets, checks them and builds the table of
@@ -23,23 +23,20 @@
 
 namespace t2sp {
 
-// Tile variants: 128 n x 128 columns by one CTA, 256 x 256 by a CTA pair, 512 x 256 by a pair whose CTAs hold two sub-tiles
-// of 128 n each (grouped_launch says when each is taken).
+// Tile variants: 128 n x 128 columns by one CTA, 256 x 256 by a CTA pair (grouped_launch says when each is taken).
 template <int MODE, int VAR>
 struct GroupedCfg {
     static constexpr bool kGrad = MODE == GR_GRAD;
     static constexpr bool kPMn = MODE != GR_FWD_K;           // the MMA's A operand (n) is MN-major
     static constexpr bool kWarps = VAR == GR_TILE_WARPS;
     static constexpr int kPair = VAR == GR_TILE_128 || VAR == GR_TILE_32 || kWarps ? 1 : 2;  // CTAs of a tile
-    static constexpr int kSub = VAR == GR_TILE_512 ? 2 : 1;  // sub-tiles of a CTA
-    static constexpr int kTileN = 128 * kPair * kSub;
+    static constexpr int kTileN = 128 * kPair;
     static constexpr int kTileC = VAR == GR_TILE_32 ? 32 : 128 * kPair;
     // columns come in steps that both CTAs' parts can take: 16 rows of a K-major operand, 64 (a swizzle atom) of an MN-major one
     static constexpr int kColStep = (kGrad ? 64 : 16) * kPair;
-    static constexpr int kAccs = 2;                           // accumulators of kTileC columns: two tiles in turn, or the two sub-tiles
-    static constexpr int kStages = kSub == 2 ? 4 : 6;
-    static constexpr int kSubBytes = 128 * 128;               // 128 n x 64 k
-    static constexpr int kPBytes = kSub * kSubBytes;
+    static constexpr int kAccs = 2;                           // accumulators of kTileC columns, for two tiles in turn
+    static constexpr int kStages = 6;
+    static constexpr int kPBytes = 128 * 128;                 // 128 n x 64 k
     static constexpr int kQBytes = 128 * 128;                 // up to 128 columns x 64 k of one CTA
     static constexpr int kStageBytes = kPBytes + kQBytes;
     static constexpr int kEpiWarps = 8;                       // two for each quarter of the tensor memory's lanes
@@ -370,12 +367,11 @@ template <int MODE, int VAR, class O>
 __global__ void __launch_bounds__(GroupedCfg<MODE, VAR>::kThreads, 1)
 grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ GroupedMaps maps) {
     using Cfg = GroupedCfg<MODE, VAR>;
-    constexpr int STAGES = Cfg::kStages, kPair = Cfg::kPair, kSub = Cfg::kSub;
+    constexpr int STAGES = Cfg::kStages, kPair = Cfg::kPair;
     // k-blocks that are added up in tensor memory before the epilogue takes them. The tensor core cuts its sums off rather than rounding them, about
     // 4e-9 of the result a step of 16 k: nothing to a 16-bit result, but 8e-5 of an fp32 gradient over 65536 rows. For fp32 results
     // the epilogue adds runs of 32 such steps in registers, rounding to nearest (5e-7 at every length).
     constexpr int kRun = sizeof(O) == 4 ? 8 : 1 << 30;
-    static_assert(sizeof(O) == 2 || kSub == 1, "runs need an accumulator to go on with");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* out_tiles = smem + STAGES * Cfg::kStageBytes;
@@ -489,23 +485,18 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
                             ptx::mbar_expect_tx(&full_bar[s], kPair * bytes);
                         }
                         const int row = g.row0 + kb * 64;
-#pragma unroll
-                        for (int u = 0; u < kSub; ++u) {
-                            load3(sp + u * Cfg::kSubBytes, &maps.p, bar, owner, n0 + u * 256, row, 0);
-                            load3(sp + u * Cfg::kSubBytes + 8192, &maps.p, bar, owner, n0 + u * 256 + 64, row, 0);
-                        }
+                        load3(sp, &maps.p, bar, owner, n0, row, 0);
+                        load3(sp + 8192, &maps.p, bar, owner, n0 + 64, row, 0);
                         load2(sq, &maps.q[0], bar, owner, c0, row);
                         if (qboxes == 2) load2(sq + 8192, &maps.q[0], bar, owner, c0 + 64, row);
                     } else {
                         if (rank == 0) ptx::mbar_expect_tx(&full_bar[s], kPair * ((Cfg::kWarps ? 0 : Cfg::kPBytes) + part * 128));
-#pragma unroll
-                        for (int u = 0; u < (Cfg::kWarps ? 0 : kSub); ++u) {
-                            if constexpr (MODE == GR_FWD_MN) {
-                                load3(sp + u * Cfg::kSubBytes, &maps.p, bar, owner, n0 + u * 256, kb * 64, g.e);
-                                load3(sp + u * Cfg::kSubBytes + 8192, &maps.p, bar, owner, n0 + u * 256 + 64, kb * 64, g.e);
-                            } else {
-                                load3(sp + u * Cfg::kSubBytes, &maps.p, bar, owner, kb * 64, n0 + u * 256, g.e);
-                            }
+                        if constexpr (Cfg::kWarps) {
+                        } else if constexpr (MODE == GR_FWD_MN) {
+                            load3(sp, &maps.p, bar, owner, n0, kb * 64, g.e);
+                            load3(sp + 8192, &maps.p, bar, owner, n0 + 64, kb * 64, g.e);
+                        } else {
+                            load3(sp, &maps.p, bar, owner, kb * 64, n0, g.e);
                         }
                         // boxes of 128, 64, 32 and 16 rows: at most three a block (eight boxes of 16 rows kept the thread busy for longer
                         // than the block's MMAs)
@@ -543,9 +534,9 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
                 return true;
             };
             auto steps_of = [&](int kb) -> int { return Cfg::kGrad && kb == g.num_kb - 1 ? (g.tail + 15) >> 4 : 4; };   // of 16 k
-            auto issue = [&](uint32_t d_tmem, int u, int kb, int i, int steps) {
+            auto issue = [&](uint32_t d_tmem, int kb, int i, int steps) {
                 const uint32_t sp = ptx::smem_u32(smem + (i % STAGES) * Cfg::kStageBytes);
-                const uint64_t dp = ptx::make_smem_desc(sp + u * Cfg::kSubBytes, Cfg::kPMn ? 8192 : 16, 1024);
+                const uint64_t dp = ptx::make_smem_desc(sp, Cfg::kPMn ? 8192 : 16, 1024);
                 const uint64_t dq = ptx::make_smem_desc(sp + Cfg::kPBytes, Cfg::kGrad ? 8192 : 16, 1024);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -554,58 +545,17 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
             for (int i_tile = 0; ok && tiles.get(i_tile, g); ++i_tile) {
                 if (g.num_kb == 0) continue;   // nothing to add up: the epilogue writes zeros
                 idesc = make_instr_desc(1, p.bf16 ? 1 : 0, Cfg::kPMn, Cfg::kGrad, 128 * kPair, g.ncols);
-                if constexpr (kSub == 1) {
-                    for (int kb0 = 0; kb0 < g.num_kb && ok; kb0 += kRun, ++lt) {
-                        const int acc = lt & 1, kb1 = min(g.num_kb, kb0 + kRun);
-                        ok = bounded_wait(&tempty_bar[acc], ((lt >> 1) & 1) ^ 1, ab, ST_TIMEOUT_MMA);
-                        ptx::tc_fence_after_sync();
-                        for (int kb = kb0; kb < kb1 && ok; ++kb) {
-                            ok = wait_block(it + kb, kb);
-                            if (!ok) break;
-                            issue(tmem_base + acc * Cfg::kTileC, 0, kb - kb0, it + kb, steps_of(kb));
-                            commit_all(&empty_bar[(it + kb) % STAGES]);
-                        }
-                        if (ok) commit_all(&tfull_bar[acc]);
-                    }
-                } else {
-                    // Both accumulators belong to this tile. Sub-tile 0 runs `lead` k-blocks ahead of sub-tile 1 at both ends of the tile, so that
-                    // its MMAs begin while accumulator 1 is still drained, and its own drain runs under sub-tile 1's last MMAs.
-                    const int n = g.num_kb, lead = min(STAGES - 1, n / 2);
-                    auto wait_drained = [&](int u) -> bool {
-                        if (!bounded_wait(&tempty_bar[u], (lt & 1) ^ 1, ab, ST_TIMEOUT_MMA)) return false;
-                        ptx::tc_fence_after_sync();
-                        return true;
-                    };
-                    auto both = [&](int u, int kb) { issue(tmem_base + u * Cfg::kTileC, u, kb, it + kb, steps_of(kb)); };
-                    ok = wait_drained(0);
-                    for (int kb = 0; kb < lead && ok; ++kb) {
-                        ok = wait_block(it + kb, kb);
-                        if (ok) both(0, kb);
-                    }
-                    ok = ok && wait_drained(1);
-                    for (int kb = 0; kb < lead && ok; ++kb) {
-                        both(1, kb);
-                        commit_all(&empty_bar[(it + kb) % STAGES]);
-                    }
-                    for (int kb = lead; kb < n - lead && ok; ++kb) {
+                for (int kb0 = 0; kb0 < g.num_kb && ok; kb0 += kRun, ++lt) {
+                    const int acc = lt & 1, kb1 = min(g.num_kb, kb0 + kRun);
+                    ok = bounded_wait(&tempty_bar[acc], ((lt >> 1) & 1) ^ 1, ab, ST_TIMEOUT_MMA);
+                    ptx::tc_fence_after_sync();
+                    for (int kb = kb0; kb < kb1 && ok; ++kb) {
                         ok = wait_block(it + kb, kb);
                         if (!ok) break;
-                        both(0, kb);
-                        both(1, kb);
+                        issue(tmem_base + acc * Cfg::kTileC, kb - kb0, it + kb, steps_of(kb));
                         commit_all(&empty_bar[(it + kb) % STAGES]);
                     }
-                    for (int kb = n - lead; kb < n && ok; ++kb) {
-                        ok = wait_block(it + kb, kb);
-                        if (ok) both(0, kb);
-                    }
-                    if (!ok) break;
-                    commit_all(&tfull_bar[0]);
-                    for (int kb = n - lead; kb < n; ++kb) {
-                        both(1, kb);
-                        commit_all(&empty_bar[(it + kb) % STAGES]);
-                    }
-                    commit_all(&tfull_bar[1]);
-                    ++lt;
+                    if (ok) commit_all(&tfull_bar[acc]);
                 }
                 it += g.num_kb;
             }
@@ -680,32 +630,29 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
                         grouped_store(dst + c * p.ldc, p.ldc, g.cols - c, sums[i]);
                     }
             } else {
+                const int acc = lt & 1;
+                const uint32_t parity = (lt >> 1) & 1;
+                const int n = g.n0 + rank * 128 + q * 32;
+                O* dst = static_cast<O*>(p.c) + (MODE == GR_GRAD ? g.e * p.bs_c : 0) + g.c0 * p.ldc + n;
+                if (g.num_kb) {
+                    if (!bounded_wait_warp(&tfull_bar[acc], parity, ab, ST_TIMEOUT_EPILOGUE, lane)) { ok = false; break; }
+                    ptx::tc_fence_after_sync();
+                }
+                const int n64 = n & ~63;   // of the two warps that write together
+                if (n64 < p.N) {
 #pragma unroll 1
-                for (int u = 0; u < kSub; ++u) {
-                    const int acc = kSub == 2 ? u : lt & 1;
-                    const uint32_t parity = kSub == 2 ? lt & 1 : (lt >> 1) & 1;
-                    const int n = g.n0 + u * 256 + rank * 128 + q * 32;
-                    O* dst = static_cast<O*>(p.c) + (MODE == GR_GRAD ? g.e * p.bs_c : 0) + g.c0 * p.ldc + n;
-                    if (g.num_kb) {
-                        if (!bounded_wait_warp(&tfull_bar[acc], parity, ab, ST_TIMEOUT_EPILOGUE, lane)) { ok = false; break; }
-                        ptx::tc_fence_after_sync();
+                    for (int c = turn * 32; c < g.cols; c += 64) {
+                        const uint32_t taddr = lane_base + acc * Cfg::kTileC + c;
+                        grouped_put(taddr, g.num_kb == 0, out_tile, dst + (n64 - n) + c * p.ldc, p.ldc, p.N - n64, g.cols - c, lane, q & 1,
+                                    1 + turn * 2 + (q >> 1));
                     }
-                    const int n64 = n & ~63;   // of the two warps that write together
-                    if (n64 < p.N) {
-#pragma unroll 1
-                        for (int c = turn * 32; c < g.cols; c += 64) {
-                            const uint32_t taddr = lane_base + acc * Cfg::kTileC + c;
-                            grouped_put(taddr, g.num_kb == 0, out_tile, dst + (n64 - n) + c * p.ldc, p.ldc, p.N - n64, g.cols - c, lane, q & 1,
-                                        1 + turn * 2 + (q >> 1));
-                        }
-                    }
-                    if (g.num_kb) {
-                        ptx::tc_fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if constexpr (kPair == 2) ptx::mbar_arrive_peer(&tempty_bar[acc], 0);
-                            else ptx::mbar_arrive(&tempty_bar[acc]);
-                        }
+                }
+                if (g.num_kb) {
+                    ptx::tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if constexpr (kPair == 2) ptx::mbar_arrive_peer(&tempty_bar[acc], 0);
+                        else ptx::mbar_arrive(&tempty_bar[acc]);
                     }
                 }
                 if (g.num_kb) ++lt;
