@@ -34,7 +34,7 @@ struct GroupedParams {
 
 struct GroupedMaps {
     CUtensorMap p;      // B (n, k, e), box 64 x 64, or (k, n, e), box 64 k x 128 n; gradient: D (n, t, 1), box 64 x 64
-    CUtensorMap q[4];   // A: forward (k, t), 64 k x 128, 64, 32 and 16 rows a box; gradient (k, t), 64 k x 64 rows (the first map)
+    CUtensorMap q[4];   // forward: A (k, t), 64 k x 128, 64, 32 and 16 rows a box; gradient: A (k, t), 64 k x 64 rows, then D and A with 16 rows a box
 };
 
 cudaError_t grouped_launch(int mode, int out, const GroupedParams& p, const GroupedMaps& maps, cudaStream_t stream);

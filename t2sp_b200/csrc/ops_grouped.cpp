@@ -83,8 +83,11 @@ int run_grouped(const char* who, int mode, uint32_t type, uint32_t out, GroupedP
         if (int e = fit_operands(vw, in_place ? nullptr : &p_op, &q_op)) return e;
         bool ok = (in_place || encode(&maps.p, type, p_op, 3, 64, mode == GR_FWD_K ? 128 : 64)) &&
                   encode(&maps.q[0], type, q_op, 2, 64, mode == GR_GRAD ? 64 : 128);
-        if (mode != GR_GRAD)
+        if (mode == GR_GRAD) {
+            ok = ok && encode(&maps.q[1], type, p_op, 3, 64, 16) && encode(&maps.q[2], type, q_op, 2, 64, 16);
+        } else {
             for (int b = 1; b < 4; ++b) ok = ok && encode(&maps.q[b], type, q_op, 2, 64, 128 >> b);
+        }
         if (!ok) return tma_unsupported(mode == GR_GRAD ? "A or D" : "A or B");
     }
     const cudaError_t e = grouped_launch(mode, out_kind, p, maps, s);

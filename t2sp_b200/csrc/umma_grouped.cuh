@@ -84,7 +84,7 @@ __device__ __forceinline__ int main_blocks(int extent, int tile) {
 
 // The t-th tile of the call; false when there are no more. Every worker takes every num_workers-th tile.
 //   forward   the groups in turn, each with its main blocks of n; then the narrow last blocks of all groups
-//             (24 groups of 64 rows, 1416 x 776: 22 us when they were dealt out among the others, 13.3 with 1416 x 768)
+//             (24 uneven groups of 73 rows on average, contraction 1416, 776 columns: 20.1 us)
 //   gradient  long groups (grouped_tables) with all their tiles; then the main blocks of the others, their narrow blocks of n, those of k
 template <int MODE, int VAR>
 __device__ bool grouped_tile(const GroupedParams& p, const int* off, const int* first, int t, GroupedTile& g) {
@@ -146,7 +146,7 @@ __device__ bool grouped_tile(const GroupedParams& p, const int* off, const int* 
 }
 
 // The first kListed tiles of a worker, prepared by as many threads at the start: every role goes through the same tiles, and working one out
-// takes 0.2 us (gradient with 24 groups, 576 tiles: XX -> YY us).
+// takes 0.2 us (gradient of 64 groups of 128 rows, 2048 x 1024: 86 -> 67 us).
 constexpr int kListed = 64;
 constexpr int kListBytes = kListed * static_cast<int>(sizeof(GroupedTile));
 template <int MODE, int VAR>
@@ -472,11 +472,12 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
                     uint64_t* bar = &full_bar[s];
                     int owner = 0;
                     if constexpr (MODE == GR_GRAD) {
-                        const int qboxes = part > 64 ? 2 : 1;
-                        const int bytes = Cfg::kPBytes + qboxes * 8192;
-                        if (g.tail < 64 && kb == g.num_kb - 1) {
-                            // ragged block: each CTA's part is credited to its own barrier, for its clearing warp; the
-                            // stage's barrier only keeps its phase
+                        const int qboxes = part > 64 ? 2 : 1, row = g.row0 + kb * 64;
+                        const bool ragged = g.tail < 64 && kb == g.num_kb - 1;
+                        const int steps = ragged ? (g.tail + 15) >> 4 : 4;   // of 16 rows
+                        const int bytes = steps * (2 + qboxes) * 2048;
+                        if (ragged) {
+                            // each CTA's part is credited to its own barrier, for its clearing warp; the stage's barrier only keeps its phase
                             ptx::mbar_expect_tx(&tail_bar[s], bytes);
                             if (rank == 0) ptx::mbar_arrive(&full_bar[s]);
                             bar = &tail_bar[s];
@@ -484,11 +485,19 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
                         } else if (rank == 0) {
                             ptx::mbar_expect_tx(&full_bar[s], kPair * bytes);
                         }
-                        const int row = g.row0 + kb * 64;
-                        load3(sp, &maps.p, bar, owner, n0, row, 0);
-                        load3(sp + 8192, &maps.p, bar, owner, n0 + 64, row, 0);
-                        load2(sq, &maps.q[0], bar, owner, c0, row);
-                        if (qboxes == 2) load2(sq + 8192, &maps.q[0], bar, owner, c0 + 64, row);
+                        if (steps == 4) {
+                            load3(sp, &maps.p, bar, owner, n0, row, 0);
+                            load3(sp + 8192, &maps.p, bar, owner, n0 + 64, row, 0);
+                            load2(sq, &maps.q[0], bar, owner, c0, row);
+                            if (qboxes == 2) load2(sq + 8192, &maps.q[0], bar, owner, c0 + 64, row);
+                        } else {   // only the steps that are multiplied (24 groups of 73 rows, 776 x 1416: 22.9 us, with whole blocks 23.8; of 1 row 21.3 and 23.5)
+                            for (int j = 0; j < steps; ++j) {
+                                load3(sp + j * 2048, &maps.q[1], bar, owner, n0, row + j * 16, 0);
+                                load3(sp + 8192 + j * 2048, &maps.q[1], bar, owner, n0 + 64, row + j * 16, 0);
+                                load2(sq + j * 2048, &maps.q[2], bar, owner, c0, row + j * 16);
+                                if (qboxes == 2) load2(sq + 8192 + j * 2048, &maps.q[2], bar, owner, c0 + 64, row + j * 16);
+                            }
+                        }
                     } else {
                         if (rank == 0) ptx::mbar_expect_tx(&full_bar[s], kPair * ((Cfg::kWarps ? 0 : Cfg::kPBytes) + part * 128));
                         if constexpr (Cfg::kWarps) {
