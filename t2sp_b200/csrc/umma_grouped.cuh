@@ -83,8 +83,8 @@ __device__ __forceinline__ int main_blocks(int extent, int tile) {
 }
 
 // The t-th tile of the call; false when there are no more. Every worker takes every num_workers-th tile.
+// (Gradient of 24 empty groups, 776 x 1416, where some workers had eight full tiles and others five: 17.8 -> 14.9 us, 0.6 of it by the list below.)
 //   forward   the groups in turn, each with its main blocks of n; then the narrow last blocks of all groups
-//             (24 uneven groups of 73 rows on average, contraction 1416, 776 columns: 20.1 us)
 //   gradient  long groups (grouped_tables) with all their tiles; then the main blocks of the others, their narrow blocks of n, those of k
 template <int MODE, int VAR>
 __device__ bool grouped_tile(const GroupedParams& p, const int* off, const int* first, int t, GroupedTile& g) {
