@@ -384,3 +384,31 @@ def test_two_threads_on_their_own_streams(lib):
     assert not errors, errors
     for (a, b, _, off), c in zip(made, outs):
         check_forward(a, b, off, c, False, c)
+
+
+@pytest.mark.parametrize("trans", [False, True])
+def test_more_tiles_than_are_listed(lib, trans):
+    """A worker's tiles beyond the ones it prepares at the start, with a narrow last block of columns: 900 groups of a row, 9 blocks of n."""
+    import torch
+    E, K, N = 900, 8, 2056
+    a, b, _, off = make(E, K, N, [1] * E, torch.bfloat16, trans, 2, 3)
+    c = torch.full((a.shape[0], N), 7.0, dtype=torch.bfloat16, device="cuda")
+    with on_stream():
+        assert t2sp_b200.grouped_gemm(buf(a), buf(b), buf(off), buf(c), GroupedDesc(int(trans))) == 0
+    x, w = a[2:2 + E].double().unsqueeze(1), (b.transpose(1, 2) if trans else b).double()
+    close(c[2:2 + E], torch.bmm(x, w).squeeze(1), torch.bmm(x.abs(), w.abs()).squeeze(1), K)
+    assert (c[:2] == 7).all() and (c[2 + E:] == 7).all()
+
+
+@pytest.mark.parametrize("E", [128, 1000])
+def test_grad_of_many_tiles(lib, E):
+    """The same for the gradient: long and short groups in the order of their rows (up to 128 groups) or as they come, narrow last blocks of n and of k."""
+    import torch
+    K, N = (520, 4104) if E == 128 else (8, 2056)
+    counts = [3 + 11 * (e % 5) for e in range(E)]
+    counts[17], counts[90], counts[91] = 700, 0, 333
+    a, _, d, off = make(E, K, N, counts, torch.bfloat16, False, 1, 2)
+    g = torch.full((E, K, N), float("nan"), dtype=torch.bfloat16, device="cuda")
+    with on_stream():
+        assert t2sp_b200.grouped_gemm_grad(buf(a), buf(d), buf(off), buf(g)) == 0
+    check_grad(a, d, off, g)
