@@ -69,6 +69,7 @@ int run_grouped(const char* who, int mode, uint32_t type, uint32_t out, GroupedP
     cudaStream_t s = rt_stream();
     p.status = rt_status_word();
     p.wait_cycles = rt_env().wait_cycles;
+    p.skip_stage = rt_env().test_skip_stage;
     p.bf16 = type == kBF16;
     if (sync_after) cudaEventRecord(rt_event(0), s);
     GroupedMaps maps;

@@ -97,6 +97,16 @@ __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
 // Named barrier of `threads` threads (whole warps).
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
+// The same; true where `ok` is true in every one of the threads.
+__device__ __forceinline__ bool bar_and(int id, int threads, bool ok) {
+    uint32_t all;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %3, 0;\n bar.red.and.pred q, %1, %2, p;\n selp.b32 %0, 1, 0, q;\n}\n"
+                 : "=r"(all)
+                 : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(ok))
+                 : "memory");
+    return all != 0;
+}
+
 // Generic-proxy writes to shared memory (st.shared) become visible to the async
 // proxy (UMMA operand reads, TMA stores) only after this fence.
 __device__ __forceinline__ void fence_proxy_async_smem() {

@@ -246,8 +246,10 @@ template <> __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(uint32_t l
 // took 5 us to leave, a multiple of its products; 64-byte pieces of one warp: 15 bytes a cycle of the 32 that an SM can write.)
 // UNROLL: rows at a time that are not all aligned; one where such rows are the rule (5 groups of 13 rows, 7552 x 7923, B by warps: 301 -> 272 us).
 // `half`: which warp of the two; `n_left`, `cols`: what exists of the 64 n and of the columns.
+// `ok`: whether this warp's accumulator is complete. Each warp waits for it by itself, and one may give up where the other still succeeds: false in
+// both where it is false in either, so that they leave together and neither meets the barriers alone.
 template <class O, int UNROLL>
-__device__ __forceinline__ void grouped_put(uint32_t taddr, bool zero, uint8_t* tile, O* dst, long long ld, int n_left, int cols, int lane,
+__device__ __forceinline__ bool grouped_put(bool ok, uint32_t taddr, bool zero, uint8_t* tile, O* dst, long long ld, int n_left, int cols, int lane,
                                             int half, int barrier) {
     uint32_t r[2][16];
     if (!zero) {
@@ -258,7 +260,7 @@ __device__ __forceinline__ void grouped_put(uint32_t taddr, bool zero, uint8_t* 
 #pragma unroll
         for (int j = 0; j < 16; ++j) r[0][j] = r[1][j] = 0u;
     }
-    ptx::bar_sync(barrier, 64);   // the tile's previous content has been read
+    if (!ptx::bar_and(barrier, 64, ok)) return false;   // the tile's previous content has been read
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int piece = half * 4 + 2 * h + ((lane >> 3) & 1);
@@ -281,7 +283,7 @@ __device__ __forceinline__ void grouped_put(uint32_t taddr, bool zero, uint8_t* 
             const int col = 16 * half + 4 * i + (lane >> 3);
             *reinterpret_cast<uint4*>(dst + col * ld) = *reinterpret_cast<const uint4*>(tile + col * 128 + ((piece ^ (col & 7)) << 4));
         }
-        return;
+        return true;
     }
 #pragma unroll(UNROLL)
     for (int i = 0; i < 4; ++i) {
@@ -289,6 +291,7 @@ __device__ __forceinline__ void grouped_put(uint32_t taddr, bool zero, uint8_t* 
         const uint4 v = *reinterpret_cast<const uint4*>(tile + col * 128 + ((piece ^ (col & 7)) << 4));
         if (col < cols && piece * 8 < n_left) row16_store(reinterpret_cast<uint16_t*>(dst + col * ld), v, n_left - piece * 8);
     }
+    return true;
 }
 
 // Writes 32 columns of fp32 results: lane = n, one output row (or k) for each column. Each store instruction writes 32 consecutive n.
@@ -479,6 +482,8 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
                     const int s = it % STAGES;
                     const uint32_t ph = (it / STAGES) & 1;
                     if (!bounded_wait(&empty_bar[s], ph ^ 1, ab, ST_TIMEOUT_PRODUCER)) { ok = false; break; }
+                    // Test hook for the bounded waits: without this k-block's copies the roles behind it give up
+                    if (p.skip_stage && it + 1 == p.skip_stage) continue;
                     uint8_t* sp = smem + s * Cfg::kStageBytes;
                     uint8_t* sq = sp + Cfg::kPBytes;
                     uint64_t* bar = &full_bar[s];
@@ -656,7 +661,7 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
                 const int n = g.n0 + rank * 128 + q * 32;
                 O* dst = static_cast<O*>(p.c) + (MODE == GR_GRAD ? g.e * p.bs_c : 0) + g.c0 * p.ldc + n;
                 if (g.num_kb) {
-                    if (!bounded_wait_warp(&tfull_bar[acc], parity, ab, ST_TIMEOUT_EPILOGUE, lane)) { ok = false; break; }
+                    ok = bounded_wait_warp(&tfull_bar[acc], parity, ab, ST_TIMEOUT_EPILOGUE, lane);
                     ptx::tc_fence_after_sync();
                 }
                 const int n64 = n & ~63;   // of the two warps that write together
@@ -664,11 +669,12 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
 #pragma unroll 1
                     for (int c = turn * 32; c < g.cols; c += 64) {
                         const uint32_t taddr = lane_base + acc * Cfg::kTileC + c;
-                        grouped_put<O, Cfg::kWarps ? 1 : 4>(taddr, g.num_kb == 0, out_tile, dst + (n64 - n) + c * p.ldc, p.ldc, p.N - n64, g.cols - c, lane, q & 1,
-                                    1 + turn * 2 + (q >> 1));
+                        ok = grouped_put<O, Cfg::kWarps ? 1 : 4>(ok, taddr, g.num_kb == 0, out_tile, dst + (n64 - n) + c * p.ldc, p.ldc, p.N - n64, g.cols - c,
+                                                                 lane, q & 1, 1 + turn * 2 + (q >> 1));
+                        if (!ok) break;
                     }
                 }
-                if (g.num_kb) {
+                if (ok && g.num_kb) {
                     ptx::tc_fence_before_sync();
                     __syncwarp();
                     if (lane == 0) {
@@ -777,6 +783,7 @@ grouped_split_kernel(const __grid_constant__ GroupedParams p, const __grid_const
                 for (int i = 0; i < nkb; ++i) {
                     const int s = (it + i) % STAGES, kb = kb0 + i;
                     if (!bounded_wait(&empty_bar[s], (((it + i) / STAGES) & 1) ^ 1, ab, ST_TIMEOUT_PRODUCER)) break;
+                    if (p.skip_stage && it + i + 1 == p.skip_stage) continue;   // test hook, as in grouped_kernel
                     uint8_t* sp = smem + s * SplitC::kStageBytes;
                     uint8_t* sq = sp + 128 * 128;
                     ptx::mbar_expect_tx(&full_bar[s], 128 * 128 + g.ncols * 128);

@@ -412,3 +412,31 @@ def test_grad_of_many_tiles(lib, E):
     with on_stream():
         assert t2sp_b200.grouped_gemm_grad(buf(a), buf(d), buf(off), buf(g)) == 0
     check_grad(a, d, off, g)
+
+
+@pytest.mark.parametrize("out", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name,counts,K,N,skip", [
+    ("split", [7], 4096, 128, 3), ("split", [100], 4096, 128, 2), ("single", [600, 400], 512, 512, 3), ("pair", [4000, 96], 512, 1024, 3),
+    ("warps", [10] * 20, 515, 1031, 3), ("grad", [700], 512, 256, 3), ("grad", [40], 512, 256, 1)])
+def test_bounded_waits_run_out(lib, name, counts, K, N, skip, out):
+    """Without the copies of one k-block (a test hook) the waits behind it run out after the shortened limit: every kernel returns by
+    itself, in each of its tile variants, the call reports it, and the next call is right."""
+    import torch
+    from tests.util import library_env
+    a, b, d, off = make(len(counts), K, N, counts, torch.bfloat16)
+    dt = getattr(torch, out)
+    c = torch.zeros(a.shape[0], N, dtype=dt, device="cuda")
+    g = torch.zeros(len(counts), K, N, dtype=dt, device="cuda")
+
+    def call():
+        with on_stream():
+            if name == "grad":
+                return t2sp_b200.grouped_gemm_grad(buf(a), buf(d), buf(off), buf(g))
+            return t2sp_b200.grouped_gemm(buf(a), buf(b), buf(off), buf(c))
+    with library_env(T2SP_B200_WAIT_CYCLES="20000000", T2SP_B200_TEST_SKIP_STAGE=str(skip)):
+        assert call() == -23
+    assert call() == 0
+    if name == "grad":
+        check_grad(a, d, off, g)
+    else:
+        check_forward(a, b, off, c, False, c)
