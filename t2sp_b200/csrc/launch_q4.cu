@@ -8,6 +8,7 @@
 #include "ptx.cuh"
 #include "q4.h"
 #include "row16.cuh"
+#include "umma_core.cuh"
 #include "umma_launch.h"
 
 namespace t2sp {
@@ -304,7 +305,6 @@ constexpr int kGemvThreads = (kGemvWarps + kGemvCopiers) * 32;
 constexpr int kGemvBlocks = 4;                        // blocks of 64 k that a warp computes at a time
 constexpr int kGemvSlot = kGemvBlocks * (512 + 64);   // a warp's share of a slot: its blocks, and up to two groups' scales for each
 constexpr int kGemvMaxShared = 227 << 10;
-constexpr int kGemvTries = 1 << 17;                   // a wait gives up after this many tests of up to 16 us
 
 // Integers: sixteen k of unsigned nibbles against signed bytes of x, exact in 32 bits.
 __device__ __forceinline__ void mma_16832(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -398,7 +398,9 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
     int* units = reinterpret_cast<int*>(smem_raw + lay.units);
     int* idx = reinterpret_cast<int*>(smem_raw + lay.idx);
     uint32_t* top = reinterpret_cast<uint32_t*>(rows + kCols);  // INT: the largest magnitude of each row, as the bits of a float
-    int* count_slot = rows + 2 * kCols;
+    int* count_slot = rows + 2 * kCols;                         // two words, then the CTA's abort flag
+    uint32_t* abort_slot = reinterpret_cast<uint32_t*>(count_slot + 2);
+    const AbortCtx ab{abort_slot, p.status, p.wait_cycles > 0 ? p.wait_cycles : kWaitTimeoutCycles};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int group = warp / gs, wig = warp % gs, num_groups = kGemvWarps / gs;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + lay.bars);   // [group][depth] filled, then [group][depth] free
@@ -409,6 +411,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
             ptx::mbar_init(&bars[num_groups * depth + i], gs);
         }
         ptx::fence_mbar_init();
+        *abort_slot = 0u;
     }
     ptx::grid_dep_launch();
     ptx::grid_dep_wait();
@@ -448,7 +451,6 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
     const long long item_end = items * (blockIdx.x + 1) / gridDim.x;
     const int chunk = gs * kGemvBlocks;                         // blocks of a slot
     const int chunks = (kblocks + chunk - 1) / chunk;           // slots of a strip
-    int tries = kGemvTries;   // a wait that runs out is reported, and the rest of the call's waits do not block (its results are lost)
 
     if (warp >= kGemvWarps) {
         // ------------------------------------------------------------ copying warps: each takes every `share`-th slot of one group
@@ -465,22 +467,22 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
         const int s_full = chunk * 64 / G * 32, s_last = groups * 32 - (chunks - 1) * s_full;
         int turn = 0, slot = 0;          // slots of the group so far, modulo `share` and `depth`
         uint32_t phase = 1;              // the first round finds every slot free
-        while (item < item_end) {
+        int left_out = p.skip_stage;
+        bool ok = true;
+        while (ok && item < item_end) {
             const int unit = static_cast<int>(item / strips);
             const int s_begin = static_cast<int>(item % strips);
             const int s_end = static_cast<int>(min(static_cast<long long>(strips), s_begin + (item_end - item)));
             item += s_end - s_begin;
             const int e = p.index ? idx[units[unit]] : 0;
-            for (int strip = s_begin + gr; strip < s_end; strip += num_groups) {
+            for (int strip = s_begin + gr; ok && strip < s_end; strip += num_groups) {
                 const long long at = static_cast<long long>(e) * strips + strip;
                 const uint8_t* q = p.q + at * kblocks * 512;
                 const uint8_t* s = reinterpret_cast<const uint8_t*>(p.s) + at * groups * 32;
                 for (int c = 1; c <= chunks; ++c, q += q_full, s += s_full) {
-                    if (turn == mine) {
-                        while (!ptx::mbar_try_wait(&freed[slot], phase)) {
-                            if (tries <= 0) break;
-                            if (--tries == 0) atomicOr(p.status, ST_TIMEOUT_PRODUCER);
-                        }
+                    // once a role has given up nothing more is brought: the slots may still be read
+                    if (turn == mine && !(ok = bounded_wait(&freed[slot], phase, ab, ST_TIMEOUT_PRODUCER) && *ab.flag == 0u)) break;
+                    if (--left_out != 0 && turn == mine) {
                         const int qb = c == chunks ? q_last : q_full, sb = c == chunks ? s_last : s_full;
                         uint8_t* dst = ring + slot * slot_bytes;
                         ptx::mbar_expect_tx(&full[slot], qb + sb);
@@ -492,6 +494,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
                 }
             }
         }
+        if (*ab.flag) __nanosleep(200000);   // for the copies on their way: the block's memory is given back when its last thread ends
         return;
     }
 
@@ -500,6 +503,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
     uint64_t* full = bars + group * depth;
     uint64_t* freed = full + num_groups * depth;
     int flip = 0, held = 0;
+    bool live = true;        // false once a wait has run out: it is reported, and the others do not block (the call's results are lost)
     int c_slot = 0;          // next slot to read
     uint32_t c_phase = 0;
 
@@ -700,10 +704,8 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
             for (int kb0 = wig * kGemvBlocks; kb0 < chunks * chunk; kb0 += chunk) {
-                while (!ptx::mbar_try_wait(&full[c_slot], c_phase)) {
-                    if (tries <= 0) break;
-                    if (--tries == 0 && lane == 0) atomicOr(p.status, ST_TIMEOUT_MMA);
-                }
+                if (live && !ptx::mbar_try_wait(&full[c_slot], c_phase)) live = bounded_wait(&full[c_slot], c_phase, ab, ST_TIMEOUT_MMA);
+                __syncwarp();
                 const uint8_t* slot = ring + c_slot * slot_bytes;
                 const uint8_t* blocks = slot + wig * (kGemvBlocks * 512) + lane * 16;
                 const uint8_t* scales = slot + chunk * 512 + wig * (kGemvBlocks * 64 / G * 32) + g * 4;
@@ -754,6 +756,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
             held = 0;
         }
     }
+    if (*ab.flag) __nanosleep(200000);   // as the copying lanes do
 }
 
 // How a call is cut: rows of x that a CTA stages at a time (as many as the instruction's columns and shared memory take; 0 when

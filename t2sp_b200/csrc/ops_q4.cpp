@@ -35,6 +35,8 @@ template <class Launch>
 int run_q4(const char* who, Q4Params& p, bool sync_after, Launch launch) {
     cudaStream_t s = rt_stream();
     p.status = rt_status_word();
+    p.wait_cycles = rt_env().wait_cycles;
+    p.skip_stage = rt_env().test_skip_stage;
     if (sync_after) cudaEventRecord(rt_event(0), s);
     const cudaError_t e = launch(p, s);
     if (e != cudaSuccess) {

@@ -38,6 +38,8 @@ struct Q4Params {
     long long ldy;
     int R, per;           // row r reads row r / per of x
     int out_f32;
+    long long wait_cycles; // limit of every mbarrier wait in SM cycles, 0: kWaitTimeoutCycles
+    int skip_stage;        // test hook for the bounded waits: the copies of this slot of every group of warps are left out (1-based; 0 = none)
     unsigned* status;
 };
 

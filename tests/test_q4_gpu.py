@@ -333,3 +333,25 @@ def test_gemv_infinities_and_nan_of_x(lib, R, dtype):
     if R > 1:
         rows = (~hit).nonzero().flatten()
         check_rows(x[rows], quantised64(w, 64), None, y[rows], 64)
+
+
+@pytest.mark.parametrize("R,E,skip", [(1, 1, 1), (1, 1, 2), (4, 1, 1), (8, 1, 1), (16, 1, 2), (20, 7, 1)])
+def test_gemv_bounded_waits_run_out(lib, R, E, skip):
+    """Without one of the weights' copies (a test hook) the waits for it run out after the shortened limit, the kernel returns by itself, the
+    call reports it, and the next call is right."""
+    import torch
+    from tests.util import library_env
+    K, N, group = 4096, 4096, 64
+    w, x = matrices(E, K, N, torch.bfloat16, 1), matrices(1, R, K, torch.bfloat16, 2)[0]
+    index = [i % E for i in range(R)]
+    idx = torch.tensor(index, dtype=torch.int32, device="cuda") if E > 1 else None
+    y = torch.zeros(R, N, dtype=torch.float32, device="cuda")
+    with on_stream():
+        Q, S = packed(w, group)
+
+        def call():
+            return t2sp_b200.q4_gemv(buf(x), buf(Q), buf(S), buf(idx) if idx is not None else None, buf(y), Q4Desc(group, 0))
+        with library_env(T2SP_B200_WAIT_CYCLES="20000000", T2SP_B200_TEST_SKIP_STAGE=str(skip)):
+            assert call() == -23
+        assert call() == 0
+    check_rows(x, quantised64(w, group), index, y, group)
