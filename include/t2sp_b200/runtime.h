@@ -231,10 +231,10 @@ int t2sp_b200_grouped_gemm_grad(halide_buffer_t *A, halide_buffer_t *D, halide_b
  * of E or more leaves the row as it was and reports halide_error_code_access_out_of_bounds (for asynchronous calls
  * at t2sp_b200_sync). Up to 1024 rows with an index. A row of X is staged in shared memory, which ends K at about 65536
  * (halide_error_code_constraint_violated beyond).
- * Up to four rows to a matrix are multiplied as integers of 31 bits times a power of two of the row: a value of X counts to
- * 2^-31 of its row's largest (values down to 2^-19 of it in f16, 2^-22 in bf16, count exactly), and a row that holds a NaN or an
- * infinity gives NaN. More rows are multiplied in X's type. The results of a row do not depend on the other rows' values, but their last bits
- * do on how many there are. For many rows, q4_unpack and grouped_gemm are faster. */
+ * Every value of X counts exactly: few rows are multiplied as integers of 31 bits times a power of two of the row, more rows, and rows that such
+ * integers do not hold (values below about 2^-22 of the row's largest in bf16; in f16 next to values of 64 and more), in X's
+ * type. Infinities and NaN of X give what their products give. The results of a row do not depend on the other rows' values, but their last
+ * bits do on how many there are. For many rows, q4_unpack and grouped_gemm are faster. */
 typedef struct t2sp_q4_desc {
     int32_t group;   /* 32, 64 or 128; 0 = 64 */
     int32_t trans_b; /* W has k innermost (q4_gemv ignores it) */

@@ -329,9 +329,9 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
 // Two ways to multiply, by the number of rows that share a pass over the weights.
 //   INT  a few rows: the weights stay unsigned nibbles, whose offset 8 the sum of x over the group takes out, and a row of x is written
 //        as 32-bit integers times one power of two, in four signed bytes; each byte is a column of m16n8k32. Two operations turn a word of weights into
-//        operands, half as many instructions as with 16-bit products, and the sums of a group are exact. A value of x is off by at most
-//        2^-31 of its row's largest, where an fp32 sum over the row rounds at 2^-24 of a partial sum at every step; values down to 2^-19
-//        of the largest (bf16: 2^-22) are exact.
+//        operands, half as many instructions as with 16-bit products, and the sums of a group are exact. A row that these integers do not hold
+//        exactly (gemv_wide: a spread of more than about 2^22 in bf16, or values that are not finite) stays in 16 bits instead, and its columns are
+//        computed as below beside the integers of the unit's other rows (1 row x 8192 x 32768, groups of 128, f16: 27.6 us as integers, 39.6 in 16 bits).
 //   else x stays in 16 bits, one column of m16n8k16 a row, with the nibbles as 16-bit numbers (Q4Frag).
 template <int NT, bool INT>
 struct GemvShape {
@@ -367,16 +367,54 @@ struct GemvLayout {
 // within 2^22 added to the bits is one added to the number, so a subtraction turns the sum into a float.
 constexpr int kGemvZero = 0x4b400000;
 
-// The largest power of two f1 * f2 that keeps a row whose largest magnitude has the bits `top` within four signed bytes (at most 127 * 16843009
-// in magnitude); true if the row holds a value that is not finite. Two factors: the power itself may leave fp32's range. Subnormal
-// numbers are taken for 2^-126, where nothing of a 16-bit type needs more.
-__device__ __forceinline__ bool gemv_scale(uint32_t top, float& f1, float& f2) {
-    const bool bad = top >= 0x7f800000u;
-    const int up = bad ? 0 : 30 - max(static_cast<int>(top >> 23) - 127, -126), up1 = up >> 1;
+// The exponent of the largest power of two that keeps a row whose largest magnitude has the bits `top` (finite) within four signed bytes, at most
+// 127 * 16843009 in magnitude: of the 16-bit types' numbers those below 1.9921875 * 2^30. Subnormal numbers are taken for 2^-126, where nothing of a
+// 16-bit type needs more.
+__device__ __forceinline__ int gemv_exponent(uint32_t top) {
+    return 30 - max(static_cast<int>(top >> 23) - 127, -126) - ((top & 0x7fffffu) >= 0x7f0000u ? 1 : 0);
+}
+// That power as two factors: the power itself may leave fp32's range.
+__device__ __forceinline__ void gemv_scale(uint32_t top, float& f1, float& f2) {
+    const int up = gemv_exponent(top), up1 = up >> 1;
     f1 = __uint_as_float(static_cast<uint32_t>(up1 + 127) << 23);
     f2 = __uint_as_float(static_cast<uint32_t>(up - up1 + 127) << 23);
-    if (__uint_as_float(top) * f1 * f2 > 2139062143.f) f2 *= 0.5f;
-    return bad;
+}
+// Whether a row holds a value that is no integer times that power, or that is not finite. `low`: the smallest magnitude of the row that is not 0, as the
+// type's bits less one (0xffff: there is none). A value's last bit counts 2^(its exponent - mantissa bits), and less only in smaller values.
+template <class T>
+__device__ __forceinline__ bool gemv_wide(uint32_t top, uint32_t low) {
+    constexpr int kBits = std::is_same<T, __half>::value ? 10 : 7, kBias = std::is_same<T, __half>::value ? 15 : 127;
+    if (top >= 0x7f800000u) return true;
+    const int last = max(static_cast<int>((low + 1) >> kBits), 1) - kBias - kBits;
+    return low < 0xffffu && last + gemv_exponent(top) < 0;
+}
+
+// `nb` blocks of a slot from block kb0 of the strip on, for rows that stay in 16 bits: row g of the unit is column g of the instruction.
+template <class T, int G>
+__device__ __forceinline__ void gemv_wide_slot(float (&acc)[4], const uint8_t* x, const uint8_t* blocks, const uint8_t* scales, int kb0, int nb) {
+    float c[4];
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < kGemvBlocks; ++u) {
+        if (u >= nb) break;
+        const uint4 q = *reinterpret_cast<const uint4*>(blocks + u * 512);
+        const uint4 b[2] = {*reinterpret_cast<const uint4*>(x + (kb0 + u) * 128), *reinterpret_cast<const uint4*>(x + (kb0 + u) * 128 + 16)};
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            uint32_t a[4];
+            Q4Frag<T>::expand((&q.x)[s], a);
+            const uint32_t b0 = (&b[s >> 1].x)[2 * (s & 1)], b1 = (&b[s >> 1].x)[2 * (s & 1) + 1];
+            if ((s == 0 && (G != 128 || u % 2 == 0)) || (G == 32 && s == 2)) mma_16816<T>(c, a, b0, b1, zero);
+            else mma_16816<T>(c, a, b0, b1, c);
+            if ((s == 3 && (G != 128 || u % 2 == 1 || u + 1 == nb)) || (G == 32 && s == 1)) {
+                const float2 f = pair_f32<T>(*reinterpret_cast<const uint32_t*>(scales + (G == 32 ? u * 2 + (s >> 1) : (G == 64 ? u : u >> 1)) * 32));
+                acc[0] += f.x * c[0];
+                acc[1] += f.x * c[1];
+                acc[2] += f.y * c[2];
+                acc[3] += f.y * c[3];
+            }
+        }
+    }
 }
 
 // Y[r] = X[r / per] x W[index[r]]. Work items are (unit, strip of 16 n), where a unit is up to `unit_rows` rows that name one matrix:
@@ -397,7 +435,8 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
     int* rows = reinterpret_cast<int*>(smem_raw + lay.rows);
     int* units = reinterpret_cast<int*>(smem_raw + lay.units);
     int* idx = reinterpret_cast<int*>(smem_raw + lay.idx);
-    uint32_t* top = reinterpret_cast<uint32_t*>(rows + kCols);  // INT: the largest magnitude of each row, as the bits of a float
+    uint32_t* top = reinterpret_cast<uint32_t*>(rows + kCols);  // INT: the largest magnitude of each row, as the bits of a float, ...
+    uint32_t* low = top + S::kRows;                             // ... then the smallest that is not 0, as the type's bits less one
     int* count_slot = rows + 2 * kCols;                         // two words, then the CTA's abort flag
     uint32_t* abort_slot = reinterpret_cast<uint32_t*>(count_slot + 2);
     const AbortCtx ab{abort_slot, p.status, p.wait_cycles > 0 ? p.wait_cycles : kWaitTimeoutCycles};
@@ -503,7 +542,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
     uint64_t* full = bars + group * depth;
     uint64_t* freed = full + num_groups * depth;
     int flip = 0, held = 0;
-    bool live = true;        // false once a wait has run out: it is reported, and the others do not block (the call's results are lost)
+    bool live = true;        // false once a wait has run out: it is reported, and the others test once only (the call's results are lost)
     int c_slot = 0;          // next slot to read
     uint32_t c_phase = 0;
 
@@ -532,7 +571,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
                 for (int i = lane; i < found; i += 32) rows[i] = lead + i;
             }
             if (lane == 0) *count_slot = found;
-            if (lane < kCols) top[lane] = 0u;
+            if (lane < kCols) top[lane] = lane < S::kRows ? 0u : 0xffffu;
         }
         ptx::bar_sync(15, kGemvWarps * 32);
         const int count = *count_slot;
@@ -569,7 +608,14 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
                 uint32_t m = max_abs2<T>(max_abs2<T>(max_abs2<T>(max_abs2<T>(0u, v.x), v.y), v.z), v.w);
                 const float2 f = pair_f32<T>(max_abs2<T>(m, __byte_perm(m, m, 0x1032)));
                 const uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(f.x) & 0x7fffffffu);   // a NaN's bits are above infinity's
-                if (lane == 0) atomicMax(&top[i / runs], b);
+                uint32_t l = 0xffffffffu;   // of each half the magnitude less one, of a zero 0xffff
+#pragma unroll
+                for (int j = 0; j < 4; ++j) l = __vminu2(l, (((&v.x)[j] & 0x7fff7fffu) + 0x7fff7fffu) ^ 0x80008000u);
+                l = __reduce_min_sync(0xffffffffu, min(l & 0xffffu, l >> 16));
+                if (lane == 0) {
+                    atomicMax(&top[i / runs], b);
+                    atomicMin(&low[i / runs], l);
+                }
             };
 #pragma unroll
             for (int n = 0; n < kKeep; ++n)
@@ -577,19 +623,32 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
             rest(look);
             ptx::bar_sync(15, kGemvWarps * 32);
         }
+        uint32_t wide = 0;   // INT: rows that stay in 16 bits
+        if constexpr (INT)
+#pragma unroll
+            for (int r = 0; r < S::kRows; ++r) wide |= static_cast<uint32_t>(gemv_wide<T>(top[r], low[r])) << r;   // not of a row that is not there
+        auto halves = [&](uint8_t* column, int k8, const uint4& v) {   // in the order j = 0, 2, 1, 3 of the weights' pairs
+            uint8_t* dst = column + (k8 >> 3) * 128 + (k8 & 1) * 64 + ((k8 >> 1) & 3) * 8;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(__byte_perm(v.x, v.y, 0x5410), __byte_perm(v.x, v.y, 0x7632));
+            *reinterpret_cast<uint2*>(dst + 32) = make_uint2(__byte_perm(v.z, v.w, 0x5410), __byte_perm(v.z, v.w, 0x7632));
+        };
         auto place = [&](int i, const uint4& v) {
             const int row = i / runs, k8 = (i - row * runs) * 32 + lane;
             const bool real = k8 < pieces;
             // k = 16 w + 4 t + j of block k8 / 8: w = (k8 % 8) / 2, t = 2 (k8 % 2) and the next
             if constexpr (INT) {
+                if (wide >> row & 1) {   // in the place of its four columns of bytes
+                    if (real) halves(smem_raw + row * 4 * lay.pitch, k8, v);
+                    return;
+                }
                 float f1, f2;
-                const bool bad = gemv_scale(top[row], f1, f2);
+                gemv_scale(top[row], f1, f2);
                 const float2 a = pair_f32<T>(v.x), b = pair_f32<T>(v.y), c = pair_f32<T>(v.z), d = pair_f32<T>(v.w);
                 const float f[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
                 // x + 0x80808080 as an unsigned number: its bytes less 128 are the signed bytes
                 uint32_t u[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) u[j] = (bad ? 0u : static_cast<uint32_t>(__float2int_rn(f[j] * f1 * f2))) + 0x80808080u;
+                for (int j = 0; j < 8; ++j) u[j] = static_cast<uint32_t>(__float2int_rn(f[j] * f1 * f2)) + 0x80808080u;
                 int sums[4];
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
@@ -617,10 +676,8 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
                     *reinterpret_cast<int4*>(xi + (k8 / kLanes) * kCols + row * 4) =
                         make_int4(kGemvZero - 8 * s0, kGemvZero - 8 * ((lo - s0) >> 16), kGemvZero - 8 * s2, kGemvZero - 8 * ((hi - s2) >> 16));
                 }
-            } else if (real) {   // in the order j = 0, 2, 1, 3 of the weights' pairs
-                uint8_t* dst = smem_raw + row * lay.pitch + (k8 >> 3) * 128 + (k8 & 1) * 64 + ((k8 >> 1) & 3) * 8;
-                *reinterpret_cast<uint2*>(dst) = make_uint2(__byte_perm(v.x, v.y, 0x5410), __byte_perm(v.x, v.y, 0x7632));
-                *reinterpret_cast<uint2*>(dst + 32) = make_uint2(__byte_perm(v.z, v.w, 0x5410), __byte_perm(v.z, v.w, 0x7632));
+            } else if (real) {
+                halves(smem_raw + row * lay.pitch, k8, v);
             }
         };
 #pragma unroll
@@ -700,60 +757,79 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
                 }
             }
         };
-        for (int strip = s_begin + group; strip < s_end; strip += num_groups) {
+        // the unit's strips; `mixed`: some of its rows stay in 16 bits (a loop of its own: tests and a call in the other one cost it 1 to 4 %)
+        auto strips_of_unit = [&](auto mixed) {
+            for (int strip = s_begin + group; strip < s_end; strip += num_groups) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-            for (int kb0 = wig * kGemvBlocks; kb0 < chunks * chunk; kb0 += chunk) {
-                if (live && !ptx::mbar_try_wait(&full[c_slot], c_phase)) live = bounded_wait(&full[c_slot], c_phase, ab, ST_TIMEOUT_MMA);
-                __syncwarp();
-                const uint8_t* slot = ring + c_slot * slot_bytes;
-                const uint8_t* blocks = slot + wig * (kGemvBlocks * 512) + lane * 16;
-                const uint8_t* scales = slot + chunk * 512 + wig * (kGemvBlocks * 64 / G * 32) + g * 4;
-                if (kb0 + kGemvBlocks <= kblocks) compute(std::true_type(), blocks, scales, kb0, kGemvBlocks);
-                else if (kb0 < kblocks) compute(std::false_type(), blocks, scales, kb0, kblocks - kb0);
-                __syncwarp();   // every lane has read the slot
-                if (lane == 0) ptx::mbar_arrive(&freed[c_slot]);
-                if (++c_slot == depth) { c_slot = 0; c_phase ^= 1u; }
-            }
-            float* mine = part + ((flip * S::kFlush + held) * kGemvWarps + warp) * 16 * S::kPartPitch;
+                for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+                float wide_acc[4];   // of rows 2 t and 2 t + 1
+                if constexpr (mixed.value) wide_acc[0] = wide_acc[1] = wide_acc[2] = wide_acc[3] = 0.f;
+                for (int kb0 = wig * kGemvBlocks; kb0 < chunks * chunk; kb0 += chunk) {
+                    if (!ptx::mbar_try_wait(&full[c_slot], c_phase) && live) live = bounded_wait(&full[c_slot], c_phase, ab, ST_TIMEOUT_MMA);
+                    __syncwarp();
+                    const uint8_t* slot = ring + c_slot * slot_bytes;
+                    const uint8_t* blocks = slot + wig * (kGemvBlocks * 512) + lane * 16;
+                    const uint8_t* scales = slot + chunk * 512 + wig * (kGemvBlocks * 64 / G * 32) + g * 4;
+                    const bool any = !mixed.value || wide != (1u << count) - 1u;   // a row of integers
+                    if (any && kb0 + kGemvBlocks <= kblocks) compute(std::true_type(), blocks, scales, kb0, kGemvBlocks);
+                    else if (any && kb0 < kblocks) compute(std::false_type(), blocks, scales, kb0, kblocks - kb0);
+                    if constexpr (mixed.value)
+                        if (kb0 < kblocks)
+                            gemv_wide_slot<T, G>(wide_acc, smem_raw + (g < count ? g : 0) * 4 * lay.pitch + t * 32, blocks, scales, kb0, min(kGemvBlocks, kblocks - kb0));
+                    __syncwarp();   // every lane has read the slot
+                    if (lane == 0) ptx::mbar_arrive(&freed[c_slot]);
+                    if (++c_slot == depth) { c_slot = 0; c_phase ^= 1u; }
+                }
+                float* mine = part + ((flip * S::kFlush + held) * kGemvWarps + warp) * 16 * S::kPartPitch;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                if constexpr (INT) {
-                    // bytes 0, 1 of a row in the lanes with even t, bytes 2, 3 in the next lanes
+                for (int n = 0; n < NT; ++n) {
+                    if constexpr (INT) {
+                        // bytes 0, 1 of a row in the lanes with even t, bytes 2, 3 in the next lanes
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float v = acc[n][2 * h] + 256.f * acc[n][2 * h + 1];
-                        const float v2 = __shfl_xor_sync(0xffffffffu, v, 1);
-                        if (t % 2 == 0) mine[(g + 8 * h) * S::kPartPitch + n * 2 + (t >> 1)] = v + 65536.f * v2;
+                        for (int h = 0; h < 2; ++h) {
+                            const float v = acc[n][2 * h] + 256.f * acc[n][2 * h + 1];
+                            const float v2 = __shfl_xor_sync(0xffffffffu, v, 1);
+                            if (t % 2 == 0 && !(mixed.value && (wide >> (n * 2 + (t >> 1)) & 1))) mine[(g + 8 * h) * S::kPartPitch + n * 2 + (t >> 1)] = v + 65536.f * v2;
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) mine[(g + (j >> 1) * 8) * S::kPartPitch + n * 8 + 2 * t + (j & 1)] = acc[n][j];
                     }
-                } else {
+                }
+                if constexpr (mixed.value)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) mine[(g + (j >> 1) * 8) * S::kPartPitch + n * 8 + 2 * t + (j & 1)] = acc[n][j];
-                }
-            }
-            if (++held < S::kFlush && strip + num_groups < s_end) continue;
-            ptx::bar_sync(1 + group, gs * 32);
-            // two buffers in turn: this one is written again only after the barrier of the next flush
-            for (int i = wig * 32 + lane; i < held * 16 * count; i += gs * 32) {
-                const int n = i & 15, col = (i >> 4) % count, f = (i >> 4) / count;
-                const float* from = part + ((flip * S::kFlush + f) * kGemvWarps + group * gs) * 16 * S::kPartPitch + n * S::kPartPitch + col;
-                float v = 0.f;
+                    for (int j = 0; j < 4; ++j)
+                        if (wide >> (2 * t + (j & 1)) & 1) mine[(g + 8 * (j >> 1)) * S::kPartPitch + 2 * t + (j & 1)] = wide_acc[j];
+                if (++held < S::kFlush && strip + num_groups < s_end) continue;
+                ptx::bar_sync(1 + group, gs * 32);
+                // two buffers in turn: this one is written again only after the barrier of the next flush
+                for (int i = wig * 32 + lane; i < held * 16 * count; i += gs * 32) {
+                    const int n = i & 15, col = (i >> 4) % count, f = (i >> 4) / count;
+                    const float* from = part + ((flip * S::kFlush + f) * kGemvWarps + group * gs) * 16 * S::kPartPitch + n * S::kPartPitch + col;
+                    float v = 0.f;
 #pragma unroll 4
-                for (int w = 0; w < gs; ++w) v += from[w * 16 * S::kPartPitch];
-                if constexpr (INT) {
-                    float f1, f2;
-                    const bool bad = gemv_scale(top[col], f1, f2);
-                    v = bad ? __int_as_float(0x7fc00000) : v * (1.f / f1) * (1.f / f2);   // powers of two
+                    for (int w = 0; w < gs; ++w) v += from[w * 16 * S::kPartPitch];
+                    if constexpr (INT) {
+                        float f1, f2;
+                        gemv_scale(top[col], f1, f2);
+                        if (!(mixed.value && (wide >> col & 1))) v = v * (1.f / f1) * (1.f / f2);   // powers of two
+                    }
+                    const int n_at = (strip - (held - 1 - f) * num_groups) * 16 + n;
+                    if (n_at < p.N) {
+                        const long long at = rows[col] * p.ldy + n_at;
+                        if (p.out_f32) static_cast<float*>(p.y)[at] = v;
+                        else static_cast<T*>(p.y)[at] = rounded<T>(v);
+                    }
                 }
-                const int n_at = (strip - (held - 1 - f) * num_groups) * 16 + n;
-                if (n_at < p.N) {
-                    const long long at = rows[col] * p.ldy + n_at;
-                    if (p.out_f32) static_cast<float*>(p.y)[at] = v;
-                    else static_cast<T*>(p.y)[at] = rounded<T>(v);
-                }
+                flip ^= 1;
+                held = 0;
             }
-            flip ^= 1;
-            held = 0;
+        };
+        if constexpr (INT) {
+            if (wide) strips_of_unit(std::true_type());
+            else strips_of_unit(std::false_type());
+        } else {
+            strips_of_unit(std::false_type());
         }
     }
     if (*ab.flag) __nanosleep(200000);   // as the copying lanes do

@@ -355,3 +355,76 @@ def test_gemv_bounded_waits_run_out(lib, R, E, skip):
             assert call() == -23
         assert call() == 0
     check_rows(x, quantised64(w, group), index, y, group)
+
+
+def spread_rows(R, K, dtype, seed=2):
+    """Rows of x whose even ones hold a value so large, at k = 5, that 31 bits from it down do not reach the others."""
+    import torch
+    x = matrices(1, R, K, dtype, seed)[0]
+    x[::2] *= 2.0 ** -30 if dtype == torch.bfloat16 else 2.0 ** -11
+    x[::2, 5] = 1000.0 if dtype == torch.bfloat16 else 60000.0
+    return x
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("R,K,N,group", [(1, 448, 48, 64), (2, 300, 33, 32), (2, 1000, 70, 128), (3, 192, 40, 64), (4, 448, 48, 32), (4, 700, 48, 128), (8, 448, 48, 64),
+                                         (4, 7500, 24, 64), (4, 8192, 24, 64), (1, 30000, 20, 64), (1, 33000, 20, 64), (5, 65, 17, 128)])
+def test_gemv_large_values_that_meet_zeros(lib, R, K, N, group, dtype):
+    """Where the row's largest value meets a zero of W, the others are the whole result: it is as exact as any. Both sides of the lengths
+    up to which a few rows are held as integers (4 rows: about 7900 values, 1 row: about 31000). Rows beside are the same to the bit."""
+    import torch
+    dt = getattr(torch, dtype)
+    w = matrices(1, K, N, dt, 1)
+    w[0, 5, ::2] = 0
+    x = spread_rows(R, K, dt)
+    plain = x.clone()
+    plain[::2] = matrices(1, R, K, dt, 5)[0][::2]
+    y, z = (torch.empty(R, N, dtype=torch.float32, device="cuda") for _ in range(2))
+    with on_stream():
+        Q, S = packed(w, group)
+        assert t2sp_b200.q4_gemv(buf(x), buf(Q), buf(S), None, buf(y), Q4Desc(group, 0)) == 0
+        assert t2sp_b200.q4_gemv(buf(plain), buf(Q), buf(S), None, buf(z), Q4Desc(group, 0)) == 0
+    check_rows(x, quantised64(w, group), None, y, group)
+    check_rows(plain, quantised64(w, group), None, z, group)
+    assert torch.equal(y[1::2], z[1::2])
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_gemv_large_values_by_expert(lib, dtype):
+    import torch
+    dt = getattr(torch, dtype)
+    E, T, per, K, N, group = 5, 7, 2, 320, 50, 64
+    w, x = matrices(E, K, N, dt, 1), spread_rows(T, K, dt)
+    w[:, 5, ::2] = 0
+    index = [3, 1, 3, 3, -1, 0, 3, 4, 3, 3, 2, 1, 1, 0]
+    idx = torch.tensor(index, dtype=torch.int32, device="cuda")
+    y = torch.full((T * per, N), 7.0, dtype=torch.float32, device="cuda")   # the large products leave f16
+    with on_stream():
+        Q, S = packed(w, group)
+        assert t2sp_b200.q4_gemv(buf(x), buf(Q), buf(S), buf(idx), buf(y), Q4Desc(group, 0)) == 0
+    check_rows(x, quantised64(w, group), index, y, group, torch.full_like(y, 7.0))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("R,K", [(1, 192), (2, 192), (4, 320), (8, 192), (4, 8192), (1, 33000)])
+def test_gemv_infinities_of_x_follow_the_products(lib, R, K, dtype):
+    """inf * q is an infinity of q's sign, and NaN where q is 0; infinities of both signs give NaN; the other rows are as ever."""
+    import torch
+    dt = getattr(torch, dtype)
+    w, x = matrices(1, K, 40, dt, 1), matrices(1, R, K, dt, 2)[0]
+    x[0, 100] = float("inf")
+    if R > 1:
+        x[1, 7], x[1, 90] = -float("inf"), float("inf")
+    if R > 3:
+        x[3, 3] = float("nan")
+    y = torch.empty(R, 40, dtype=torch.float32, device="cuda")
+    values = quantised64(w, 64)
+    with on_stream():
+        Q, S = packed(w, 64)
+        assert t2sp_b200.q4_gemv(buf(x), buf(Q), buf(S), None, buf(y), Q4Desc(64, 0)) == 0
+    for r in range(R):
+        want = (x[r].double()[:, None] * values[0]).sum(0)
+        if x[r].isfinite().all():
+            check_rows(x[r:r + 1], values, None, y[r:r + 1], 64)
+        else:
+            assert not want.isfinite().any() and torch.equal(y[r].double().nan_to_num(7.0, 8.0, 9.0), want.nan_to_num(7.0, 8.0, 9.0))
