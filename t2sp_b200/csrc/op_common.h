@@ -227,10 +227,14 @@ int check_capture(const char* who, bool waits, bool scratch) {
     return halide_error_code_constraint_violated;
 }
 
-// A device copy of an output that the call writes only in part starts from the caller's values.
+// An output that the call writes only in part starts from the caller's values: a device copy of host memory, and a device
+// allocation whose host side is the newer one.
 int preload_output(halide_buffer_t* b, DeviceView* v) {
-    if (v->borrowed || v->preloaded || v->bytes == 0) return 0;
-    if (cudaMemcpyAsync(v->ptr, b->host, v->bytes, cudaMemcpyHostToDevice, rt_stream()) != cudaSuccess) {
+    if (v->preloaded || v->bytes == 0) return 0;
+    if (v->borrowed && !((b->flags & 1u) && b->host)) return 0;
+    const bool ok = v->borrowed ? rt_move_buffer(b, false)
+                                : cudaMemcpyAsync(v->ptr, b->host, v->bytes, cudaMemcpyHostToDevice, rt_stream()) == cudaSuccess;
+    if (!ok) {
         cudaGetLastError();
         return halide_error_code_copy_to_device_failed;
     }

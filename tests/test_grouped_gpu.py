@@ -440,3 +440,41 @@ def test_bounded_waits_run_out(lib, name, counts, K, N, skip, out):
         check_grad(a, d, off, g)
     else:
         check_forward(a, b, off, c, False, c)
+
+
+@pytest.mark.parametrize("name", ["grouped_gemm", "grouped_gemm_grad", "q4_gemv"])
+def test_newer_host_values_of_a_resident_output_stay(lib, name):
+    """An output with a device allocation whose host side was changed (host_dirty): what the call does not write comes back from
+    copy_to_host as the host had it."""
+    import torch
+    from t2sp_b200 import Buffer, Q4Desc
+    from tests.device_util import packed
+    a, b, d, off = make(2, 64, 48, [5, 4], torch.bfloat16, before=2, behind=3)
+    w = b.contiguous()
+    M, K, N = a.shape[0], 64, 48
+    shape = {"grouped_gemm": (M, N + 8), "grouped_gemm_grad": (2, K + 2, N + 8), "q4_gemv": (M, N)}[name]
+    out = np.zeros(shape, np.float32)
+    C = Buffer.from_numpy(out)
+    assert lib.t2sp_b200_device_malloc(C.ptr) == 0 and lib.t2sp_b200_copy_to_device(C.ptr) == 0
+    out[:] = 7.0
+    C.raw.flags |= 1   # host_dirty
+    with on_stream():
+        if name == "grouped_gemm":
+            rc = t2sp_b200.grouped_gemm(buf(a), buf(b), buf(off), C)
+        elif name == "grouped_gemm_grad":
+            rc = t2sp_b200.grouped_gemm_grad(buf(a), buf(d), buf(off), C)
+        else:
+            Q, S = packed(w, 64)
+            index = torch.tensor([-1, 0, 1, -1] + [0] * (M - 4), dtype=torch.int32, device="cuda")
+            rc = t2sp_b200.q4_gemv(buf(a), buf(Q), buf(S), buf(index), C, Q4Desc(64, 0))
+    assert rc == 0 and not C.raw.flags & 1
+    assert lib.t2sp_b200_copy_to_host(C.ptr) == 0 and lib.t2sp_b200_device_free(C.ptr) == 0
+    got = torch.from_numpy(out).cuda()
+    if name == "grouped_gemm":
+        check_forward(a, b, off, got[:, :N], False, torch.full_like(got, 7.0)[:, :N])
+        assert (got[:, N:] == 7).all()
+    elif name == "grouped_gemm_grad":
+        check_grad(a, d, off, got[:, :K, :N])
+        assert (got[:, K:] == 7).all() and (got[:, :, N:] == 7).all()
+    else:
+        assert (got[[0, 3]] == 7).all() and not (got[[1, 2, 4]] == 7).any()
