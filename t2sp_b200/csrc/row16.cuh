@@ -5,9 +5,11 @@
 
 namespace t2sp {
 
-__device__ __forceinline__ uint4 load16_stream(const void* p) {
+// An ordinary load: some of the kernels that call this start while the kernel before still writes what they are about to read, and a load through the
+// read-only path is defined only for memory that nobody writes while the kernel runs, from its start on.
+__device__ __forceinline__ uint4 load16(const void* p) {
     uint4 v;
-    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
 
@@ -29,10 +31,10 @@ __device__ __forceinline__ uint4 row16_cut(const uint4& a, const uint4& b, int m
 __device__ __forceinline__ uint4 row16_load(const uint16_t* src, int left, const uint16_t* begin, const uint16_t* end) {
     const int m = static_cast<int>(reinterpret_cast<uintptr_t>(src) & 15) >> 1;
     const uint16_t* base = src - m;
-    if (left >= 8 && m == 0) return load16_stream(src);
+    if (left >= 8 && m == 0) return load16(src);
     uint4 v = make_uint4(0, 0, 0, 0);
     if (left >= 8 && base >= begin && base + 16 <= end) {
-        const uint4 a = load16_stream(base), b = load16_stream(base + 8);
+        const uint4 a = load16(base), b = load16(base + 8);
         return row16_cut(a, b, m);
     }
 #pragma unroll

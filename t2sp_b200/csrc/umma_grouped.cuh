@@ -342,8 +342,8 @@ __device__ __forceinline__ void grouped_load(const GroupedParams& p, const Group
                     for (int j = 0; j < kBatch; ++j) {
                         const uint16_t* at = src + min(r0 + (i + j) * kStep, rows - 1) * p.b_ld;
                         const uint16_t* base = reinterpret_cast<const uint16_t*>(reinterpret_cast<uintptr_t>(at) & ~uintptr_t(15));
-                        lo[j] = load16_stream(base);
-                        hi[j] = load16_stream(base + 8);
+                        lo[j] = load16(base);
+                        hi[j] = load16(base + 8);
                     }
 #pragma unroll
                     for (int j = 0; j < kBatch; ++j) {

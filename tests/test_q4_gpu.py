@@ -428,3 +428,43 @@ def test_gemv_infinities_of_x_follow_the_products(lib, R, K, dtype):
             check_rows(x[r:r + 1], values, None, y[r:r + 1], 64)
         else:
             assert not want.isfinite().any() and torch.equal(y[r].double().nan_to_num(7.0, 8.0, 9.0), want.nan_to_num(7.0, 8.0, 9.0))
+
+
+@pytest.mark.parametrize("rows,K,N,pad", [(1, 256, 512, 0), (8, 256, 512, 3), (160, 515, 1031, 0)])
+def test_results_of_one_call_are_the_next_ones_operand(lib, rows, K, N, pad):
+    """Asynchronous calls on one stream, each reading at once what the one before writes: rows for q4_gemv, B with rows off 16 bytes
+    for the grouped product. Two sets of inputs in turn, so that what an earlier round left would show; equal to synchronous calls."""
+    import torch
+    from tests.device_util import packed as pack
+    dt = torch.bfloat16
+    E, group = 8, 64
+    sets = [matrices(1, rows, K, dt, s)[0] for s in (1, 2)]
+    ds = [matrices(1, rows, N, dt, s)[0] for s in (3, 4)]
+    w, b = matrices(1, N, 96, dt, 5), matrices(E, K, N, dt, 6, K ** -0.5)
+    off = torch.tensor([i * rows // E for i in range(E + 1)], dtype=torch.int32, device="cuda")
+    mid = torch.zeros(rows, N + pad, dtype=dt, device="cuda")[:, :N]
+    g = torch.zeros(E, K, N, dtype=dt, device="cuda")
+    out = torch.zeros(rows, N, dtype=dt, device="cuda")
+    y = torch.zeros(rows, 96, dtype=torch.float32, device="cuda")
+
+    def chain(i, L=None):
+        assert t2sp_b200.grouped_gemm_grad(buf(sets[i]), buf(ds[i]), buf(off), buf(g)) == 0
+        assert t2sp_b200.grouped_gemm(buf(sets[1 - i]), buf(g), buf(off), buf(out)) == 0
+        assert t2sp_b200.grouped_gemm(buf(sets[i]), buf(b), buf(off), buf(mid)) == 0
+        assert t2sp_b200.q4_gemv(buf(mid), buf(Q), buf(S), None, buf(y), Q4Desc(group, 0)) == 0
+    with on_stream():
+        Q, S = pack(w, group)
+        want = []
+        for i in (0, 1):
+            chain(i)
+            want.append([t.clone() for t in (g, out, mid, y)])
+        check_rows(want[1][2], quantised64(w, group), None, want[1][3], group)
+    keep = []
+    with on_stream(asynchronous=True) as L:
+        for n in range(40):
+            chain(n % 2)
+            if n >= 30:
+                keep.append((n % 2, [t.clone() for t in (g, out, mid, y)]))
+        assert L.t2sp_b200_sync() == 0
+    for i, got in keep:
+        assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
