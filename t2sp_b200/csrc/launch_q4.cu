@@ -576,7 +576,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
         ptx::bar_sync(15, kGemvWarps * 32);
         const int count = *count_slot;
         // x in pieces of 8 k, a warp's 32 pieces of one row at a time; the first ones stay in registers between the two looks at them
-        const int pieces = kblocks * 8, runs = (pieces + 31) / 32, total = count * runs;
+        const int pieces = kblocks * 8, runs = max(1, (pieces + 31) / 32), total = count * runs;   // of no k: one run without pieces
         constexpr int kLanes = G / 8;                                   // lanes that hold a group
         constexpr int kKeep = INT ? 4 : 8;
         auto piece = [&](int i) -> uint4 {

@@ -468,3 +468,19 @@ def test_results_of_one_call_are_the_next_ones_operand(lib, rows, K, N, pad):
         assert L.t2sp_b200_sync() == 0
     for i, got in keep:
         assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
+
+
+@pytest.mark.parametrize("R,indexed", [(1, False), (2, True), (5, False), (17, True)])
+def test_gemv_of_no_k(lib, R, indexed):
+    """K = 0: the sums are empty, the results zeros, in every form of the product; a row without a matrix is left as it was."""
+    import torch
+    N, E = 24, 2 if indexed else 1
+    y = torch.full((R, N), 7.0, dtype=torch.float32, device="cuda")
+    index = torch.tensor([(i % 3) - 1 for i in range(R)], dtype=torch.int32, device="cuda")
+    X = Buffer((0, R), "f16", host=y.data_ptr())       # nothing of an empty operand is read
+    Q = Buffer((512, 0, 2, E), "u8", host=y.data_ptr())
+    S = Buffer((16, 0, 2, E), "f16", host=y.data_ptr())
+    with on_stream():
+        assert t2sp_b200.q4_gemv(X, Q, S, buf(index) if indexed else None, buf(y), Q4Desc(32, 0)) == 0
+    left = (index < 0) if indexed else torch.zeros(R, dtype=torch.bool, device="cuda")
+    assert (y[left] == 7).all() and not y[~left].any()
