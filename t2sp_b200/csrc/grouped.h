@@ -15,6 +15,8 @@ enum : int { GR_FWD_MN = 0, GR_FWD_K = 1, GR_GRAD = 2 };  // B with n innermost,
 // a B that warps bring
 enum : int { GR_TILE_128 = 0, GR_TILE_256 = 1, GR_TILE_32 = 2, GR_TILE_WARPS = 3 };
 enum : int { GR_OUT_F32 = 0, GR_OUT_BF16 = 1, GR_OUT_F16 = 2 };
+// k-blocks of 64 whose products are added up in tensor memory at a time (see grouped_kernel)
+__host__ __device__ constexpr int grouped_run(int out) { return out == GR_OUT_F32 ? 8 : (out == GR_OUT_BF16 ? 1024 : 128); }
 
 // Forward: C[t][n] = sum_k A[t][k] * B[e][k][n] for offsets[e] <= t < offsets[e+1]; rows outside every group are not
 // touched. Gradient of B: G[e][k][n] = sum_{t in e} A[t][k] * D[t][n], zero for an empty group.

@@ -8,10 +8,10 @@ namespace t2sp {
 
 namespace {
 
-template <int MODE, int VAR, class O>
+template <int MODE, int VAR, class O, bool LONG>
 cudaError_t launch_typed(const GroupedParams& p, const GroupedMaps& maps, int workers, cudaStream_t stream) {
     using Cfg = GroupedCfg<MODE, VAR>;
-    auto kern = grouped_kernel<MODE, VAR, O>;
+    auto kern = grouped_kernel<MODE, VAR, O, LONG>;
     static std::atomic<bool> configured[kMaxDev];
     if (cudaError_t e = allow_smem(kern, Cfg::kSmemBytes, configured)) return e;
     cudaLaunchConfig_t cfg = {};
@@ -32,14 +32,14 @@ cudaError_t launch_typed(const GroupedParams& p, const GroupedMaps& maps, int wo
     return cudaLaunchKernelEx(&cfg, kern, p, maps);
 }
 
-template <int MODE, int VAR>
+template <int MODE, int VAR, bool LONG = false>
 cudaError_t launch_var(int out, const GroupedParams& p, const GroupedMaps& maps, long long tiles, cudaStream_t stream) {
     const long long slots = core_sm_count() / GroupedCfg<MODE, VAR>::kPair;
     const int workers = static_cast<int>(tiles < slots ? (tiles > 0 ? tiles : 1) : slots);
     if constexpr (VAR != GR_TILE_WARPS)
-        if (out == GR_OUT_F32) return launch_typed<MODE, VAR, float>(p, maps, workers, stream);
-    if (out == GR_OUT_BF16) return launch_typed<MODE, VAR, __nv_bfloat16>(p, maps, workers, stream);
-    return launch_typed<MODE, VAR, __half>(p, maps, workers, stream);
+        if (out == GR_OUT_F32) return launch_typed<MODE, VAR, float, false>(p, maps, workers, stream);
+    if (out == GR_OUT_BF16) return launch_typed<MODE, VAR, __nv_bfloat16, LONG>(p, maps, workers, stream);
+    return launch_typed<MODE, VAR, __half, LONG>(p, maps, workers, stream);
 }
 
 template <int MODE, int VAR, class O>
@@ -83,6 +83,10 @@ long long count_tiles(int mode, const GroupedParams& p, int tn, int tc, bool mos
     return nblk * groups * ((mean + tc - 1) / tc);
 }
 
+// Whether a 16-bit result's contraction (of the gradient: the rows of all groups together) may be longer than a run. (The LONG form of the kernel costs
+// the gradient of 64 groups of 256 rows, 2048 x 1024, 6 % where no group is: 206 -> 218 us.)
+bool is_long(int mode, int out, const GroupedParams& p) { return out != GR_OUT_F32 && (mode == GR_GRAD ? p.rows : p.K) > 64 * grouped_run(out); }
+
 // Which tiles. 256 x 256 by a pair brings an SM 32 KB a k-block, and its two accumulators let one tile drain under the next one's products.
 // (512 x 256, 48 KB for twice the products but one accumulator, was taken out: 16384 rows in 8 groups, K = 4096, N = 8192: 776 us against 766; gradient
 // with 1024 rows a group, 2048 x 2048: 143 against 120.) 128 x 128 by single CTAs where all of them run at once (1000 rows,
@@ -92,6 +96,7 @@ long long count_tiles(int mode, const GroupedParams& p, int tn, int tc, bool mos
 // 11.2 + 0.09 kb, 9.3 + 0.046 kb and 8.3 + 0.026 kb.
 template <int MODE>
 cudaError_t launch_mode(int out, const GroupedParams& p, const GroupedMaps& maps, cudaStream_t stream) {
+    const bool runs = is_long(MODE, out, p);
     if constexpr (MODE != GR_GRAD) {
         if (p.b_src) return launch_var<MODE, GR_TILE_WARPS>(out, p, maps, count_tiles(MODE, p, 128, 128, true), stream);
         const long long t128 = count_tiles(MODE, p, 128, 128, false);
@@ -100,14 +105,17 @@ cudaError_t launch_mode(int out, const GroupedParams& p, const GroupedMaps& maps
         for (int splits = 8; splits >= 2; splits /= 2) {
             const int least = narrow ? (splits == 8 ? 12 : splits == 4 ? 16 : 28) : (splits == 8 ? 32 : splits == 4 ? 48 : 128);
             if (t128 * splits <= core_sm_count() - (splits == 8 ? 20 : 4) && kb >= least &&   // clusters do not fill every GPC
-                (out != GR_OUT_F32 || kb <= 8 * splits))                                       // kRun of the other kernel
+                kb <= grouped_run(out) * splits)                                               // no longer runs than in the other kernel
                 return narrow ? launch_split<MODE, GR_TILE_32>(out, p, maps, count_tiles(MODE, p, 128, 32, true), splits, stream)
                               : launch_split<MODE, GR_TILE_128>(out, p, maps, count_tiles(MODE, p, 128, 128, true), splits, stream);
         }
-        if (t128 <= core_sm_count())
-            return launch_var<MODE, GR_TILE_128>(out, p, maps, count_tiles(MODE, p, 128, 128, true), stream);
+        if (t128 <= core_sm_count()) {
+            const long long tiles = count_tiles(MODE, p, 128, 128, true);
+            return runs ? launch_var<MODE, GR_TILE_128, true>(out, p, maps, tiles, stream) : launch_var<MODE, GR_TILE_128>(out, p, maps, tiles, stream);
+        }
     }
-    return launch_var<MODE, GR_TILE_256>(out, p, maps, count_tiles(MODE, p, 256, 256, true), stream);
+    const long long tiles = count_tiles(MODE, p, 256, 256, true);
+    return runs ? launch_var<MODE, GR_TILE_256, true>(out, p, maps, tiles, stream) : launch_var<MODE, GR_TILE_256>(out, p, maps, tiles, stream);
 }
 
 __global__ void __launch_bounds__(256) repack16_kernel(const Repack a, const Repack b) {
@@ -137,7 +145,7 @@ cudaError_t grouped_launch(int mode, int out, const GroupedParams& p, const Grou
 // the warps read B again for every tile (250 rows, 1001 x 2001: 54 against 44), and with few tiles they cannot keep the memory busy while the
 // copy lets a cluster share a tile (2 tiles, K = 5378: 60 against 15).
 bool grouped_warps_worthwhile(int mode, int out, const GroupedParams& p) {
-    if (mode == GR_GRAD || out == GR_OUT_F32 || p.rows == 0 || p.E == 0) return false;
+    if (mode == GR_GRAD || out == GR_OUT_F32 || p.rows == 0 || p.E == 0 || is_long(mode, out, p)) return false;
     const long long groups = p.rows < p.E ? p.rows : p.E;
     return p.rows <= 128 * groups && 3 * count_tiles(mode, p, 128, 128, false) >= 2 * core_sm_count();
 }

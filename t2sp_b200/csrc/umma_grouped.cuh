@@ -230,6 +230,10 @@ __device__ __forceinline__ bool grouped_tables(const GroupedParams& p, int* off,
     return true;   // the caller synchronises the CTA before the tables are used
 }
 
+template <class O> __device__ __forceinline__ O grouped_round(float v);
+template <> __device__ __forceinline__ float grouped_round<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half grouped_round<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 grouped_round<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <class O> __device__ __forceinline__ uint32_t pack16(uint32_t lo, uint32_t hi);
 template <> __device__ __forceinline__ uint32_t pack16<__half>(uint32_t lo, uint32_t hi) {
     const __half2 v = __floats2half2_rn(__uint_as_float(lo), __uint_as_float(hi));
@@ -294,11 +298,12 @@ __device__ __forceinline__ bool grouped_put(bool ok, uint32_t taddr, bool zero, 
     return true;
 }
 
-// Writes 32 columns of fp32 results: lane = n, one output row (or k) for each column. Each store instruction writes 32 consecutive n.
-__device__ __forceinline__ void grouped_store(float* dst, long long ld, int cols, const float (&r)[32]) {
+// Writes 32 columns of results from fp32 sums: lane = n, one output row (or k) for each column. Each store instruction writes 32 consecutive n.
+template <class O>
+__device__ __forceinline__ void grouped_store(O* dst, long long ld, int cols, const float (&r)[32]) {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-        if (j < cols) dst[j * ld] = r[j];
+        if (j < cols) dst[j * ld] = grouped_round<O>(r[j]);
 }
 
 // The blocks of a B whose rows do not start on 16 bytes, brought by two warps for each stage of the ring (a stage stays with its warps: a wait on
@@ -378,15 +383,18 @@ __device__ __forceinline__ void grouped_load(const GroupedParams& p, const Group
     }
 }
 
-template <int MODE, int VAR, class O>
+template <int MODE, int VAR, class O, bool LONG>
 __global__ void __launch_bounds__(GroupedCfg<MODE, VAR>::kThreads, 1)
 grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ GroupedMaps maps) {
     using Cfg = GroupedCfg<MODE, VAR>;
     constexpr int STAGES = Cfg::kStages, kPair = Cfg::kPair;
-    // k-blocks that are added up in tensor memory before the epilogue takes them. The tensor core cuts its sums off rather than rounding them, about
-    // 4e-9 of the result a step of 16 k: nothing to a 16-bit result, but 8e-5 of an fp32 gradient over 65536 rows. For fp32 results
-    // the epilogue adds runs of 32 such steps in registers, rounding to nearest (5e-7 at every length).
-    constexpr int kRun = sizeof(O) == 4 ? 8 : 1 << 30;
+    // k-blocks that are added up in tensor memory before the epilogue takes them. The tensor core cuts its sums off rather than rounding them: a step of
+    // 16 k takes about 4e-9 of the result where signs are mixed (8e-5 of an fp32 gradient over 65536 rows) and 1.1e-7 where all products are positive
+    // (7e-3 of a gradient over 2^20 rows). For fp32 results the epilogue adds runs of 32 steps in registers, rounding to nearest (5e-7 at every length, 2.7e-6 of positive products); for
+    // 16-bit ones, in the LONG form that longer contractions take, runs of 512 steps (f16) or 4096 (bf16): about 5.5e-5 and 4.4e-4 of positive products, a
+    // ninth of what the rounding to that type does. In the gradient each tile goes by its own group's rows.
+    constexpr bool kRuns = sizeof(O) == 4 || LONG;
+    constexpr int kRun = kRuns ? grouped_run(sizeof(O) == 4 ? GR_OUT_F32 : (std::is_same<O, __half>::value ? GR_OUT_F16 : GR_OUT_BF16)) : 1 << 30;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* out_tiles = smem + STAGES * Cfg::kStageBytes;
@@ -620,42 +628,45 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
         bool ok = true;
         GroupedTile g;
         for (int i_tile = 0; ok && tiles.get(i_tile, g); ++i_tile) {
-            if constexpr (sizeof(O) == 4) {
-                constexpr int kPieces = Cfg::kTileC / 64;   // of 32 columns for each warp
-                float sums[kPieces][32];
+            constexpr bool kPuts = sizeof(O) == 2 && (!LONG || MODE == GR_GRAD);
+            if (kRuns && (!kPuts || g.num_kb > kRun)) {
+                if constexpr (kRuns) {
+                    constexpr int kPieces = Cfg::kTileC / 64;   // of 32 columns for each warp
+                    float sums[kPieces][32];
 #pragma unroll
-                for (int i = 0; i < kPieces; ++i)
+                    for (int i = 0; i < kPieces; ++i)
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) sums[i][j] = 0.f;
-                for (int kb = 0; kb < g.num_kb && ok; kb += kRun, ++lt) {
-                    const int acc = lt & 1;
-                    ok = bounded_wait_warp(&tfull_bar[acc], (lt >> 1) & 1, ab, ST_TIMEOUT_EPILOGUE, lane);
-                    if (!ok) break;
-                    ptx::tc_fence_after_sync();
+                        for (int j = 0; j < 32; ++j) sums[i][j] = 0.f;
+                    for (int kb = 0; kb < g.num_kb && ok; kb += kRun, ++lt) {
+                        const int acc = lt & 1;
+                        ok = bounded_wait_warp(&tfull_bar[acc], (lt >> 1) & 1, ab, ST_TIMEOUT_EPILOGUE, lane);
+                        if (!ok) break;
+                        ptx::tc_fence_after_sync();
 #pragma unroll
-                    for (int i = 0; i < kPieces; ++i) {
-                        uint32_t r[32];
-                        ptx::tmem_ld_32x32(lane_base + acc * Cfg::kTileC + turn * 32 + i * 64, r);
-                        ptx::tmem_ld_wait();
+                        for (int i = 0; i < kPieces; ++i) {
+                            uint32_t r[32];
+                            ptx::tmem_ld_32x32(lane_base + acc * Cfg::kTileC + turn * 32 + i * 64, r);
+                            ptx::tmem_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) sums[i][j] += __uint_as_float(r[j]);
+                            for (int j = 0; j < 32; ++j) sums[i][j] += __uint_as_float(r[j]);
+                        }
+                        ptx::tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if constexpr (kPair == 2) ptx::mbar_arrive_peer(&tempty_bar[acc], 0);
+                            else ptx::mbar_arrive(&tempty_bar[acc]);
+                        }
                     }
-                    ptx::tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if constexpr (kPair == 2) ptx::mbar_arrive_peer(&tempty_bar[acc], 0);
-                        else ptx::mbar_arrive(&tempty_bar[acc]);
-                    }
+                    const int n = g.n0 + rank * 128 + q * 32 + lane;
+                    O* dst = static_cast<O*>(p.c) + (MODE == GR_GRAD ? g.e * p.bs_c : 0) + g.c0 * p.ldc + n;
+                    if (ok && n < p.N)
+#pragma unroll
+                        for (int i = 0; i < kPieces; ++i) {
+                            const int c = turn * 32 + i * 64;
+                            grouped_store(dst + c * p.ldc, p.ldc, g.cols - c, sums[i]);
+                        }
                 }
-                const int n = g.n0 + rank * 128 + q * 32 + lane;
-                float* dst = static_cast<float*>(p.c) + (MODE == GR_GRAD ? g.e * p.bs_c : 0) + g.c0 * p.ldc + n;
-                if (ok && n < p.N)
-#pragma unroll
-                    for (int i = 0; i < kPieces; ++i) {
-                        const int c = turn * 32 + i * 64;
-                        grouped_store(dst + c * p.ldc, p.ldc, g.cols - c, sums[i]);
-                    }
-            } else {
+            } else if constexpr (kPuts) {
                 const int acc = lt & 1;
                 const uint32_t parity = (lt >> 1) & 1;
                 const int n = g.n0 + rank * 128 + q * 32;
@@ -864,9 +875,7 @@ grouped_split_kernel(const __grid_constant__ GroupedParams p, const __grid_const
                 for (int k = 1; k < splits; ++k) v += part[k * 1024];
                 if (n < p.N) {
                     O* dst = static_cast<O*>(p.c) + (g.c0 + col) * p.ldc + n;
-                    if constexpr (sizeof(O) == 4) *dst = v;
-                    else if constexpr (std::is_same<O, __half>::value) *dst = __float2half_rn(v);
-                    else *dst = __float2bfloat16_rn(v);
+                    *dst = grouped_round<O>(v);
                 }
             }
         }

@@ -478,3 +478,81 @@ def test_newer_host_values_of_a_resident_output_stay(lib, name):
         assert (got[:, K:] == 7).all() and (got[:, :, N:] == 7).all()
     else:
         assert (got[[0, 3]] == 7).all() and not (got[[1, 2, 4]] == 7).any()
+
+
+def long_tolerance(ref):
+    """All products positive. Beside the final rounding to f16 (2^-11): runs of 512 steps, each of which cuts off less than 2^-23 of the sum
+    (2^-14), and fewer than 512 sums of runs or parts in fp32 (2^-15), relative. One sum over 2^17 rows would be 8e-4 low, over 2^20 7e-3."""
+    return ref * (2.0 ** -11 + 2.0 ** -14 + 2.0 ** -15) * (1 + 2.0 ** -11)
+
+
+def positive(seed, *shape):
+    import torch
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return (torch.rand(*shape, generator=g, device="cuda") * 0.1 + 0.1).half()
+
+
+def test_long_f16_gradient(lib):
+    """A group of 2^20 rows, an empty one, one of 40 rows and one of 2^17."""
+    import torch
+    counts = [(1 << 20) + 37, 0, 40, 1 << 17]
+    rows = sum(counts)
+    a, d = positive(3, rows, 72), positive(4, rows, 88)
+    off = torch.tensor(np.concatenate([[0], np.cumsum(counts)]), dtype=torch.int32, device="cuda")
+    out = torch.empty(4, 72, 88, dtype=torch.float16, device="cuda")
+    with on_stream():
+        assert t2sp_b200.grouped_gemm_grad(buf(a), buf(d), buf(off), buf(out)) == 0
+    o = off.tolist()
+    for e in (0, 2, 3):
+        ref = sum(a[i:min(o[e + 1], i + 65536)].double().T @ d[i:min(o[e + 1], i + 65536)].double() for i in range(o[e], o[e + 1], 65536))
+        assert ((out[e].double() - ref).abs() <= long_tolerance(ref)).all(), e
+    assert not out[1].any()
+
+
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("counts,K,N", [([5, 0, 30], 140000, 40), ([3, 300], 131085, 300), ([20], 60000, 136), ([2000, 3000], 131072, 1032)])
+def test_long_f16_contractions(lib, counts, K, N, trans):
+    """Few tiles (with the contraction shared by a cluster up to 65536 k), and many."""
+    import torch
+    E, M = len(counts), sum(counts) + 3
+    a, b = positive(5, M, K), positive(6, E, *((N, K) if trans else (K, N)))
+    off = torch.tensor(1 + np.concatenate([[0], np.cumsum(counts)]), dtype=torch.int32, device="cuda")
+    c = torch.full((M, N), 7.0, dtype=torch.float16, device="cuda")
+    with on_stream():
+        assert t2sp_b200.grouped_gemm(buf(a), buf(b), buf(off), buf(c), GroupedDesc(int(trans))) == 0
+    o = off.tolist()
+    for e in range(E):
+        if counts[e]:
+            w = b[e].T if trans else b[e]
+            ref = sum(a[o[e]:o[e + 1], k:k + 16384].double() @ w[k:k + 16384].double() for k in range(0, K, 16384))
+            assert ((c[o[e]:o[e + 1]].double() - ref).abs() <= long_tolerance(ref)).all(), e
+    assert (c[:1] == 7).all() and (c[o[-1]:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("counts,K,N", [([5, 0, 30], 8200, 1040), ([3, 300] * 20, 8193, 300), ([700, 900], 16500, 1100)])
+def test_contractions_of_some_runs(lib, counts, K, N, trans, dtype):
+    import torch
+    dt = getattr(torch, dtype)
+    a, b, d, off = make(len(counts), K, N, counts, dt, trans, 1, 2)
+    a, b = a * 2.0 ** -6, b * 2.0 ** -6
+    for out in (dt, torch.float32):
+        c = torch.full((a.shape[0], N), 7.0, dtype=out, device="cuda")
+        with on_stream():
+            assert t2sp_b200.grouped_gemm(buf(a), buf(b), buf(off), buf(c), GroupedDesc(int(trans))) == 0
+        check_forward(a, b, off, c, trans, torch.full_like(c, 7.0))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_grad_of_long_and_short_groups(lib, dtype):
+    """Groups of more and of fewer rows than a run, ragged and empty ones, in one call."""
+    import torch
+    dt = getattr(torch, dtype)
+    counts = [9000, 0, 8192, 8193, 40, 17000, 1, 640] if dtype == "float16" else [70000, 0, 65536, 65537, 40, 140000, 1, 640]
+    a, _, d, off = make(len(counts), 200, 264, counts, dt, False, 3, 5)
+    g = torch.full((len(counts), 200, 264), float("nan"), dtype=dt, device="cuda")
+    with on_stream():
+        assert t2sp_b200.grouped_gemm_grad(buf(a), buf(d), buf(off), buf(g)) == 0
+    check_grad(a, d, off, g)
