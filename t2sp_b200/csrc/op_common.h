@@ -181,7 +181,7 @@ int check_min0(const Arg& a) {
 
 // Outer strides that address memory forwards; for an output also without two coordinates on one element.
 int check_strides(const Arg& a) {
-    int64_t reach = 1;   // elements that the dimensions so far span, in the order of their strides
+    int64_t reach = 1;   // elements from the first to behind the last that the dimensions so far address, in the order of their strides
     int order[8], n = 0;
     for (int d = 0; d < a.b->dimensions; ++d)
         if (a.b->dim[d].extent == 0) return 0;
@@ -195,7 +195,7 @@ int check_strides(const Arg& a) {
             return constraint(v.c_str(), a.b->dim[order[i]].stride, a.is_output ? "at least the elements it strides over" : "positive",
                               static_cast<int>(std::min<int64_t>(reach, 0x7fffffff)));
         }
-        reach = std::max(reach, stride * a.b->dim[order[i]].extent);
+        reach += stride * (a.b->dim[order[i]].extent - 1);
     }
     return 0;
 }

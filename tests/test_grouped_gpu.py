@@ -556,3 +556,21 @@ def test_grad_of_long_and_short_groups(lib, dtype):
     with on_stream():
         assert t2sp_b200.grouped_gemm_grad(buf(a), buf(d), buf(off), buf(g)) == 0
     check_grad(a, d, off, g)
+
+
+def test_matrices_of_an_output_that_interlock(lib):
+    """G's rows have a pitch, and a matrix begins where the last row of the one before ends: in device and in host memory."""
+    import torch
+    from t2sp_b200 import Buffer
+    a, _, d, off = make(3, 40, 24, [10, 0, 70], torch.bfloat16)
+    big = torch.full((3 * (39 * 32 + 24) + 8,), 5.0, dtype=torch.float32, device="cuda")
+    g = big.as_strided((3, 40, 24), (39 * 32 + 24, 32, 1))
+    host = big.cpu().numpy().copy()
+    with on_stream():
+        assert t2sp_b200.grouped_gemm_grad(buf(a), buf(d), buf(off), buf(g)) == 0
+        G = Buffer((24, 40, 3), "f32", host=host.ctypes.data, strides=(1, 32, 39 * 32 + 24), keepalive=host)
+        assert t2sp_b200.grouped_gemm_grad(buf(a), buf(d), buf(off), G) == 0
+    check_grad(a, d, off, g)
+    assert torch.equal(torch.from_numpy(host).cuda(), big)
+    g.fill_(5.0)
+    assert (big == 5).all()

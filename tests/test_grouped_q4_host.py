@@ -215,3 +215,12 @@ def test_q4_bounds_queries_of_products_and_reading(lib):
         assert t2sp_b200.q4_unpack(a["Q"], a["S"], w, Q4Desc(32, trans)) == 0
         assert [e for _, e, _ in w.shape()] == ([128, 48, 2] if trans else [48, 128, 2]) and w.raw.type.bits == 16
     assert t2sp_b200.q4_pack(Buffer.query(3), Buffer.query(4), Buffer.query(4)) == -34
+
+
+def test_output_strides_of_matrices_that_interlock(lib):
+    """An output's matrices may begin where the last row of the one before ends, not only a whole pitch later."""
+    near, over = strided((24, 16, 3), (1, 32, 15 * 32 + 24), "f32"), strided((24, 16, 3), (1, 32, 15 * 32 + 23), "f32")
+    assert grad(G=over) == -8
+    if no_device():
+        assert grad(G=near) == -36
+        assert t2sp_b200.q4_unpack(q4_args()["Q"], q4_args()["S"], strided((40, 100, 2), (1, 48, 99 * 48 + 40)), Q4Desc(32, 0)) == -36
