@@ -208,6 +208,16 @@ int check_extent_limit(const Arg& a) {
     return 0;
 }
 
+// The buffers of a bounds query that say something: their extents are ones that a call takes.
+int check_query_known(const Arg* args, int n) {
+    for (int i = 0; i < n; ++i) {
+        if (!args[i].b || buf_is_bounds_query(args[i].b)) continue;
+        if (int e = check_extents_nonneg(args[i])) return e;
+        if (int e = check_extent_limit(args[i])) return e;
+    }
+    return 0;
+}
+
 // A device address is a multiple of the element's size (the kernels that take any 16-bit alignment need at least that).
 int check_device_address(const Arg& a) {
     const int bytes = (a.b->type.bits + 7) / 8, off = static_cast<int>(a.b->device % uint64_t(bytes));

@@ -110,6 +110,9 @@ extern "C" int t2sp_b200_grouped_gemm(halide_buffer_t* A, halide_buffer_t* B, ha
     if (int e = check_null(args, 4)) return e;
     const int tb = desc && desc->trans_b ? 1 : 0;
     if (buf_is_bounds_query(A) || buf_is_bounds_query(B) || buf_is_bounds_query(offsets) || buf_is_bounds_query(C)) {
+        if (int e = check_query_known(args, 4)) return e;
+        if (!buf_is_bounds_query(offsets) && offsets->dimensions == 1)
+            if (int e = check_offsets(args[2])) return e;
         int K = 0, M = 0, N = 0, E = 0;
         if (!buf_is_bounds_query(A) && A->dimensions == 2) { K = A->dim[0].extent; M = A->dim[1].extent; }
         if (!buf_is_bounds_query(B) && B->dimensions == 3) {
@@ -186,6 +189,9 @@ extern "C" int t2sp_b200_grouped_gemm_grad(halide_buffer_t* A, halide_buffer_t* 
     Arg args[4] = {{A, "A", false, 2}, {D, "D", false, 2}, {offsets, "offsets", false, 1}, {G, "G", true, 3}};
     if (int e = check_null(args, 4)) return e;
     if (buf_is_bounds_query(A) || buf_is_bounds_query(D) || buf_is_bounds_query(offsets) || buf_is_bounds_query(G)) {
+        if (int e = check_query_known(args, 4)) return e;
+        if (!buf_is_bounds_query(offsets) && offsets->dimensions == 1)
+            if (int e = check_offsets(args[2])) return e;
         int K = 0, M = 0, N = 0, E = 0;
         if (!buf_is_bounds_query(A) && A->dimensions == 2) { K = A->dim[0].extent; M = A->dim[1].extent; }
         if (!buf_is_bounds_query(D) && D->dimensions == 2) { N = D->dim[0].extent; if (!M) M = D->dim[1].extent; }

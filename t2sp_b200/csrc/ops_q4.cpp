@@ -54,21 +54,32 @@ void packed_extents(int N, int K, int E, int group, int* q, int* s) {
     s[0] = 16; s[1] = q4_groups(K, group); s[2] = q4_strips(N); s[3] = E;
 }
 
+// The K and N that a packed matrix holds at the most, within the limit of extents.
+int packed_most(const Arg& q, int* K, int* N) {
+    for (int d = 1; d < 3; ++d) {
+        const int64_t most = int64_t(q.b->dim[d].extent) * (d == 1 ? 64 : 16);
+        if (most > (1 << 30)) return halide_error_buffer_extents_too_large(nullptr, q.name, most, int64_t(1) << 30);
+        *(d == 1 ? K : N) = static_cast<int>(most);
+    }
+    return 0;
+}
+
 // Bounds queries of q4_pack and q4_unpack: the packed shapes from W, or the largest W that the packed shapes hold.
 int query_w_q_s(Arg* args, int w, int q, int s, int tb, int group) {
     halide_buffer_t *W = args[w].b, *Q = args[q].b, *S = args[s].b;
+    if (int e = check_query_known(args, 3)) return e;
     if (buf_is_bounds_query(W)) {
         if (buf_is_bounds_query(Q)) return halide_error_host_is_null(nullptr, args[w].role().c_str());
         if (int e = check_type_dims(args[q], kU8)) return e;
         const uint32_t t = buf_is_bounds_query(S) ? kBF16 : buf_type_word(S);
-        const int N = Q->dim[2].extent * 16, K = Q->dim[1].extent * 64;
+        int N = 0, K = 0;
+        if (int e = packed_most(args[q], &K, &N)) return e;
         const int we[3] = {tb ? K : N, tb ? N : K, Q->dim[3].extent};
         fill_query(W, t, 3, we);
     } else {
         const uint32_t t = buf_type_word(W);
         if (t != kBF16 && t != kF16) return halide_error_bad_type(nullptr, args[w].role().c_str(), t, kBF16);
         if (int e = check_type_dims(args[w], t)) return e;
-        if (int e = check_extents_nonneg(args[w])) return e;
     }
     int qe[4], se[4];
     packed_extents(W->dim[tb ? 1 : 0].extent, W->dim[tb ? 0 : 1].extent, W->dim[2].extent, group, qe, se);
@@ -178,10 +189,14 @@ extern "C" int t2sp_b200_q4_gemv(halide_buffer_t* X, halide_buffer_t* Q, halide_
     if (int e = resolve_group(desc, &group)) return e;
     const bool query_index = index && buf_is_bounds_query(index);
     if (buf_is_bounds_query(X) || buf_is_bounds_query(Q) || buf_is_bounds_query(S) || buf_is_bounds_query(Y) || query_index) {
+        if (int e = check_query_known(args, n_args)) return e;
         // where X or Y does not say K or N, the most that the packed matrices hold
         int K = 0, N = 0, T = 0, R = 0, E = 1;
         uint32_t t = kBF16;
-        if (!buf_is_bounds_query(Q) && Q->dimensions == 4) { K = Q->dim[1].extent * 64; N = Q->dim[2].extent * 16; E = Q->dim[3].extent; }
+        if (!buf_is_bounds_query(Q) && Q->dimensions == 4) {
+            if (int e = packed_most(args[1], &K, &N)) return e;
+            E = Q->dim[3].extent;
+        }
         if (!buf_is_bounds_query(S)) t = buf_type_word(S);
         if (!buf_is_bounds_query(X) && X->dimensions == 2) { t = buf_type_word(X); K = X->dim[0].extent; T = R = X->dim[1].extent; }
         if (index && !query_index && index->dimensions == 1) R = index->dim[0].extent;

@@ -224,3 +224,28 @@ def test_output_strides_of_matrices_that_interlock(lib):
     if no_device():
         assert grad(G=near) == -36
         assert t2sp_b200.q4_unpack(q4_args()["Q"], q4_args()["S"], strided((40, 100, 2), (1, 48, 99 * 48 + 40)), Q4Desc(32, 0)) == -36
+
+
+def test_bounds_queries_refuse_shapes_that_no_call_takes(lib):
+    """Negative extents, extents beyond 2^30 and packed shapes whose matrix would have them give an error, not a shape."""
+    a = q4_args()
+    for extent, code in ((-1, -28), ((1 << 30) + 1, -6)):
+        A = h16(8, 16)
+        A.dims[1].extent = extent
+        assert grouped(A=A, C=Buffer.query(2)) == code and grad(A=A, G=Buffer.query(3)) == code
+        X = h16(3, 100)
+        X.dims[1].extent = extent
+        assert gemv(X=X, Y=Buffer.query(2)) == code
+        W = h16(2, 100, 40)
+        W.dims[0].extent = extent
+        assert t2sp_b200.q4_pack(W, Buffer.query(4), Buffer.query(4), a["desc"]) == code
+        Q = q4_args()["Q"]
+        Q.dims[2].extent = extent
+        assert t2sp_b200.q4_unpack(Q, a["S"], Buffer.query(3), a["desc"]) == code
+        assert gemv(Q=Q, X=Buffer.query(2)) == code
+    for d, n in ((1, 1 << 25), (2, 1 << 28)):   # K or N of 2^31 and 2^32
+        Q = q4_args()["Q"]
+        Q.dims[d].extent = n
+        assert t2sp_b200.q4_unpack(Q, a["S"], Buffer.query(3), a["desc"]) == -6
+        assert gemv(Q=Q, X=Buffer.query(2), Y=Buffer.query(2)) == -6
+    assert grouped(offsets=i32(0), B=Buffer.query(3)) == -8 and grad(offsets=i32(0), G=Buffer.query(3)) == -8
