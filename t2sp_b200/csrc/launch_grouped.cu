@@ -84,7 +84,8 @@ long long count_tiles(int mode, const GroupedParams& p, int tn, int tc, bool mos
 }
 
 // Whether a 16-bit result's contraction (of the gradient: the rows of all groups together) may be longer than a run. (The LONG form of the kernel costs
-// the gradient of 64 groups of 256 rows, 2048 x 1024, 6 % where no group is: 206 -> 218 us.)
+// the gradient of 64 groups of 256 rows, 2048 x 1024, 6 % where no group is: 206 -> 218 us. Where it has the registers of the warps that bring B, it costs
+// 27 groups of 2 rows, 9001 x 1409, f16, 220 -> 261 us.)
 bool is_long(int mode, int out, const GroupedParams& p) { return out != GR_OUT_F32 && (mode == GR_GRAD ? p.rows : p.K) > 64 * grouped_run(out); }
 
 // Which tiles. 256 x 256 by a pair brings an SM 32 KB a k-block, and its two accumulators let one tile drain under the next one's products.
@@ -98,7 +99,10 @@ template <int MODE>
 cudaError_t launch_mode(int out, const GroupedParams& p, const GroupedMaps& maps, cudaStream_t stream) {
     const bool runs = is_long(MODE, out, p);
     if constexpr (MODE != GR_GRAD) {
-        if (p.b_src) return launch_var<MODE, GR_TILE_WARPS>(out, p, maps, count_tiles(MODE, p, 128, 128, true), stream);
+        if (p.b_src) {
+            const long long tiles = count_tiles(MODE, p, 128, 128, true);
+            return runs ? launch_var<MODE, GR_TILE_WARPS, true>(out, p, maps, tiles, stream) : launch_var<MODE, GR_TILE_WARPS>(out, p, maps, tiles, stream);
+        }
         const long long t128 = count_tiles(MODE, p, 128, 128, false);
         const int kb = (p.K + 63) / 64;
         const bool narrow = p.rows <= 32ll * p.E;   // about a tile of 32 columns to a group
@@ -145,7 +149,7 @@ cudaError_t grouped_launch(int mode, int out, const GroupedParams& p, const Grou
 // the warps read B again for every tile (250 rows, 1001 x 2001: 54 against 44), and with few tiles they cannot keep the memory busy while the
 // copy lets a cluster share a tile (2 tiles, K = 5378: 60 against 15).
 bool grouped_warps_worthwhile(int mode, int out, const GroupedParams& p) {
-    if (mode == GR_GRAD || out == GR_OUT_F32 || p.rows == 0 || p.E == 0 || is_long(mode, out, p)) return false;
+    if (mode == GR_GRAD || out == GR_OUT_F32 || p.rows == 0 || p.E == 0) return false;
     const long long groups = p.rows < p.E ? p.rows : p.E;
     return p.rows <= 128 * groups && 3 * count_tiles(mode, p, 128, 128, false) >= 2 * core_sm_count();
 }

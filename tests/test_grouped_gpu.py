@@ -574,3 +574,31 @@ def test_matrices_of_an_output_that_interlock(lib):
     assert torch.equal(torch.from_numpy(host).cuda(), big)
     g.fill_(5.0)
     assert (big == 5).all()
+
+
+@pytest.mark.parametrize("trans", [False, True])
+def test_long_contraction_off_16_bytes_in_a_capture(lib, trans):
+    """B with rows off 16 bytes, read by warps in place: no scratch memory, so the call can be captured, at lengths of several runs too."""
+    import torch
+    E, K, N = 12, 9005, 1099
+    M = 2 * E
+    a, b = positive(1, M, K + 3)[:, :K], positive(2, E, *((N, K) if trans else (K, N)))
+    a = torch.nn.functional.pad(a, (0, 3))[:, :K]       # rows of A start on 16 bytes
+    off = torch.arange(0, M + 1, 2, dtype=torch.int32, device="cuda")
+    c = torch.zeros(M, N, dtype=torch.float16, device="cuda")
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    A, B, O, C = (buf(t) for t in (a, b, off, c))
+    torch.cuda.synchronize()
+    with on_stream(side, asynchronous=True):
+        assert t2sp_b200.grouped_gemm(A, B, O, C, GroupedDesc(int(trans))) == 0
+        side.synchronize()
+        c.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            rc = t2sp_b200.grouped_gemm(A, B, O, C, GroupedDesc(int(trans)))
+    assert rc == 0
+    graph.replay()
+    torch.cuda.synchronize()
+    for e in range(E):
+        ref = a[2 * e:2 * e + 2].double() @ (b[e].T if trans else b[e]).double()
+        assert ((c[2 * e:2 * e + 2].double() - ref).abs() <= long_tolerance(ref)).all(), e
