@@ -364,8 +364,10 @@ struct GemvLayout {
 };
 
 // What an integer sum of a group starts from, beside -8 times the sum of x's bytes: as the bits of a float this is 1.5 * 2^23, and an integer
-// within 2^22 added to the bits is one added to the number, so a subtraction turns the sum into a float.
+// within 2^22 added to the bits is one added to the number, so one multiply-add turns the sum into a float of x's own size (sums in x's integers,
+// scaled back at the end, would leave fp32's range 2^31 before the results do).
 constexpr int kGemvZero = 0x4b400000;
+__device__ __forceinline__ float gemv_power(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }   // 2^e, of a normal number
 
 // The exponent of the largest power of two that keeps a row whose largest magnitude has the bits `top` (finite) within four signed bytes, at most
 // 127 * 16843009 in magnitude: of the 16-bit types' numbers those below 1.9921875 * 2^30. Subnormal numbers are taken for 2^-126, where nothing of a
@@ -373,12 +375,14 @@ constexpr int kGemvZero = 0x4b400000;
 __device__ __forceinline__ int gemv_exponent(uint32_t top) {
     return 30 - max(static_cast<int>(top >> 23) - 127, -126) - ((top & 0x7fffffu) >= 0x7f0000u ? 1 : 0);
 }
-// That power as two factors: the power itself may leave fp32's range.
+// 2 to that exponent as two factors: the power itself may leave fp32's range.
 __device__ __forceinline__ void gemv_scale(uint32_t top, float& f1, float& f2) {
     const int up = gemv_exponent(top), up1 = up >> 1;
     f1 = __uint_as_float(static_cast<uint32_t>(up1 + 127) << 23);
     f2 = __uint_as_float(static_cast<uint32_t>(up - up1 + 127) << 23);
 }
+// The exponent of what a row's integers count on the way to the result, which is scaled by the rest: so that what a sum starts from stays in fp32's range.
+__device__ __forceinline__ int gemv_unit(uint32_t top) { return max(-100, min(-gemv_exponent(top), 86)); }
 // Whether a row holds a value that is no integer times that power, or that is not finite. `low`: the smallest magnitude of the row that is not 0, as the
 // type's bits less one (0xffff: there is none). A value's last bit counts 2^(its exponent - mantissa bits), and less only in smaller values.
 template <class T>
@@ -691,6 +695,14 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
 #pragma unroll
         for (int n = 0; n < NT; ++n)
             xlane[n] = smem_raw + (n * 8 + g < count * S::kPerRow ? n * 8 + g : 0) * lay.pitch + t * (S::kBlockBytes / 4);
+        // INT, of the row whose columns 2 t and 2 t + 1 are: what the lower one's byte counts, and that times what the sums start from
+        float unit_of[NT], zero_of[NT];
+        if constexpr (INT)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                unit_of[n] = gemv_power(gemv_unit(top[n * 2 + (t >> 1)]) + 16 * (t & 1));
+                zero_of[n] = -__int_as_float(kGemvZero) * unit_of[n];
+            }
         float acc[NT][4];
         // the warp's blocks of one slot, kGemvBlocks of them or `nb` at the strip's end
         auto compute = [&](auto full_slot, const uint8_t* blocks, const uint8_t* scales, int kb0, int nb) {
@@ -742,10 +754,10 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             if constexpr (INT) {
-                                acc[n][0] += f.x * (__int_as_float(ci[n][0]) - __int_as_float(kGemvZero));
-                                acc[n][1] += f.x * (__int_as_float(ci[n][1]) - __int_as_float(kGemvZero));
-                                acc[n][2] += f.y * (__int_as_float(ci[n][2]) - __int_as_float(kGemvZero));
-                                acc[n][3] += f.y * (__int_as_float(ci[n][3]) - __int_as_float(kGemvZero));
+                                acc[n][0] += f.x * __fmaf_rn(__int_as_float(ci[n][0]), unit_of[n], zero_of[n]);
+                                acc[n][1] += f.x * __fmaf_rn(__int_as_float(ci[n][1]), unit_of[n], zero_of[n]);
+                                acc[n][2] += f.y * __fmaf_rn(__int_as_float(ci[n][2]), unit_of[n], zero_of[n]);
+                                acc[n][3] += f.y * __fmaf_rn(__int_as_float(ci[n][3]), unit_of[n], zero_of[n]);
                             } else {
                                 acc[n][0] += f.x * c[n][0];
                                 acc[n][1] += f.x * c[n][1];
@@ -789,7 +801,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
                         for (int h = 0; h < 2; ++h) {
                             const float v = acc[n][2 * h] + 256.f * acc[n][2 * h + 1];
                             const float v2 = __shfl_xor_sync(0xffffffffu, v, 1);
-                            if (t % 2 == 0 && !(mixed.value && (wide >> (n * 2 + (t >> 1)) & 1))) mine[(g + 8 * h) * S::kPartPitch + n * 2 + (t >> 1)] = v + 65536.f * v2;
+                            if (t % 2 == 0 && !(mixed.value && (wide >> (n * 2 + (t >> 1)) & 1))) mine[(g + 8 * h) * S::kPartPitch + n * 2 + (t >> 1)] = v + v2;
                         }
                     } else {
 #pragma unroll
@@ -809,11 +821,8 @@ __global__ void __launch_bounds__(kGemvThreads, 1) q4_gemv_kernel(const Q4Params
                     float v = 0.f;
 #pragma unroll 4
                     for (int w = 0; w < gs; ++w) v += from[w * 16 * S::kPartPitch];
-                    if constexpr (INT) {
-                        float f1, f2;
-                        gemv_scale(top[col], f1, f2);
-                        if (!(mixed.value && (wide >> col & 1))) v = v * (1.f / f1) * (1.f / f2);   // powers of two
-                    }
+                    if constexpr (INT)
+                        if (!(mixed.value && (wide >> col & 1))) v *= gemv_power(-gemv_exponent(top[col]) - gemv_unit(top[col]));
                     const int n_at = (strip - (held - 1 - f) * num_groups) * 16 + n;
                     if (n_at < p.N) {
                         const long long at = rows[col] * p.ldy + n_at;

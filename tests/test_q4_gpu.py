@@ -484,3 +484,23 @@ def test_gemv_of_no_k(lib, R, indexed):
         assert t2sp_b200.q4_gemv(X, Q, S, buf(index) if indexed else None, buf(y), Q4Desc(32, 0)) == 0
     left = (index < 0) if indexed else torch.zeros(R, dtype=torch.bool, device="cuda")
     assert (y[left] == 7).all() and not y[~left].any()
+
+
+@pytest.mark.parametrize("R", [1, 2, 4, 8])
+@pytest.mark.parametrize("w_scale,x_scale", [(2.0 ** 122, 2.0 ** -40), (2.0 ** 122, 2.0 ** -120), (2.0 ** 60, 2.0 ** 50), (2.0 ** -110, 2.0 ** 90), (2.0 ** -60, 2.0 ** -60),
+                                             (2.0 ** 100, 2.0 ** -75), (2.0 ** 10, 2.0 ** -126)])
+def test_gemv_ranges_of_w_and_x(lib, R, w_scale, x_scale):
+    """Large matrices times small rows and the other way round, over bf16's range: finite wherever the result is, and as exact as any (sums below
+    fp32's smallest normal number 2^-126 have steps of 2^-149)."""
+    import torch
+    K, N, group = 448, 48, 64
+    w = (matrices(1, K, N, torch.float32, 1).clamp(-8, 8) * w_scale).bfloat16()
+    x = (matrices(1, R, K, torch.float32, 2)[0] * x_scale).bfloat16()
+    assert w.isfinite().all()
+    y = torch.empty(R, N, dtype=torch.float32, device="cuda")
+    with on_stream():
+        Q, S = packed(w, group)
+        assert t2sp_b200.q4_gemv(buf(x), buf(Q), buf(S), None, buf(y), Q4Desc(group, 0)) == 0
+    v, u = x.double(), quantised64(w, group)[0]
+    tol = ((group // 16 + 16) + (K // group + 16)) * 2.0 ** -23 * (v.abs() @ u.abs()) + 2.0 ** -140
+    assert ((y.double() - v @ u).abs() <= tol).all()
