@@ -31,7 +31,7 @@ struct GroupedParams {
     const uint16_t *b_src, *b_end;
     long long b_ld, b_bs;
     long long wait_cycles; // limit of every mbarrier wait in SM cycles, 0: kWaitTimeoutCycles
-    int skip_stage;        // test hook for the bounded waits: the producers leave out the copies of this k-block (1-based; 0 = none)
+    int skip_stage;        // test hook for the bounded waits: the producers leave out the copies from this k-block on (1-based; 0 = none)
     unsigned* status;
 };
 

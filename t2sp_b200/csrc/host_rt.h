@@ -58,7 +58,7 @@ struct Env {
     int pair2 = -1;            // 512-row pair tiles: -1 = choose, 0 / 1 = forced
     unsigned long long fail_alloc_above = 0;  // host-side fault injection: allocations of at least this many bytes fail (0 = off)
     long long wait_cycles = 0;                // bounded-wait limit of the kernels in SM cycles, 0 = default
-    int test_skip_stage = 0;                  // test hook: the producers of the single-CTA and the grouped kernels leave out this k-block's copies
+    int test_skip_stage = 0;                  // test hook: the producers leave out this k-block's copies (the single-CTA kernel), or those from it on
     std::string exec_time_path;               // where exec_time.txt goes, empty = nowhere
 };
 const Env& rt_env();

@@ -419,7 +419,7 @@ def test_grad_of_many_tiles(lib, E):
     ("split", [7], 4096, 128, 3), ("split", [100], 4096, 128, 2), ("single", [600, 400], 512, 512, 3), ("pair", [4000, 96], 512, 1024, 3),
     ("warps", [10] * 20, 515, 1031, 3), ("grad", [700], 512, 256, 3), ("grad", [40], 512, 256, 1)])
 def test_bounded_waits_run_out(lib, name, counts, K, N, skip, out):
-    """Without the copies of one k-block (a test hook) the waits behind it run out after the shortened limit: every kernel returns by
+    """Without the copies from one k-block on (a test hook) the waits behind it run out after the shortened limit: every kernel returns by
     itself, in each of its tile variants, the call reports it, and the next call is right."""
     import torch
     from tests.util import library_env
