@@ -12,9 +12,9 @@ namespace {
 
 // Partial slabs [split][col][row] (dense, `rows` fastest) summed into out[col * ld_out + row]. Four neighbouring
 // lanes share an element: lane part p adds slabs p, p + 4, p + 8, ... in that order, then the four sums are added
-// as (s0 + s1) + (s2 + s3): a fixed order whatever the launch, so the result is reproducible bit for bit.
-__global__ void reduce_partials_kernel(const float* __restrict__ partials, float* __restrict__ out, int rows, int cols,
-                                       long long ld_out, int splits) {
+// as (s0 + s1) + (s2 + s3): a fixed order whatever the launch, so the result is reproducible bit for bit. The slabs are written while this grid is
+// already there, so their pointer must not promise read-only memory (`const __restrict__`), here and in splitk_finalize_kernel.
+__global__ void reduce_partials_kernel(const float* partials, float* out, int rows, int cols, long long ld_out, int splits) {
     const long long elems = static_cast<long long>(rows) * cols;
     const long long tid = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
     const long long idx = tid >> 2;
@@ -102,7 +102,7 @@ __global__ void b_images_kernel(const BImageParams q, uint8_t* __restrict__ dst)
 }
 
 // One thread per row and four consecutive columns; the sum over the slabs runs in slab order.
-__global__ void splitk_finalize_kernel(const float* __restrict__ part, long long ld_part, long long slab_elems, int splits,
+__global__ void splitk_finalize_kernel(const float* part, long long ld_part, long long slab_elems, int splits,
                                        const __grid_constant__ CoreParams f) {
     const int quads = (f.N + 3) >> 2;
     const long long idx = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
