@@ -155,7 +155,7 @@ __device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t v) {   // of e
 }
 
 // v / scale rounded to the nearest integer, ties to even, plus kNibble0, as the bits of a float: the integer is in the last bits. `inv` = 1 / scale,
-// or 0 for a scale of 0. v * inv is off the quotient by less than 2^-20, and a quotient that is no tie is at
+// or 0 for a scale of 0. v * inv is off the quotient by less than 2^-19, and a quotient that is no tie is at
 // least 2^-12 away from one: v and scale are integers a, b < 2^11 times powers of two, |v / scale - (h + 1/2)| = |2 v - (2 h + 1) scale| / (2
 // scale), and the numerator is a multiple of the scale's last bit. So the product rounded to a multiple of 2^-14 (by the first sum, whose last
 // bit that is) is a tie exactly where the quotient is one. A normal scale is at least (1 - 2^-8) max / 7, so the integer is within

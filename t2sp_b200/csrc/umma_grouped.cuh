@@ -713,8 +713,8 @@ grouped_kernel(const __grid_constant__ GroupedParams p, const __grid_constant__ 
 // ---------------------------------------------------------------- few tiles: the contraction split over a cluster
 // Forward products of a few rows, or with a few columns, have fewer 128 x 128 tiles than the GPU has SMs, and one SM brings weights at 60 to 80 GB/s
 // only. Here a cluster of `splits` CTAs shares a tile: each adds up its run of k-blocks, hands the fp32 sums of 32 n x 32 columns to the CTA that owns
-// them through distributed shared memory, and the owners add the parts in the order of the ranks and write the results. (8 groups of
-// 2 rows, 1024 x 1024, 64 tiles: two CTAs a tile.) Tiles of 32 columns for groups of a few rows leave room for twice the blocks in flight.
+// them through distributed shared memory, and the owners add the parts in the order of the ranks and write the results. (64 rows, 16384 x 4096, 32
+// tiles: four CTAs a tile, 36 us.) Tiles of 32 columns for groups of a few rows leave room for twice the blocks in flight.
 template <int VAR>
 struct SplitCfg {
     static constexpr int kTileC = VAR == GR_TILE_32 ? 32 : 128;
